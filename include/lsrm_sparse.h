@@ -51,6 +51,10 @@ extern "C" {
 
 #define LSRM_DTYPE_F16 0
 #define LSRM_DTYPE_BF16 1
+/* only where an entry point names them */
+#define LSRM_DTYPE_F32 2
+#define LSRM_DTYPE_E4M3 3
+#define LSRM_DTYPE_INT8 4
 
 /* Variable-length metadata shared by the attention entry points (device
  * pointers, int32).  Mirrors the arguments of native_sparse_attend
@@ -463,6 +467,103 @@ int lsrm_qkv_norm_fwd(int64_t M, int32_t K, int32_t N, int32_t head_dim, const v
                       float* rstd, int* err_flags, void* stream);
 int lsrm_qkv_norm_bwd(int64_t M, int32_t N, int32_t head_dim, const lsrm_qkv_grad_segment* segs, int32_t n_segs,
                       const float* rstd, void* grad_pre, void* stream);
+
+/* ---------------------------------------------------------------------- */
+/* Attention with a sliding window and sinks (no reference counterpart)     */
+/* ---------------------------------------------------------------------- */
+/* Packed sequences, q [total_q, Hq, D], k / v [total_k, Hkv, D] (token
+ * strides given, multiples of 8 elements; contiguous heads).  Sequence b has
+ * queries [cu_seqlens_q[b], cu_seqlens_q[b+1]) and keys [cu_seqlens_k[b],
+ * cu_seqlens_k[b+1]); query i stands at position pos = i + Lk - Lq and sees
+ * key j when
+ *   causal:    j <= pos and (pos - j < window or j < sinks)
+ *   otherwise: |pos - j| <= window / 2 or j < sinks.
+ * A query that sees no key gets o = 0 and lse = -inf, and its gradients are
+ * zero; so do tokens after the last sequence, whose contents are not used.
+ * Offsets that leave the tensors set LSRM_ERR_BAD_INDEX in err_flags. */
+typedef struct lsrm_window_shape {
+  int32_t num_seqs, total_q, total_k;
+  int32_t num_q_heads;  /* Hq, a multiple of Hkv, at most 64 times as many */
+  int32_t num_kv_heads;
+  int32_t head_dim;     /* 32, 64 or 128 */
+  int32_t dtype;        /* bf16 or fp16 */
+  int32_t window;       /* >= 1 */
+  int32_t sinks;        /* 0..128 */
+  int32_t causal;
+  int64_t q_token_stride, k_token_stride, v_token_stride;
+  float softmax_scale;  /* <= 0 selects 1/sqrt(D) */
+} lsrm_window_shape;
+
+/* out [total_q, Hq, D], lse [total_q, Hq] fp32 (natural log). */
+int lsrm_window_attn_fwd(const lsrm_window_shape* shape, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                         const void* q, const void* k, const void* v, void* out, float* lse, int* err_flags,
+                         void* stream);
+/* dout, dq [total_q, Hq, D], dk, dv [total_k, Hkv, D], contiguous; sums are
+ * taken in a fixed order. */
+size_t lsrm_window_attn_workspace_bytes(const lsrm_window_shape* shape);
+int lsrm_window_attn_bwd(const lsrm_window_shape* shape, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                         const void* q, const void* k, const void* v, const void* out, const float* lse,
+                         const void* dout, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                         int* err_flags, void* stream);
+
+/* The causal form for one new token a sequence, over a ring cache [batch,
+ * capacity, Hkv, D] (strides in elements, multiples of 8).  Sequence b holds
+ * lengths[b] tokens; the new one takes that position.  Position j is kept in
+ * slot j while j < sinks, else in slot sinks + (j - sinks) % (capacity -
+ * sinks), so a cache that never fills is a plain one.  The call writes k_new
+ * and v_new [batch, Hkv, D] to their slots and attends to the first `sinks`
+ * positions and the last `window` ones (the new token's included); slots that
+ * no position fills are not read into any result.  lengths[b] < 0: an idle
+ * row, out = 0, nothing written.  out [batch, Hq, D] contiguous. */
+typedef struct lsrm_window_decode_shape {
+  int32_t batch;
+  int32_t num_q_heads, num_kv_heads, head_dim, dtype; /* as lsrm_window_shape */
+  int32_t capacity;                                   /* >= sinks + window */
+  int32_t window, sinks;
+  int64_t q_stride, k_new_stride, v_new_stride;       /* between sequences */
+  int64_t k_batch_stride, k_slot_stride, v_batch_stride, v_slot_stride;
+  float softmax_scale;                                /* <= 0 selects 1/sqrt(D) */
+} lsrm_window_decode_shape;
+int lsrm_window_decode(const lsrm_window_decode_shape* shape, const void* q, const void* k_new, const void* v_new,
+                       void* k_cache, void* v_cache, const int32_t* lengths, void* out, void* stream);
+
+/* ---------------------------------------------------------------------- */
+/* Residual RMS norm and counter-based dropout (no reference counterpart)   */
+/* ---------------------------------------------------------------------- */
+/* Dropout without a stored mask: element e of the flat tensor draws word
+ * e % 4 of the Philox4x32-10 block with counter offset + e / 4 and key `seed`;
+ * it is kept, times 1 / (1 - p), when the word is >= floor(p * 2^32), else it
+ * is 0 (whatever x holds).  p in [0, 1); dtype bf16, fp16 or fp32; x and y
+ * 16-byte aligned.  The gradient is the same call on the output's gradient. */
+int lsrm_dropout(int64_t n, int32_t dtype, double p, uint64_t seed, uint64_t offset, const void* x, void* y,
+                 void* stream);
+
+/* h = residual + dropout(x); y = h / sqrt(mean_c(h^2) + eps) * weight over
+ * rows of `cols` (1..16384) elements, contiguous and 16-byte aligned.  x, y:
+ * `dtype` (bf16 / fp16); residual, h: `stream_dtype` (the same or fp32);
+ * weight: `weight_dtype` (the same or fp32).  residual, weight and rstd may
+ * be NULL; rstd [rows] fp32 is what the backward needs. */
+int lsrm_residual_rms_norm_fwd(int64_t rows, int32_t cols, int32_t dtype, int32_t stream_dtype, int32_t weight_dtype,
+                               float eps, double p, uint64_t seed, uint64_t offset, const void* x,
+                               const void* residual, const void* weight, void* y, void* h, float* rstd, void* stream);
+/* From the gradients dy of y and dh of h (may be NULL): dresidual
+ * (stream_dtype), dx (dtype; may be NULL where it equals dresidual: p = 0 and
+ * one type) and dweight (weight_dtype; may be NULL). */
+size_t lsrm_residual_rms_norm_workspace_bytes(int64_t rows, int32_t cols);
+int lsrm_residual_rms_norm_bwd(int64_t rows, int32_t cols, int32_t dtype, int32_t stream_dtype, int32_t weight_dtype,
+                               double p, uint64_t seed, uint64_t offset, const void* h, const float* rstd,
+                               const void* weight, const void* dy, const void* dh, void* dx, void* dresidual,
+                               void* dweight, void* workspace, size_t workspace_bytes, void* stream);
+/* The forward with y in 8 bits (e4m3 or int8) and fp32 scales [rows,
+ * ceil(cols / group)] per `group` columns (32, 64, 128; 0: one per row):
+ * scale = max|y| / 448 (e4m3) or / 127 (int8), 1 for zeros; values =
+ * y / scale rounded to nearest even. */
+int lsrm_residual_rms_norm_8bit(int64_t rows, int32_t cols, int32_t dtype, int32_t stream_dtype, int32_t weight_dtype,
+                                float eps, int32_t out_dtype, int32_t group, const void* x, const void* residual,
+                                const void* weight, void* values, float* scales, void* h, void* stream);
+/* y = values * scale, in bf16, fp16 or fp32. */
+int lsrm_dequantize_8bit(int64_t rows, int32_t cols, int32_t in_dtype, int32_t out_dtype, int32_t group,
+                         const void* values, const float* scales, void* y, void* stream);
 
 /* ---------------------------------------------------------------------- */
 /* Self-test of the tcgen05 / TMA building blocks (used by the GPU tests)   */

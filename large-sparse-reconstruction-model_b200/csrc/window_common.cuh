@@ -1,0 +1,96 @@
+// What the windowed attention kernels share: which keys a query sees.
+//
+// Query i of a sequence with Lq queries and Lk keys stands at position
+// pos = i + Lk - Lq.  It sees key j (0 <= j < Lk) when
+//   causal:     j <= pos and (pos - j < window or j < sinks)
+//   symmetric:  |pos - j| <= window / 2 or j < sinks.
+#pragma once
+
+#include <cstdint>
+
+#include "lsrm_sparse.h"
+
+namespace lsrm {
+
+struct WindowParams {
+  int num_seqs, total_q, total_k;
+  int hq, hkv, g;        // query heads, kv heads, query heads per kv head
+  int left, right;       // the window's reach on both sides of pos
+  int sinks, causal;
+  float scale;           // softmax scale
+  const int32_t *cu_q, *cu_k;
+  long long q_stride, k_stride, v_stride;  // elements between tokens
+  const void *q, *k, *v;
+  void* out;
+  float* lse;            // [total_q, hq], natural log
+  int* err;
+};
+
+// One sequence's tokens.  Index num_seqs stands for the tokens after the last
+// sequence, which see and are seen by nothing (their outputs are zero).
+struct Seq {
+  int q0, lq, k0, lk;
+};
+
+__device__ __forceinline__ Seq seq_of(const WindowParams& p, int b) {
+  const bool tail = b >= p.num_seqs;
+  int q0 = p.cu_q[b], k0 = p.cu_k[b];
+  int q1 = tail ? p.total_q : p.cu_q[b + 1], k1 = tail ? p.total_k : p.cu_k[b + 1];
+  // offsets outside the tensors or out of order: report and touch nothing
+  if (q0 < 0 || q1 < q0 || q1 > p.total_q || k0 < 0 || k1 < k0 || k1 > p.total_k) {
+    if (p.err) atomicOr(p.err, LSRM_ERR_BAD_INDEX);
+    return Seq{0, 0, 0, 0};
+  }
+  return Seq{q0, q1 - q0, k0, k1 - k0};
+}
+
+// Keys that a query at `pos` sees: [lo, hi) and [0, sink) (sink <= lo, so the
+// two never overlap).
+struct Seen {
+  int sink, lo, hi;
+};
+
+__device__ __forceinline__ Seen keys_of(const WindowParams& p, int pos, int lk, bool live) {
+  Seen s;
+  s.lo = max(0, pos - p.left);
+  s.hi = min(lk, pos + p.right + 1);
+  s.sink = min(min(p.sinks, p.causal ? pos + 1 : lk), lk);
+  if (!live || s.hi < 0) s.hi = 0;
+  if (!live || s.sink < 0) s.sink = 0;
+  if (s.hi <= s.lo) s.lo = s.hi = max(s.sink, 0);
+  if (s.sink >= s.lo) {  // the window reaches into the sinks: one range
+    s.hi = max(s.hi, s.sink);
+    s.lo = 0;
+    s.sink = 0;
+  }
+  return s;
+}
+
+// Tiles of `rows` tokens of ragged sequences: sequence b's tiles start at slot
+// cu[b] / rows + b, which leaves each sequence at least as many slots as it
+// has tiles; total / rows + num_seqs + 1 slots cover all, the tail's included.
+__host__ __device__ __forceinline__ int tile_slots(int total, int num_seqs, int rows) {
+  return total / rows + num_seqs + 1;
+}
+
+__device__ __forceinline__ int seq_of_slot(const int32_t* cu, int num_seqs, int rows, int slot) {
+  int lo = 0, hi = num_seqs;  // the last sequence whose first slot is <= slot
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (cu[mid] / rows + mid <= slot) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int seq_of_token(const int32_t* cu, int num_seqs, int token) {
+  int lo = 0, hi = num_seqs;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (cu[mid] <= token) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+}  // namespace lsrm

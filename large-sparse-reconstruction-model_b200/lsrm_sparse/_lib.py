@@ -63,6 +63,20 @@ class QkvGradSegment(ctypes.Structure):
                 ("grad_norm", c_void_p)]
 
 
+class WindowShape(ctypes.Structure):
+    _fields_ = [(n, c_int32) for n in ("num_seqs", "total_q", "total_k", "num_q_heads", "num_kv_heads", "head_dim",
+                                       "dtype", "window", "sinks", "causal")] + [
+        ("q_token_stride", c_int64), ("k_token_stride", c_int64), ("v_token_stride", c_int64),
+        ("softmax_scale", c_float)]
+
+
+class WindowDecodeShape(ctypes.Structure):
+    _fields_ = [(n, c_int32) for n in ("batch", "num_q_heads", "num_kv_heads", "head_dim", "dtype", "capacity",
+                                       "window", "sinks")] + [
+        (n, c_int64) for n in ("q_stride", "k_new_stride", "v_new_stride", "k_batch_stride", "k_slot_stride",
+                               "v_batch_stride", "v_slot_stride")] + [("softmax_scale", c_float)]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     "lsrm_abi_version": (c_int, []),
@@ -174,6 +188,34 @@ _SIGS = {
                 ctypes.c_float, c_void_p, c_void_p, c_void_p]
     ),
     "lsrm_qkv_norm_bwd": (c_int, [c_int64, c_int32, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p]),
+    "lsrm_window_attn_fwd": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
+    ),
+    "lsrm_window_attn_workspace_bytes": (c_size_t, [c_void_p]),
+    "lsrm_window_attn_bwd": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]
+    ),
+    "lsrm_window_decode": (
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
+    ),
+    "lsrm_dropout": (c_int, [c_int64, c_int32, ctypes.c_double, c_uint64, c_uint64, c_void_p, c_void_p, c_void_p]),
+    "lsrm_residual_rms_norm_fwd": (
+        c_int, [c_int64, c_int32, c_int32, c_int32, c_int32, c_float, ctypes.c_double, c_uint64, c_uint64, c_void_p,
+                c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
+    ),
+    "lsrm_residual_rms_norm_workspace_bytes": (c_size_t, [c_int64, c_int32]),
+    "lsrm_residual_rms_norm_bwd": (
+        c_int, [c_int64, c_int32, c_int32, c_int32, c_int32, ctypes.c_double, c_uint64, c_uint64, c_void_p, c_void_p,
+                c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]
+    ),
+    "lsrm_residual_rms_norm_8bit": (
+        c_int, [c_int64, c_int32, c_int32, c_int32, c_int32, c_float, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
+                c_void_p, c_void_p, c_void_p, c_void_p]
+    ),
+    "lsrm_dequantize_8bit": (
+        c_int, [c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p]
+    ),
     "lsrm_umma_selftest": (
         c_int, [c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
     ),

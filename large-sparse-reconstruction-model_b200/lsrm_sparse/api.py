@@ -111,3 +111,86 @@ def compressed_attention(q, compressed_k, compressed_v, cu_seqlens_q, compressed
     out, lse = F.dense_attention(q.contiguous(), compressed_k.contiguous(), compressed_v.contiguous(), meta,
                                  ops.DENSE_COMPRESSED, 0, softmax_scale)
     return (out, lse) if return_lse else out
+
+
+# ---------------------------------------------------------------------------
+# A decoder layer's other operators (extensions: no reference counterpart)
+# ---------------------------------------------------------------------------
+
+
+def window_sink_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, window: int, sinks: int = 0,
+                          causal: bool = True, softmax_scale: Optional[float] = None, return_lse: bool = False):
+    """Attention with a sliding window and a few first tokens that stay
+    visible, over packed sequences: q [Nq, Hq, D], k / v [Nk, Hkv, D] (bf16 /
+    fp16; D 32, 64 or 128; Hq a multiple of Hkv), int32 offsets [sequences + 1]
+    (``cu_seqlens_k`` defaults to ``cu_seqlens_q``).  Query i of a sequence
+    stands at position i + Lk - Lq and sees key j when
+
+    * causal:    j <= pos and (pos - j < window or j < sinks)
+    * symmetric: |pos - j| <= window // 2 or j < sinks (``sliding_window_attention``'s
+      band, with sinks)
+
+    A query that sees nothing gives 0.  Differentiable in q, k and v.  With
+    ``return_lse`` also the natural-log LSE [Hq, Nq] fp32."""
+    cu_k = cu_seqlens_q if cu_seqlens_k is None else cu_seqlens_k
+    out, lse = F.window_sink_attention(q, k, v, cu_seqlens_q, cu_k, window, sinks, causal, softmax_scale)
+    _raise_on_device_errors()
+    return (out, lse.t()) if return_lse else out
+
+
+def window_sink_decode(q, k_new, v_new, k_cache, v_cache, lengths, *, window: int, sinks: int = 0,
+                       softmax_scale: Optional[float] = None):
+    """The causal form for one new token of each sequence over a ring cache:
+    q [B, Hq, D], k_new / v_new [B, Hkv, D], caches [B, capacity, Hkv, D] with
+    capacity >= sinks + window, lengths [B] int32 (tokens before the new one;
+    negative: an idle row).  Writes the new key and value to their slot (position
+    j lives in slot j below ``sinks``, else in sinks + (j - sinks) % (capacity -
+    sinks)) and returns the attention's output [B, Hq, D].  ``lengths`` is not
+    advanced.  Not differentiable."""
+    with torch.no_grad():
+        return ops.window_decode(q, k_new, v_new, k_cache, v_cache, lengths, window, sinks, softmax_scale)
+
+
+def dropout(x, p: float, seed: int, offset: int = 0):
+    """Dropout whose mask is a function of (seed, offset, element index) and is
+    never stored: the backward, or a second call, regenerates it.  Element e
+    draws word e % 4 of the Philox4x32-10 block ``offset + e // 4``, so calls that
+    must differ take other seeds, or offsets that are numel / 4 apart.  p in [0, 1)."""
+    if not 0.0 <= p < 1.0:
+        raise ValueError(f"dropout: p ({p}) must be in [0, 1)")
+    return F.dropout(x, float(p), seed, offset)
+
+
+def residual_rms_norm(x, residual=None, weight=None, *, eps: float = 1e-6, p: float = 0.0, seed: int = 0,
+                      offset: int = 0):
+    """The step between a block's branches: h = residual + dropout(x) and
+    y = h / sqrt(mean(h**2) + eps) * weight over the last dimension.  Returns
+    (y, h): y in x's dtype, h in the residual's (x's or fp32).  Differentiable in
+    x, residual and weight; the dropout is ``dropout``'s, with its mask."""
+    if not 0.0 <= p < 1.0:
+        raise ValueError(f"residual_rms_norm: p ({p}) must be in [0, 1)")
+    return F.residual_rms_norm(x, residual, weight, float(eps), float(p), seed, offset)
+
+
+def residual_rms_norm_8bit(x, residual=None, weight=None, *, eps: float = 1e-6, dtype=torch.float8_e4m3fn,
+                           group: int = 0):
+    """``residual_rms_norm`` (without dropout) with y in 8 bits: returns
+    (values, scales, h).  ``dtype`` is float8_e4m3fn or int8; one fp32 scale per
+    row, or per ``group`` (32, 64, 128) columns; y ~ values * scale.  Not
+    differentiable."""
+    if group not in (0, 32, 64, 128):
+        raise ValueError(f"residual_rms_norm_8bit: group ({group}) must be 0, 32, 64 or 128")
+    with torch.no_grad():
+        return ops.residual_rms_norm_8bit(x, residual, weight, eps, dtype, group)
+
+
+def dequantize_8bit(values, scales, dtype=torch.bfloat16):
+    """values * scale of ``residual_rms_norm_8bit``, in ``dtype``."""
+    groups, c = scales.shape[-1], values.shape[-1]
+    if scales.shape[:-1] != values.shape[:-1]:
+        raise ValueError(f"dequantize_8bit: scales {tuple(scales.shape)} do not go with values {tuple(values.shape)}")
+    group = 0 if groups == 1 else next((g for g in (32, 64, 128) if -(-c // g) == groups), None)
+    if group is None:
+        raise ValueError(f"dequantize_8bit: {groups} scales do not divide {c} columns")
+    with torch.no_grad():
+        return ops.dequantize_8bit(values, scales, dtype, group)

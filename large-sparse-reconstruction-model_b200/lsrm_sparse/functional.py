@@ -228,3 +228,87 @@ def qkv_norm(x, linears, outputs, head_dim: int, eps: float = 1e-5):
         n = next(flat).reshape(*lead, cols) if norm else None
         res.append((r, n))
     return res
+
+
+class WindowSinkAttnFn(torch.autograd.Function):
+    """Windowed attention with sinks (lsrm_window_attn_fwd / _bwd)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, window, sinks, causal, scale):
+        out, lse = ops.window_attn_fwd(q, k, v, cu_q, cu_k, window, sinks, causal, scale)
+        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
+        ctx.args = (window, sinks, causal, scale)
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, _dlse):
+        q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
+        dq, dk, dv = ops.window_attn_bwd(q, k, v, out, lse, dout, cu_q, cu_k, *ctx.args)
+        return dq, dk, dv, None, None, None, None, None, None
+
+
+class DropoutFn(torch.autograd.Function):
+    """Counter-based dropout; the backward regenerates the mask."""
+
+    @staticmethod
+    def forward(ctx, x, p, seed, offset):
+        ctx.args = (p, seed, offset)
+        return ops.dropout(x, p, seed, offset)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        return ops.dropout(dy, *ctx.args), None, None, None
+
+
+class ResidualRmsNormFn(torch.autograd.Function):
+    """(y, h) of lsrm_residual_rms_norm_fwd; the backward keeps h and 1/rms."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps, p, seed, offset):
+        y, h, rstd = ops.residual_rms_norm_fwd(x, residual, weight, eps, p, seed, offset)
+        ctx.save_for_backward(h, rstd, weight)
+        ctx.args = (p, seed, offset)
+        ctx.has_residual = residual is not None
+        ctx.set_materialize_grads(False)
+        return y, h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh):
+        h, rstd, weight = ctx.saved_tensors
+        p, seed, offset = ctx.args
+        if dy is None:  # only the stream was used
+            if dh is None:
+                return (None,) * 7
+            dx = ops.dropout(dh, p, seed, offset) if p else dh
+            dw = torch.zeros_like(weight) if weight is not None and ctx.needs_input_grad[2] else None
+            return dx, dh if ctx.has_residual else None, dw, None, None, None, None
+        dx, dres, dw = ops.residual_rms_norm_bwd(h, rstd, weight, dy, dh, p, seed, offset, ctx.needs_input_grad[2])
+        return dx, dres if ctx.has_residual else None, dw, None, None, None, None
+
+
+def _grad_needed(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def window_sink_attention(q, k, v, cu_seqlens_q, cu_seqlens_k, window, sinks, causal, softmax_scale=None):
+    """(out, lse [Nq, Hq])."""
+    args = (q, k, v, cu_seqlens_q, cu_seqlens_k, int(window), int(sinks), bool(causal), softmax_scale)
+    ops.check_window_attn(*args[:7])
+    return WindowSinkAttnFn.apply(*args) if _grad_needed(q, k, v) else ops.window_attn_fwd(*args)
+
+
+def dropout(x, p, seed, offset=0):
+    if p == 0.0:
+        return x
+    return DropoutFn.apply(x, p, seed, offset) if _grad_needed(x) else ops.dropout(x, p, seed, offset)
+
+
+def residual_rms_norm(x, residual=None, weight=None, eps=1e-6, p=0.0, seed=0, offset=0):
+    """(y, h)."""
+    if _grad_needed(x, residual, weight):
+        return ResidualRmsNormFn.apply(x, residual, weight, eps, p, seed, offset)
+    return ops.residual_rms_norm_fwd(x, residual, weight, eps, p, seed, offset, need_rstd=False)[:2]

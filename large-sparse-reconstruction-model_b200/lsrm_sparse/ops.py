@@ -446,3 +446,230 @@ def qkv_norm_bwd(M: int, N: int, head_dim: int, segments, rstd: torch.Tensor, de
     rc = L.lsrm_qkv_norm_bwd(M, N, int(head_dim), segs, len(segments), _ptr(rstd), _ptr(out), _stream())
     check(rc, "lsrm_qkv_norm_bwd")
     return out
+
+
+# ---------------------------------------------------------------------------
+# Windowed attention with sinks, residual RMS norm, counter-based dropout
+# ---------------------------------------------------------------------------
+
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2, torch.float8_e4m3fn: 3, torch.int8: 4}
+
+
+def _need(cond: bool, msg: str):
+    if not cond:
+        raise ValueError(msg)
+
+
+def _cuda(name: str, *ts):
+    """All tensors (None passes) on one CUDA device, which is returned."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        _need(t.is_cuda, f"{name}: tensors must be on a CUDA device, got {t.device}")
+        _need(dev is None or t.device == dev, f"{name}: tensors are on {dev} and {t.device}")
+        dev = t.device
+    return dev
+
+
+def _run(dev: torch.device, name: str, *args):
+    """Call the entry point ``name`` on the current stream of ``dev``."""
+    fn = getattr(_lib.lib(), name)
+    if dev.index == torch.cuda.current_device():
+        check(fn(*args, torch.cuda.current_stream().cuda_stream), name)
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, torch.cuda.current_stream().cuda_stream), name)
+
+
+def _flat(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """Contiguous and 16-byte aligned (a copy for any other layout)."""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _token_rows(t: torch.Tensor):
+    """[..., heads, head_dim] with contiguous heads in aligned rows, as is or
+    copied, and the row stride (the stride of the dimension before the heads)."""
+    h, d = t.shape[-2:]
+    n, lead = t.shape[-3], t.stride(-3)
+    ok = (t.stride(-1) == 1 or d == 1) and (h == 1 or t.stride(-2) == d) and t.data_ptr() % 16 == 0
+    if ok and n <= 1:
+        return t, h * d
+    if ok and lead >= h * d and lead % 8 == 0:
+        return t, lead
+    return _flat(t), h * d
+
+
+def _window_shape(q, k, v, cu_q, window, sinks, causal, scale):
+    q, qs = _token_rows(q)
+    k, ks = _token_rows(k)
+    v, vs = _token_rows(v)
+    sh = _lib.WindowShape(cu_q.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2],
+                          _dtype_code(q), min(int(window), 2**31 - 1), int(sinks), int(bool(causal)), qs, ks, vs,
+                          float(scale) if scale else 0.0)
+    return sh, q, k, v
+
+
+def check_window_attn(q, k, v, cu_seqlens_q, cu_seqlens_k, window, sinks):
+    name = "window_sink_attention"
+    _cuda(name, q, k, v, cu_seqlens_q, cu_seqlens_k)
+    _need(q.dim() == k.dim() == v.dim() == 3, f"{name}: q, k and v must be [tokens, heads, head_dim]")
+    _need(k.shape == v.shape and q.shape[2] == k.shape[2],
+          f"{name}: shapes {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)} do not go together")
+    _need(q.dtype == k.dtype == v.dtype, f"{name}: q, k and v must have one dtype")
+    for t in (cu_seqlens_q, cu_seqlens_k):
+        _need(t.dim() == 1 and t.numel() >= 1 and t.dtype == torch.int32,
+              f"{name}: cu_seqlens must be int32 [sequences + 1]")
+    _need(cu_seqlens_q.numel() == cu_seqlens_k.numel(), f"{name}: cu_seqlens_q and cu_seqlens_k differ in length")
+    _need(int(window) >= 1, f"{name}: window ({window}) must be at least 1")
+    _need(int(sinks) >= 0, f"{name}: sinks ({sinks}) must not be negative")
+
+
+def window_attn_fwd(q, k, v, cu_q, cu_k, window: int, sinks: int, causal: bool, softmax_scale=None):
+    """Returns (out [Nq, Hq, D], lse [Nq, Hq] fp32, natural log)."""
+    sh, q, k, v = _window_shape(q, k, v, cu_q, window, sinks, causal, softmax_scale)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(q.shape[0], q.shape[1], dtype=torch.float32, device=q.device)
+    cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
+    _run(q.device, "lsrm_window_attn_fwd", ctypes.byref(sh), _addr(cu_q), _addr(cu_k), _addr(q), _addr(k), _addr(v),
+         _addr(out), _addr(lse), _addr(_err_word(q.device)))
+    return out, lse
+
+
+def window_attn_bwd(q, k, v, out, lse, dout, cu_q, cu_k, window: int, sinks: int, causal: bool, softmax_scale=None):
+    """Returns (dq, dk, dv)."""
+    sh, q, k, v = _window_shape(q, k, v, cu_q, window, sinks, causal, softmax_scale)
+    dout = _flat(dout)
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    dv = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
+    ws = _workspace(_lib.lib().lsrm_window_attn_workspace_bytes(ctypes.byref(sh)), q.device)
+    _run(q.device, "lsrm_window_attn_bwd", ctypes.byref(sh), _addr(cu_q), _addr(cu_k), _addr(q), _addr(k), _addr(v),
+         _addr(out), _addr(lse), _addr(dout), _addr(dq), _addr(dk), _addr(dv), _addr(ws), ws.numel(),
+         _addr(_err_word(q.device)))
+    return dq, dk, dv
+
+
+def window_decode(q, k_new, v_new, k_cache, v_cache, lengths, window: int, sinks: int, softmax_scale=None):
+    """One token a sequence over a ring cache, which is updated in place.
+    q [B, Hq, D], k_new / v_new [B, Hkv, D], caches [B, capacity, Hkv, D],
+    lengths [B] int32.  Returns out [B, Hq, D]."""
+    name = "window_sink_decode"
+    dev = _cuda(name, q, k_new, v_new, k_cache, v_cache, lengths)
+    _need(q.dim() == 3 and k_new.dim() == 3 and k_cache.dim() == 4,
+          f"{name}: q and k_new must be [batch, heads, head_dim], the caches [batch, capacity, heads, head_dim]")
+    b, hkv, d = k_new.shape
+    _need(k_new.shape == v_new.shape and k_cache.shape == v_cache.shape and q.shape[0] == b and q.shape[2] == d
+          and (k_cache.shape[0], *k_cache.shape[2:]) == (b, hkv, d),
+          f"{name}: shapes {tuple(q.shape)}, {tuple(k_new.shape)} and {tuple(k_cache.shape)} do not go together")
+    _need(q.dtype == k_new.dtype == v_new.dtype == k_cache.dtype == v_cache.dtype, f"{name}: tensors must have one dtype")
+    _need(lengths.dtype == torch.int32 and tuple(lengths.shape) == (b,), f"{name}: lengths must be int32 [batch]")
+    for c in (k_cache, v_cache):  # written in place: no copy may stand in
+        _need(c.stride(3) == 1 and (hkv == 1 or c.stride(2) == d) and c.stride(1) % 8 == 0 and c.stride(0) % 8 == 0
+              and c.stride(1) >= hkv * d and (b == 1 or c.stride(0) >= hkv * d) and c.data_ptr() % 16 == 0,
+              f"{name}: the caches need contiguous heads and strides of 8 elements, aligned to 16 bytes")
+    (q, qs), (k_new, ks), (v_new, vs) = _token_rows(q), _token_rows(k_new), _token_rows(v_new)
+    lengths = lengths.contiguous()
+    sh = _lib.WindowDecodeShape(b, q.shape[1], hkv, d, _dtype_code(q), k_cache.shape[1], min(int(window), 2**31 - 1),
+                                int(sinks), qs, ks, vs, k_cache.stride(0), k_cache.stride(1), v_cache.stride(0),
+                                v_cache.stride(1), float(softmax_scale) if softmax_scale else 0.0)
+    out = torch.empty(b, q.shape[1], d, dtype=q.dtype, device=dev)
+    _run(dev, "lsrm_window_decode", ctypes.byref(sh), _addr(q), _addr(k_new), _addr(v_new), _addr(k_cache),
+         _addr(v_cache), _addr(lengths), _addr(out))
+    return out
+
+
+def _seed(v: int) -> int:
+    return int(v) & (2**64 - 1)
+
+
+def dropout(x: torch.Tensor, p: float, seed: int, offset: int = 0) -> torch.Tensor:
+    """x / (1 - p) where the counter-based generator keeps the element, else 0."""
+    dev = _cuda("dropout", x)
+    _need(x.dtype in (torch.bfloat16, torch.float16, torch.float32), f"dropout: dtype {x.dtype} is not supported")
+    x = _flat(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    _run(dev, "lsrm_dropout", x.numel(), _DTYPES[x.dtype], float(p), _seed(seed), _seed(offset), _addr(x), _addr(y))
+    return y
+
+
+def _check_norm(name, x, residual, weight):
+    dev = _cuda(name, x, residual, weight)
+    _need(x.dim() >= 1, f"{name}: x must have at least one dimension")
+    stream = x.dtype if residual is None else residual.dtype
+    _need(x.dtype in (torch.bfloat16, torch.float16), f"{name}: x must be bf16 or fp16, got {x.dtype}")
+    _need(stream in (x.dtype, torch.float32), f"{name}: the residual must have x's dtype or fp32, got {stream}")
+    _need(residual is None or residual.shape == x.shape, f"{name}: the residual must have x's shape")
+    _need(weight is None or (tuple(weight.shape) == tuple(x.shape[-1:]) and weight.dtype in (x.dtype, torch.float32)),
+          f"{name}: the weight must be [{x.shape[-1]}] of x's dtype or fp32")
+    return dev, stream
+
+
+def _rows_of(x):
+    c = x.shape[-1]
+    return (x.numel() // c if c else 0), c
+
+
+def residual_rms_norm_fwd(x, residual, weight, eps: float, p: float, seed: int, offset: int, need_rstd: bool = True):
+    """Returns (y, h, rstd [rows] fp32 or None)."""
+    dev, stream = _check_norm("residual_rms_norm", x, residual, weight)
+    x, residual, weight = _flat(x), _flat(residual), _flat(weight)
+    rows, c = _rows_of(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+    h = torch.empty(x.shape, dtype=stream, device=dev)
+    rstd = torch.empty(rows, dtype=torch.float32, device=dev) if need_rstd else None
+    _run(dev, "lsrm_residual_rms_norm_fwd", rows, c, _DTYPES[x.dtype], _DTYPES[stream],
+         _DTYPES[x.dtype if weight is None else weight.dtype], float(eps), float(p), _seed(seed), _seed(offset),
+         _addr(x), _addr(residual), _addr(weight), _addr(y), _addr(h), _addr(rstd))
+    return y, h, rstd
+
+
+def residual_rms_norm_bwd(h, rstd, weight, dy, dh, p: float, seed: int, offset: int, need_dw: bool = True):
+    """Gradients (dx, dresidual, dweight) from dy and dh (None: zero); dx is
+    dresidual itself where the two are equal."""
+    dev = h.device
+    weight, dy, dh = _flat(weight), _flat(dy), _flat(dh)
+    rows, c = _rows_of(h)
+    same = p == 0.0 and dy.dtype == h.dtype
+    dres = torch.empty(h.shape, dtype=h.dtype, device=dev)
+    dx = dres if same else torch.empty(h.shape, dtype=dy.dtype, device=dev)
+    need_dw = need_dw and weight is not None
+    dw = torch.empty_like(weight) if need_dw else None
+    ws = _workspace(_lib.lib().lsrm_residual_rms_norm_workspace_bytes(rows, c), dev) if need_dw else None
+    _run(dev, "lsrm_residual_rms_norm_bwd", rows, c, _DTYPES[dy.dtype], _DTYPES[h.dtype],
+         _DTYPES[dy.dtype if weight is None else weight.dtype], float(p), _seed(seed), _seed(offset), _addr(h),
+         _addr(rstd), _addr(weight), _addr(dy), _addr(dh), None if same else _addr(dx), _addr(dres), _addr(dw),
+         _addr(ws), ws.numel() if ws is not None else 0)
+    return dx, dres, dw
+
+
+def residual_rms_norm_8bit(x, residual, weight, eps: float, dtype: torch.dtype, group: int):
+    """Returns (values [.., C] in ``dtype``, scales [.., groups] fp32, h)."""
+    dev, stream = _check_norm("residual_rms_norm_8bit", x, residual, weight)
+    _need(dtype in (torch.float8_e4m3fn, torch.int8), f"residual_rms_norm_8bit: dtype {dtype} is not e4m3 or int8")
+    x, residual, weight = _flat(x), _flat(residual), _flat(weight)
+    rows, c = _rows_of(x)
+    groups = -(-c // group) if group > 0 else 1
+    q = torch.empty(x.shape, dtype=dtype, device=dev)
+    scales = torch.empty(*x.shape[:-1], groups, dtype=torch.float32, device=dev)
+    h = torch.empty(x.shape, dtype=stream, device=dev)
+    _run(dev, "lsrm_residual_rms_norm_8bit", rows, c, _DTYPES[x.dtype], _DTYPES[stream],
+         _DTYPES[x.dtype if weight is None else weight.dtype], float(eps), _DTYPES[dtype], int(group), _addr(x),
+         _addr(residual), _addr(weight), _addr(q), _addr(scales), _addr(h))
+    return q, scales, h
+
+
+def dequantize_8bit(values, scales, dtype: torch.dtype, group: int):
+    dev = _cuda("dequantize_8bit", values, scales)
+    _need(values.dtype in (torch.float8_e4m3fn, torch.int8) and scales.dtype == torch.float32
+          and dtype in (torch.bfloat16, torch.float16, torch.float32), "dequantize_8bit: unsupported dtypes")
+    values, scales = _flat(values), scales.contiguous()
+    rows, c = _rows_of(values)
+    y = torch.empty(values.shape, dtype=dtype, device=dev)
+    _run(dev, "lsrm_dequantize_8bit", rows, c, _DTYPES[values.dtype], _DTYPES[dtype], int(group), _addr(values),
+         _addr(scales), _addr(y))
+    return y
