@@ -37,7 +37,8 @@ static EncodeTiledFn get_encode_fn() {
 }
 
 int make_tmap_3d(CUtensorMap* map, const void* base, int D, int n_head, long long n_tok, long long tok_stride,
-                 int box_h, int box_n) {
+                 int box_h, int box_n, int box_d) {
+  if (box_d == 0) box_d = D;
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) {
     set_error("cuTensorMapEncodeTiled is unavailable from the driver");
@@ -54,10 +55,10 @@ int make_tmap_3d(CUtensorMap* map, const void* base, int D, int n_head, long lon
   if (n_tok < 1) n_tok = 1;
   cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)n_head, (cuuint64_t)n_tok};
   cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)tok_stride * 2};
-  cuuint32_t box[3] = {(cuuint32_t)D, (cuuint32_t)box_h, (cuuint32_t)box_n};
+  cuuint32_t box[3] = {(cuuint32_t)box_d, (cuuint32_t)box_h, (cuuint32_t)box_n};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUtensorMapSwizzle swz = (D * 2 == 128) ? CU_TENSOR_MAP_SWIZZLE_128B
-                           : (D * 2 == 64) ? CU_TENSOR_MAP_SWIZZLE_64B
+  CUtensorMapSwizzle swz = (box_d * 2 == 128) ? CU_TENSOR_MAP_SWIZZLE_128B
+                           : (box_d * 2 == 64) ? CU_TENSOR_MAP_SWIZZLE_64B
                                            : CU_TENSOR_MAP_SWIZZLE_32B;
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,

@@ -67,11 +67,11 @@ class ProfScope {
 
 // Encodes a 3-D tiled tensor map over a [n_tok, n_head, D] 16-bit tensor:
 // dims {D, n_head, n_tok}, strides in elements (head stride D, token stride
-// `tok_stride`), box {D, box_h, box_n}, swizzle matched to the row size
-// (D*2 = 128 B -> 128B swizzle, 64 B -> 64B swizzle).  Out-of-range rows
-// read as zero.
+// `tok_stride`), box {box_d, box_h, box_n} (box_d = 0: D), swizzle matched to
+// the box's row size (128 B -> 128B swizzle, 64 B -> 64B swizzle).
+// Out-of-range rows read as zero.
 int make_tmap_3d(CUtensorMap* map, const void* base, int D, int n_head, long long n_tok, long long tok_stride,
-                 int box_h, int box_n);
+                 int box_h, int box_n, int box_d = 0);
 
 // Fills maps_k/maps_v (box heights 8 << i rows, i < n) over k and v.
 int make_kv_maps(CUtensorMap* maps_k, CUtensorMap* maps_v, int n, const void* k, const void* v, int D, int n_head,

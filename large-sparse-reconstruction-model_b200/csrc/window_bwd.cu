@@ -14,14 +14,10 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include "host_util.h"
-#include "window_common.cuh"
+#include "window_host.h"
 
 namespace lsrm {
 namespace {
-
-constexpr int kMaxD = 128;
-constexpr int kMaxSinks = 128;
 
 template <typename T>
 __device__ __forceinline__ float dot_row(const float* a, const T* b, int d) {
@@ -35,60 +31,10 @@ __device__ __forceinline__ float dot_row(const float* a, const T* b, int d) {
   return s;
 }
 
-__device__ __forceinline__ float warp_max(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
-}
-
-template <typename T, int D>
-__global__ void __launch_bounds__(128) window_fwd_kernel(const WindowParams p) {
-  __shared__ float sq[4][D];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * 4 + warp;
-  if (row >= (long long)p.total_q * p.hq) return;
-  const int tok = (int)(row / p.hq), h = (int)(row % p.hq), hk = h / p.g;
-  const int b = seq_of_token(p.cu_q, p.num_seqs, tok);
-  const Seq sq_ = seq_of(p, b);
-  const int pos = tok - sq_.q0 + sq_.lk - sq_.lq;
-  const Seen seen = keys_of(p, pos, sq_.lk, b < p.num_seqs);
-  const T* q = static_cast<const T*>(p.q) + tok * p.q_stride + h * D;
-  for (int d = lane; d < D; d += 32) sq[warp][d] = (float)q[d] * p.scale;
-  __syncwarp();
-  const T* k = static_cast<const T*>(p.k) + sq_.k0 * p.k_stride + hk * D;
-  const T* v = static_cast<const T*>(p.v) + sq_.k0 * p.v_stride + hk * D;
-  float m = -INFINITY, l = 0.f, acc[D / 32];
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
-  const int n = seen.sink + seen.hi - seen.lo;
-  for (int base = 0; base < n; base += 32) {
-    const int idx = base + lane;
-    const int j = idx < seen.sink ? idx : seen.lo + idx - seen.sink;
-    const float s = idx < n ? dot_row(sq[warp], k + j * p.k_stride, D) : -INFINITY;
-    const float m_new = fmaxf(m, warp_max(s));
-    const float off = m_new == -INFINITY ? 0.f : m_new;
-    const float r = expf(m - off), e = expf(s - off);
-    l = l * r + warp_sum(e);
-    m = m_new;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) acc[i] *= r;
-    const int cnt = min(32, n - base);
-    for (int t = 0; t < cnt; ++t) {
-      const float pt = __shfl_sync(0xffffffffu, e, t);
-      const int jt = __shfl_sync(0xffffffffu, j, t);
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(pt, (float)v[jt * p.v_stride + lane + 32 * i], acc[i]);
-    }
-  }
-  T* out = static_cast<T*>(p.out) + row * D;
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) out[lane + 32 * i] = (T)(l == 0.f ? 0.f : acc[i] / l);
-  if (lane == 0) p.lse[row] = l == 0.f ? -INFINITY : m + logf(l);
 }
 
 struct WindowBwdParams : WindowParams {
@@ -200,80 +146,10 @@ __global__ void __launch_bounds__(128) window_dkv_kernel(const WindowBwdParams p
   }
 }
 
-int check_window(const lsrm_window_shape* s, const int32_t* cu_q, const int32_t* cu_k, const void* q, const void* k,
-                 const void* v) {
-  LSRM_CHECK_ARG(s, "shape must not be NULL");
-  LSRM_CHECK_ARG(s->num_seqs >= 0 && s->total_q >= 0 && s->total_k >= 0, "sizes must not be negative");
-  LSRM_CHECK_ARG(s->num_kv_heads >= 1 && s->num_q_heads >= 1 && s->num_q_heads % s->num_kv_heads == 0,
-                 "num_q_heads (%d) must be a multiple of num_kv_heads (%d)", s->num_q_heads, s->num_kv_heads);
-  LSRM_CHECK_ARG(s->num_q_heads / s->num_kv_heads <= 64, "at most 64 query heads per kv head");
-  LSRM_CHECK_ARG(s->head_dim == 32 || s->head_dim == 64 || s->head_dim == 128, "head_dim (%d) must be 32, 64 or 128",
-                 s->head_dim);
-  LSRM_CHECK_ARG(s->dtype == LSRM_DTYPE_BF16 || s->dtype == LSRM_DTYPE_F16, "dtype must be bf16 or fp16");
-  LSRM_CHECK_ARG(s->window >= 1, "window (%d) must be at least 1", s->window);
-  LSRM_CHECK_ARG(s->sinks >= 0 && s->sinks <= kMaxSinks, "sinks (%d) must be in [0, %d]", s->sinks, kMaxSinks);
-  const int64_t qr = (int64_t)s->num_q_heads * s->head_dim, kr = (int64_t)s->num_kv_heads * s->head_dim;
-  LSRM_CHECK_ARG(s->q_token_stride >= qr && s->k_token_stride >= kr && s->v_token_stride >= kr,
-                 "token strides must cover the heads");
-  LSRM_CHECK_ARG(s->q_token_stride % 8 == 0 && s->k_token_stride % 8 == 0 && s->v_token_stride % 8 == 0,
-                 "token strides must be multiples of 8 elements");
-  LSRM_CHECK_ARG((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v) & 15) == 0, "q, k and v must be 16-byte aligned");
-  LSRM_CHECK_ARG(cu_q && cu_k, "the sequence offsets must not be NULL");
-  LSRM_CHECK_ARG((s->total_q == 0 || q) && (s->total_k == 0 || (k && v)), "q, k and v must not be NULL");
-  return LSRM_OK;
-}
-
-WindowParams window_params(const lsrm_window_shape* s, const int32_t* cu_q, const int32_t* cu_k, const void* q,
-                           const void* k, const void* v, void* out, float* lse, int* err) {
-  WindowParams p{};
-  p.num_seqs = s->num_seqs, p.total_q = s->total_q, p.total_k = s->total_k;
-  p.hq = s->num_q_heads, p.hkv = s->num_kv_heads, p.g = p.hq / p.hkv;
-  p.left = s->causal ? s->window - 1 : s->window / 2;
-  p.right = s->causal ? 0 : s->window / 2;
-  // reaches past every key are the same reach: keeps the index arithmetic in range
-  p.left = std::min(p.left, std::max(p.total_q, p.total_k));
-  p.right = std::min(p.right, std::max(p.total_q, p.total_k));
-  p.sinks = s->sinks, p.causal = s->causal;
-  p.scale = s->softmax_scale > 0.f ? s->softmax_scale : 1.f / sqrtf((float)s->head_dim);
-  p.cu_q = cu_q, p.cu_k = cu_k;
-  p.q_stride = s->q_token_stride, p.k_stride = s->k_token_stride, p.v_stride = s->v_token_stride;
-  p.q = q, p.k = k, p.v = v, p.out = out, p.lse = lse, p.err = err;
-  return p;
-}
-
 }  // namespace
 }  // namespace lsrm
 
 using namespace lsrm;
-
-#define WINDOW_TYPES(CALL)                                             \
-  if (shape->dtype == LSRM_DTYPE_BF16) {                               \
-    if (shape->head_dim == 32) CALL(__nv_bfloat16, 32)                 \
-    else if (shape->head_dim == 64) CALL(__nv_bfloat16, 64)            \
-    else CALL(__nv_bfloat16, 128)                                      \
-  } else {                                                             \
-    if (shape->head_dim == 32) CALL(__half, 32)                        \
-    else if (shape->head_dim == 64) CALL(__half, 64)                   \
-    else CALL(__half, 128)                                             \
-  }
-
-extern "C" int lsrm_window_attn_fwd(const lsrm_window_shape* shape, const int32_t* cu_seqlens_q,
-                                    const int32_t* cu_seqlens_k, const void* q, const void* k, const void* v,
-                                    void* out, float* lse, int* err_flags, void* stream) {
-  int rc = check_window(shape, cu_seqlens_q, cu_seqlens_k, q, k, v);
-  if (rc) return rc;
-  if (shape->total_q == 0) return LSRM_OK;
-  LSRM_CHECK_ARG(out && lse, "out and lse must not be NULL");
-  const WindowParams p = window_params(shape, cu_seqlens_q, cu_seqlens_k, q, k, v, out, lse, err_flags);
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  ProfScope ps("window_attn_fwd", s);
-  const unsigned grid = (unsigned)(((long long)p.total_q * p.hq + 3) / 4);
-#define CALL(T, D) window_fwd_kernel<T, D><<<grid, 128, 0, s>>>(p);
-  WINDOW_TYPES(CALL)
-#undef CALL
-  LSRM_LAUNCH_CHECK();
-  return LSRM_OK;
-}
 
 extern "C" size_t lsrm_window_attn_workspace_bytes(const lsrm_window_shape* shape) {
   if (!shape || shape->total_q < 0 || shape->num_q_heads < 1) return 0;
@@ -303,7 +179,7 @@ extern "C" int lsrm_window_attn_bwd(const lsrm_window_shape* shape, const int32_
   if (p.total_q > 0) {
     ProfScope ps("window_attn_dq", s);
     const unsigned grid = (unsigned)(((long long)p.total_q * p.hq + 3) / 4);
-#define CALL(T, D) window_dq_kernel<T, D><<<grid, 128, 0, s>>>(p);
+#define CALL(BF, D) window_dq_kernel<std::conditional_t<BF, __nv_bfloat16, __half>, D><<<grid, 128, 0, s>>>(p);
     WINDOW_TYPES(CALL)
 #undef CALL
     LSRM_LAUNCH_CHECK();
@@ -311,7 +187,7 @@ extern "C" int lsrm_window_attn_bwd(const lsrm_window_shape* shape, const int32_
   if (p.total_k > 0) {
     ProfScope ps("window_attn_dkv", s);
     const unsigned grid = (unsigned)(((long long)p.total_k * p.hkv + 3) / 4);
-#define CALL(T, D) window_dkv_kernel<T, D><<<grid, 128, 0, s>>>(p);
+#define CALL(BF, D) window_dkv_kernel<std::conditional_t<BF, __nv_bfloat16, __half>, D><<<grid, 128, 0, s>>>(p);
     WINDOW_TYPES(CALL)
 #undef CALL
     LSRM_LAUNCH_CHECK();
