@@ -7,14 +7,16 @@
 // CTA per multiprocessor walks work items (two tiles of 128 packed query rows
 // of one kv head and the keys that either sees):
 //   warps 0-3, 4-7  softmax of row tile 0 and 1, a row a thread: S from TMEM,
-//                   mask, running maximum, P = exp2(S - m) back over S as
-//                   16-bit operand, at the end O / l to global memory
+//                   mask, running maximum, P = exp2(S - m) to TMEM as 16-bit
+//                   operand, at the end O / l to global memory
 //   warps 8, 9      tensor-core issue for row tile 0 and 1: S = Q K^T, O += P V
-//                   (P from TMEM); while one tile is in its softmax the other
-//                   one's products run
+//                   (P from TMEM)
 //   warp 10         producer: work items, TMA of Q, K and V
 // K and V tiles (128 keys) go through one ring and serve both row tiles, which
-// halves the L2 reads per product.  Rounding: S, m, l and O are fp32; P is
+// halves the L2 reads per product.  Up to 64 channels P has TMEM columns of its
+// own and the next S is computed while this one's softmax runs; at 128 channels
+// TMEM is full, P lies over S, and the row tiles' turns hide each other's
+// products.  Rounding: S, m, l and O are fp32; P is
 // rounded to the operand type (the sum l takes it unrounded), O once at the end.
 #include "window_host.h"
 #include "window_tile.cuh"
@@ -44,9 +46,9 @@ struct FwSmem {
   static constexpr int OFF_KV = 2 * NQ * TILE;
   static constexpr int OFF_ITEM = OFF_KV + NS * TILE;
   static constexpr int OFF_BAR = OFF_ITEM + kFwItems * (int)sizeof(FwItem);
-  // q_full[2][NQ], q_empty[2][NQ], kv_full[NS], kv_empty[NS], s_full[2], p_full[2], pv_done[2], item_full[],
-  // item_empty[], mma_done[2]
-  static constexpr int NBAR = 4 * NQ + 2 * NS + 6 + 2 * kFwItems + 2;
+  // q_full[2][NQ], q_empty[2][NQ], kv_full[NS], kv_empty[NS], s_full[2], s_free[2], p_full[2], pv_done[2],
+  // item_full[], item_empty[], mma_done[2]
+  static constexpr int NBAR = 4 * NQ + 2 * NS + 8 + 2 * kFwItems + 2;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int BYTES = OFF_MISC + 16 + 1024;
   static constexpr int ALLOC = BYTES > kOneCtaPerSmSmem ? BYTES : kOneCtaPerSmSmem;
@@ -105,7 +107,8 @@ __global__ void __launch_bounds__(kFwThreads, 1)
   uint64_t* kv_full = q_empty + 2 * L::NQ;
   uint64_t* kv_empty = kv_full + L::NS;
   uint64_t* s_full = kv_empty + L::NS;
-  uint64_t* p_full = s_full + 2;
+  uint64_t* s_free = s_full + 2;
+  uint64_t* p_full = s_free + 2;
   uint64_t* pv_done = p_full + 2;
   uint64_t* item_full = pv_done + 2;
   uint64_t* item_empty = item_full + kFwItems;
@@ -121,6 +124,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
     for (int i = 0; i < L::NS; ++i) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], 2);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], 4);
       mbar_init(&p_full[i], 4);
       mbar_init(&pv_done[i], 1);
       mbar_init(&mma_done[i], 1);
@@ -137,131 +141,165 @@ __global__ void __launch_bounds__(kFwThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // TMEM columns: S [0, 256), O [256, 256 + 2 D), P (64 a row tile) in [384, 512) up to D = 64, else over S
+  constexpr bool kOwnP = D <= 64;
 
   if (warp == 10) {
     // ------------------------------ producer ------------------------------
-    if (lane == 0) {
+    // The whole warp walks the items; one elected lane issues (under elect.sync
+    // the compiler knows that one lane is active and issues TMA and tensor-core
+    // instructions from uniform registers; under `lane == 0` each took some 120
+    // cycles).
+    if (elect_one()) {
       tma_prefetch_desc(&tm_q);
       tma_prefetch_desc(&tm_k);
       tma_prefetch_desc(&tm_v);
-      const uint32_t q_bytes = (uint32_t)(G * TT * D * 2);
-      int n_it = 0, J = 0, nq[2] = {0, 0};
-      bool ok = true;
-      for (int w = blockIdx.x; ok; w += gridDim.x) {
-        FwItem it;
-        it.stop = w >= n_items;
-        if (!it.stop) {
-          const int slot = w / p.hkv;
-          it.hk = w - slot * p.hkv;
-          const int b = seq_of_slot(p.cu_q, p.num_seqs, 2 * TT, slot);
-          const Seq s = seq_of(p, b);
-          const int i0 = (slot - (p.cu_q[b] / (2 * TT) + b)) * 2 * TT;
-          if (i0 < 0 || i0 >= s.lq) continue;
-          it.tok = s.q0 + i0;
-          it.n[0] = min(TT, s.lq - i0);
-          it.n[1] = max(0, min(TT, s.lq - i0 - TT));
-          it.lk = b < p.num_seqs ? s.lk : 0;
-          it.pos = i0 + s.lk - s.lq;
-          it.key0 = s.k0;
-          plan_tiles(p, it, TT);
-        }
-        const int r = n_it % kFwItems;
-        if (!mbar_wait(&item_empty[r], ((n_it / kFwItems) & 1) ^ 1, abort_flag, p.err)) { ok = false; break; }
+    }
+    const uint32_t q_bytes = (uint32_t)(G * TT * D * 2);
+    int n_it = 0, J = 0, nq[2] = {0, 0};
+    bool ok = true;
+    for (int w = blockIdx.x; ok; w += gridDim.x) {
+      FwItem it;
+      it.stop = w >= n_items;
+      if (!it.stop) {
+        const int slot = w / p.hkv;
+        it.hk = w - slot * p.hkv;
+        const int b = seq_of_slot(p.cu_q, p.num_seqs, 2 * TT, slot);
+        const Seq s = seq_of(p, b);
+        const int i0 = (slot - (p.cu_q[b] / (2 * TT) + b)) * 2 * TT;
+        if (i0 < 0 || i0 >= s.lq) continue;
+        it.tok = s.q0 + i0;
+        it.n[0] = min(TT, s.lq - i0);
+        it.n[1] = max(0, min(TT, s.lq - i0 - TT));
+        it.lk = b < p.num_seqs ? s.lk : 0;
+        it.pos = i0 + s.lk - s.lq;
+        it.key0 = s.k0;
+        plan_tiles(p, it, TT);
+      }
+      const int r = n_it % kFwItems;
+      if (!wait_phase(&item_empty[r], ((n_it / kFwItems) & 1) ^ 1, abort_flag, p.err)) break;
+      if (lane == 0) {
         items[r] = it;
         mbar_arrive(&item_full[r]);
-        ++n_it;
-        if (it.stop) break;
-        for (int u = 0; u < 2 && ok; ++u) {
-          if (it.b[u] <= it.a[u]) continue;
-          const int st = u * L::NQ + nq[u] % L::NQ;
-          if (!mbar_wait(&q_empty[st], ((nq[u] / L::NQ) & 1) ^ 1, abort_flag, p.err)) { ok = false; break; }
+      }
+      __syncwarp();
+      ++n_it;
+      if (it.stop) break;
+      for (int u = 0; u < 2 && ok; ++u) {
+        if (it.b[u] <= it.a[u]) continue;
+        const int st = u * L::NQ + nq[u] % L::NQ;
+        if (!(ok = wait_phase(&q_empty[st], ((nq[u] / L::NQ) & 1) ^ 1, abort_flag, p.err))) break;
+        if (elect_one()) {
           mbar_arrive_expect_tx(&q_full[st], q_bytes);
           load_tile<D>(sQ + st * L::TILE, 128, &tm_q, it.hk * G, it.tok + u * TT, &q_full[st]);
-          ++nq[u];
         }
-        for (int t = 0; t < it.tiles && ok; ++t) {
-          const int key = it.key0 + tile_key(it, t);
-          for (int kv = 0; kv < 2; ++kv, ++J) {
-            const int st = J % L::NS;
-            if (!mbar_wait(&kv_empty[st], ((J / L::NS) & 1) ^ 1, abort_flag, p.err)) { ok = false; break; }
+        __syncwarp();
+        ++nq[u];
+      }
+      for (int t = 0; t < it.tiles && ok; ++t) {
+        const int key = it.key0 + tile_key(it, t);
+        for (int kv = 0; kv < 2; ++kv) {
+          const int st = J % L::NS;
+          if (!(ok = wait_phase(&kv_empty[st], ((J / L::NS) & 1) ^ 1, abort_flag, p.err))) break;
+          if (elect_one()) {
             mbar_arrive_expect_tx(&kv_full[st], L::TILE);
             load_tile<D>(sKV + st * L::TILE, 128, kv ? &tm_v : &tm_k, it.hk, key, &kv_full[st]);
           }
+          __syncwarp();
+          ++J;
         }
       }
-      // after an abort: copies in flight land before the CTA exits
-      if (*abort_flag) {
-        for (int u = 0; u < 2; ++u)
-          for (int k = max(0, nq[u] - L::NQ); k < nq[u]; ++k)
-            mbar_wait_drain(&q_full[u * L::NQ + k % L::NQ], (k / L::NQ) & 1);
-        for (int j = max(0, J - L::NS); j < J; ++j) mbar_wait_drain(&kv_full[j % L::NS], (j / L::NS) & 1);
-      }
+    }
+    // after an abort: copies in flight land before the CTA exits
+    if (lane == 0 && *abort_flag) {
+      for (int u = 0; u < 2; ++u)
+        for (int k = max(0, nq[u] - L::NQ); k < nq[u]; ++k)
+          mbar_wait_drain(&q_full[u * L::NQ + k % L::NQ], (k / L::NQ) & 1);
+      for (int j = max(0, J - L::NS); j < J; ++j) mbar_wait_drain(&kv_full[j % L::NS], (j / L::NS) & 1);
     }
     __syncwarp();
   } else if (warp >= 8) {
     // --------------------------- tensor-core issue ---------------------------
     const int u = warp - 8;
-    const uint32_t tm_s = tmem + u * 128, tm_o = tmem + 256 + u * D;
+    const uint32_t tm_s = tmem + u * 128, tm_o = tmem + 256 + u * D, tm_p = kOwnP ? tmem + 384 + u * 64 : tm_s;
     const uint32_t idesc_o = make_idesc(AB, 0, 1, 128, D);
-    int n_it = 0, J = 0, nq = 0, np = 0;
-    bool ok = true;
-    while (ok) {
+    int n_it = 0, J = 0, nq = 0, ns = 0, np = 0;  // items, ring slots, Q tiles, S and P V products so far
+    while (true) {
       const int r = n_it % kFwItems;
-      if (!warp_wait(&item_full[r], (n_it / kFwItems) & 1, abort_flag, p.err)) break;
+      if (!wait_phase(&item_full[r], (n_it / kFwItems) & 1, abort_flag, p.err)) break;
       const FwItem& it = items[r];
       ++n_it;
       if (it.stop) break;
       const int st_q = u * L::NQ + nq % L::NQ;
       const uint32_t q_base = smem_u32(sQ + st_q * L::TILE);
       const int a = it.a[u], b = it.b[u];
-      if (b > a && !warp_wait(&q_full[st_q], (nq / L::NQ) & 1, abort_flag, p.err)) break;
-      for (int t = 0; t < it.tiles; ++t, J += 2) {
-        const int sk = J % L::NS, sv = (J + 1) % L::NS;
-        if (!warp_wait(&kv_full[sk], (J / L::NS) & 1, abort_flag, p.err)) { ok = false; break; }
-        if (t < a || t >= b) {  // the other row tile's keys only
-          if (!warp_wait(&kv_full[sv], ((J + 1) / L::NS) & 1, abort_flag, p.err)) { ok = false; break; }
-          if (lane == 0) {
-            mbar_arrive(&kv_empty[sk]);
-            mbar_arrive(&kv_empty[sv]);
-          }
-          continue;
-        }
-        // sinks of their own tile: only as many columns as they need
-        const int cols = it.sep && t == 0 ? (p.sinks + 31) / 32 * 32 : 128;
-        // P lies over S: the last product that reads it has to be over
-        if (np > 0 && !warp_wait(&pv_done[u], (np - 1) & 1, abort_flag, p.err)) { ok = false; break; }
-        tc_fence_after();
+      // sinks of their own tile: only as many columns as they need
+      auto cols_of = [&](int t) { return it.sep && t == 0 ? (p.sinks + 31) / 32 * 32 : 128; };
+      auto wait_slot = [&](int j) { return wait_phase(&kv_full[j % L::NS], (j / L::NS) & 1, abort_flag, p.err); };
+      // keys that only the other row tile sees
+      auto pass = [&](int t) {
+        if (!wait_slot(J + 2 * t) || !wait_slot(J + 2 * t + 1)) return false;
         if (lane == 0) {
-          const uint32_t k_base = smem_u32(sKV + sk * L::TILE);
-          const uint32_t idesc_s = make_idesc(AB, 0, 0, 128, cols);
+          mbar_arrive(&kv_empty[(J + 2 * t) % L::NS]);
+          mbar_arrive(&kv_empty[(J + 2 * t + 1) % L::NS]);
+        }
+        __syncwarp();
+        return true;
+      };
+      auto issue_s = [&](int t) {
+        const int j = J + 2 * t, st = j % L::NS;
+        if (!wait_slot(j)) return false;
+        // the last S has been read; where P lies over S, the product that reads P is over
+        if (kOwnP && ns > 0 && !wait_phase(&s_free[u], (ns - 1) & 1, abort_flag, p.err)) return false;
+        if (!kOwnP && np > 0 && !wait_phase(&pv_done[u], (np - 1) & 1, abort_flag, p.err)) return false;
+        ++ns;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t k_base = smem_u32(sKV + st * L::TILE);
+          const uint32_t idesc_s = make_idesc(AB, 0, 0, 128, cols_of(t));
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks)
             umma_f16(tm_s, desc_k<D>(q_base, 128, ks), desc_k<D>(k_base, 128, ks), idesc_s, ks > 0);
           umma_commit(&s_full[u]);
-          umma_commit(&kv_empty[sk]);
+          umma_commit(&kv_empty[st]);
           if (t == b - 1) umma_commit(&q_empty[st_q]);
         }
         __syncwarp();
-        if (!warp_wait(&kv_full[sv], ((J + 1) / L::NS) & 1, abort_flag, p.err)) { ok = false; break; }
-        const int valid = tile_valid(it, t);
-        if (valid < cols) zero_rows<D>(sKV + sv * L::TILE, 128, valid);
-        if (!warp_wait(&p_full[u], np & 1, abort_flag, p.err)) { ok = false; break; }
+        return true;
+      };
+      bool ok = true;
+      for (int t = 0; t < a && ok; ++t) ok = pass(t);
+      if (ok && b > a) {
+        ok = wait_phase(&q_full[st_q], (nq / L::NQ) & 1, abort_flag, p.err) && issue_s(a);
+        ++nq;
+      }
+      for (int t = a; t < b && ok; ++t) {
+        if (kOwnP && t + 1 < b && !(ok = issue_s(t + 1))) break;
+        const int j = J + 2 * t + 1, st = j % L::NS, cols = cols_of(t), valid = tile_valid(it, t);
+        if (!(ok = wait_slot(j))) break;
+        if (valid < cols) zero_rows<D>(sKV + st * L::TILE, 128, valid);
+        if (!(ok = wait_phase(&p_full[u], np & 1, abort_flag, p.err))) break;
         ++np;
         tc_fence_after();
-        if (lane == 0) {
-          const uint32_t v_base = smem_u32(sKV + sv * L::TILE);
-          for (int ks = 0; ks < cols / 16; ++ks)
-            umma_f16_ts(tm_o, tm_s + ks * 8, desc_mn<D>(v_base, 128, ks), idesc_o, (t > a || ks > 0) ? 1u : 0u);
+        if (elect_one()) {
+          const uint32_t v_base = smem_u32(sKV + st * L::TILE);
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks)
+            if (ks < cols / 16)
+              umma_f16_ts(tm_o, tm_p + ks * 8, desc_mn<D>(v_base, 128, ks), idesc_o, (t > a || ks > 0) ? 1u : 0u);
           umma_commit(&pv_done[u]);
-          umma_commit(&kv_empty[sv]);
+          umma_commit(&kv_empty[st]);
         }
         __syncwarp();
+        if (!kOwnP && t + 1 < b) ok = issue_s(t + 1);
       }
-      if (b > a) ++nq;
+      for (int t = b > a ? b : a; t < it.tiles && ok; ++t) ok = pass(t);
+      if (!ok) break;
+      J += 2 * it.tiles;
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[r]);
     }
-    if (lane == 0) {
+    if (elect_one()) {
       umma_commit(&mma_done[u]);
       mbar_wait_drain(&mma_done[u], 0);
     }
@@ -271,19 +309,23 @@ __global__ void __launch_bounds__(kFwThreads, 1)
     // A thread owns a row.  The maximum is lazy: P = exp2(s - m) may reach 2^8
     // before O and l are rescaled to a new one (fp32 sums, and a 16-bit P keeps
     // its relative precision), so after a row's first tiles O is hardly ever
-    // touched.
+    // touched.  S is swept twice in chunks of 32 columns, the next chunk in
+    // flight: once for the maximum, once for P (holding a row's 128 scores
+    // between the two spills).  A chunk that no row of the warp sees is skipped
+    // and one that all see is not masked, which leaves one masked chunk of a
+    // window's slanted edge.
     constexpr float kLazy = 8.f;
     const int u = warp >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const int t_row = row / G, g = row - t_row * G;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t tm_s = tmem + u * 128 + lanes, tm_o = tmem + 256 + u * D + lanes;
+    const uint32_t tm_p = (kOwnP ? tmem + 384 + u * 64 : tmem + u * 128) + lanes;
     const float sl2 = p.scale * 1.4426950408889634f;
-    int n_it = 0, ns = 0;
-    bool ok = true;
-    while (ok) {
+    int n_it = 0, ns = 0;  // items, tiles so far
+    while (true) {
       const int r = n_it % kFwItems;
-      if (!warp_wait(&item_full[r], (n_it / kFwItems) & 1, abort_flag, p.err)) break;
+      if (!wait_phase(&item_full[r], (n_it / kFwItems) & 1, abort_flag, p.err)) break;
       const FwItem& it = items[r];
       ++n_it;
       if (it.stop) break;
@@ -291,52 +333,55 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       const bool live = t_row < it.n[u] && t_row < TT;
       const RowKeys keys = row_keys(p, it.pos + u * TT + t_row, it.lk);
       float m = -INFINITY;
-      float2 l2 = make_float2(0.f, 0.f);
+      float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      bool ok = true;
+      float s[2][32];
       for (int t = a; t < b; ++t) {
         const int key = tile_key(it, t);
         const bool sinks_only = it.sep && t == 0;
         const int lo = sinks_only ? 0 : keys.lo - key, hi = sinks_only ? 0 : keys.hi - key;
         const int sink = it.sep && t > 0 ? 0 : keys.sink - key;
-        const int nch = sinks_only ? (p.sinks + 31) / 32 : 4;
-        if (!warp_wait(&s_full[u], ns & 1, abort_flag, p.err)) { ok = false; break; }
-        ++ns;
-        tc_fence_after();
-        // two sweeps over S, 32 columns at a time with the next ones in flight:
-        // the maximum, then P (holding all 128 columns of a row spills)
-        float s[2][32];
-        const bool full = __all_sync(0xffffffffu, !live || (lo <= 0 && hi >= 128));
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        tmem_ld32(tm_s, s[0]);
+        // columns 32 c .. + 31: which of them this row sees; per warp, chunks that some and that all rows see
+        uint32_t some = 0u, all = 0u;
+        uint32_t bits[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          if (c < nch) {
-            tmem_wait_ld32(s[c & 1]);
-            if (c < 3 && c + 1 < nch) tmem_ld32(tm_s + 32 * (c + 1), s[(c + 1) & 1]);
-            float* v = s[c & 1];
-            if (!full) {
-              const uint32_t bits = seen_bits(lo, hi, sink, 32 * c);
+          bits[c] = live ? seen_bits(lo, hi, sink, 32 * c) : 0u;
+          some |= (__any_sync(0xffffffffu, bits[c] != 0u) ? 1u : 0u) << c;
+          all |= (__all_sync(0xffffffffu, !live || bits[c] == 0xffffffffu) ? 1u : 0u) << c;
+        }
+        if (!(ok = wait_phase(&s_full[u], ns & 1, abort_flag, p.err))) break;
+        ++ns;
+        tc_fence_after();
+        float mt = -INFINITY;
+        if (some & 1u) tmem_ld32(tm_s, s[0]);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = (bits >> i & 1u) ? v[i] : -INFINITY;
-            }
-#pragma unroll
-            for (int i = 0; i < 32; ++i) mx[i & 3] = fmaxf(mx[i & 3], v[i]);
+        for (int c = 0; c < 4; ++c) {
+          tmem_wait_values<32>(s[c & 1]);
+          if (c < 3 && (some >> (c + 1) & 1u)) tmem_ld32(tm_s + 32 * (c + 1), s[(c + 1) & 1]);
+          if (some >> c & 1u) {
+            if (!(all >> c & 1u)) mask32(s[c & 1], bits[c]);
+            mt = fmaxf(mt, max32(s[c & 1]));
           }
         }
-        tmem_ld32(tm_s, s[0]);  // the second sweep's first columns, in flight over what follows
-        const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+        if (some & 1u) tmem_ld32(tm_s, s[0]);  // in flight over what follows
+        mt *= sl2;
+        // P's columns and O are free once the product of the tile before is over
+        if (t > a && !wait_phase(&pv_done[u], (ns - 2) & 1, abort_flag, p.err)) { ok = false; break; }
         const bool move = mt > m + kLazy || (m == -INFINITY && mt > -INFINITY);
         if (__any_sync(0xffffffffu, move)) {
           const float m_new = move ? mt : m;
           const float f = m == -INFINITY ? 0.f : ex2(m - m_new);
           m = m_new;
-          l2.x *= f;
-          l2.y *= f;
-          if (t > a) {  // O holds the tiles before this one (their products precede this S)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) l2[j] = mul2(l2[j], make_float2(f, f));
+          if (t > a) {
+            tc_fence_after();
 #pragma unroll
             for (int c = 0; c < D; c += 16) {
               float o[16];
               tmem_ld16(tm_o + c, o);
-              tmem_wait_ld();
+              tmem_wait_values<16>(o);
 #pragma unroll
               for (int i = 0; i < 16; ++i) o[i] *= f;
               tmem_st16(tm_o + c, reinterpret_cast<const uint32_t*>(o));
@@ -347,26 +392,29 @@ __global__ void __launch_bounds__(kFwThreads, 1)
         const float2 sc = make_float2(sl2, sl2), no2 = make_float2(-off, -off);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          if (c < nch) {
-            tmem_wait_ld32(s[c & 1]);
-            if (c < 3 && c + 1 < nch) tmem_ld32(tm_s + 32 * (c + 1), s[(c + 1) & 1]);
-            float* v = s[c & 1];
-            if (!full) {
-              const uint32_t bits = seen_bits(lo, hi, sink, 32 * c);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = (bits >> i & 1u) ? v[i] : -INFINITY;
-            }
-            uint32_t w[16];
+          tmem_wait_values<32>(s[c & 1]);
+          if (c < 3 && (some >> (c + 1) & 1u)) tmem_ld32(tm_s + 32 * (c + 1), s[(c + 1) & 1]);
+          if (c == 3 && kOwnP) {  // S is in registers: the next one may be computed
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_free[u]);
+          }
+          uint32_t w[16];
+          if (some >> c & 1u) {
+            if (!(all >> c & 1u)) mask32(s[c & 1], bits[c]);
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
-              float2 e = fma2(make_float2(v[i], v[i + 1]), sc, no2);
+              float2 e = fma2(make_float2(s[c & 1][i], s[c & 1][i + 1]), sc, no2);
               e.x = ex2(e.x);
               e.y = ex2(e.y);
-              l2 = add2(l2, e);
+              l2[(i >> 1) & 1] = add2(l2[(i >> 1) & 1], e);
               w[i / 2] = pack2<BF16>(e.x, e.y);
             }
-            tmem_st16(tm_s + 16 * c, w);  // P's columns lie in S's first half, which this sweep has passed
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = 0u;
           }
+          tmem_st16(tm_p + 16 * c, w);  // over S, its columns are ones that this sweep has passed
         }
         tmem_wait_st();
         tc_fence_before();
@@ -375,25 +423,25 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       }
       if (!ok) break;
       if (b > a) {
-        if (!warp_wait(&pv_done[u], (ns - 1) & 1, abort_flag, p.err)) break;
+        if (!wait_phase(&pv_done[u], (ns - 1) & 1, abort_flag, p.err)) break;
         tc_fence_after();
       }
-      const float l = l2.x + l2.y;
+      const float l = l2[0].x + l2[0].y + l2[1].x + l2[1].y;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const long long orow = (long long)(it.tok + u * TT + t_row) * p.hq + it.hk * G + g;
       uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + orow * D);
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
-        float o[32];
+        float* o = s[0];
         if (b > a) {
           tmem_ld32(tm_o + c, o);
-          tmem_wait_ld32(o);
+          tmem_wait_values<32>(o);
         }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = l == 0.f ? 0.f : o[i] * inv;
-        if (live) {
+        for (int i = 0; i < 32; i += 8) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8)
+          for (int j = i; j < i + 8; ++j) o[j] = l == 0.f ? 0.f : o[j] * inv;
+          if (live)
             out[(c + i) / 8] = make_uint4(pack2<BF16>(o[i], o[i + 1]), pack2<BF16>(o[i + 2], o[i + 3]),
                                           pack2<BF16>(o[i + 4], o[i + 5]), pack2<BF16>(o[i + 6], o[i + 7]));
         }

@@ -24,6 +24,26 @@ struct TileShape {
   static constexpr int bytes(int rows) { return rows * 2 * D; }
 };
 
+// Waits for a barrier's phase, bounded like common.cuh's waits (kWaitLimitNs at
+// 2 GHz) but on the cycle counter: %globaltimer takes some 500 cycles to read,
+// which every wait that is not over at once would pay before it looks again.
+// All lanes of a warp call it; false when this or another wait of the CTA ran out.
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err) {
+  bool ok = mbar_test(bar, parity);
+  if (!ok) {
+    const long long t0 = clock64();
+    while (!(ok = mbar_test(bar, parity))) {
+      if (*abort_flag) break;
+      if (clock64() - t0 > 2 * (long long)kWaitLimitNs) {
+        *abort_flag = 1;
+        if (err) atomicOr(err, LSRM_ERR_TIMEOUT);
+        break;
+      }
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+
 // Descriptors of a [rows][D] tile at shared address `base`: as a K-major
 // operand (the contraction runs over D; step ks takes 16 channels), and as an
 // MN-major one (the contraction runs over the rows; step ks takes 16 of them).
@@ -100,6 +120,29 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   return r;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+__device__ __forceinline__ float max32(const float* s) {
+  float m[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    m[j] = fmaxf(s[j], s[j + 4]);
+#pragma unroll
+    for (int i = 8; i < 32; i += 8) m[j] = max3(m[j], s[i + j], s[i + j + 4]);
+  }
+  return fmaxf(max3(m[0], m[1], m[2]), m[3]);
+}
+
+// Scores outside `bits` to -inf (whatever they hold).
+__device__ __forceinline__ void mask32(float* s, uint32_t bits) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) s[i] = (bits >> i & 1u) ? s[i] : -INFINITY;
+}
+
 // Keys that one row sees, before the window and the sinks are merged: [lo, hi)
 // and [0, sink).
 struct RowKeys {
@@ -113,16 +156,13 @@ __device__ __forceinline__ RowKeys row_keys(const WindowParams& p, int pos, int 
   return r;
 }
 
-// Waits for the outstanding TMEM loads, and ties the 32 values of one of them
+// Waits for the outstanding TMEM loads, and ties the N values of one of them
 // to the wait: nothing that reads them may be scheduled ahead of it.
-__device__ __forceinline__ void tmem_wait_ld32(float* v) {
+template <int N>
+__device__ __forceinline__ void tmem_wait_values(float* v) {
   tmem_wait_ld();
-  asm volatile(""
-               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
-               "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]),
-               "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]),
-               "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]),
-               "+f"(v[29]), "+f"(v[30]), "+f"(v[31]));
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+f"(v[i]));
 }
 
 template <int N>
