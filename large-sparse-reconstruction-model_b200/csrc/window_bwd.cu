@@ -1,149 +1,965 @@
-// Attention with a sliding window and a few first tokens that stay visible
-// (sinks): forward and backward over packed sequences, grouped query heads.
-//   s_ij = scale q_i . k_j over the keys that window_common.cuh names,
-//   lse_i = log sum_j exp s_ij,  o_i = sum_j exp(s_ij - lse_i) v_j
-// (a query that sees no key: o = 0, lse = -inf).  Backward:
-//   delta_i = o_i . do_i,  p = exp(s - lse),  ds = p (do_i . v_j - delta_i)
-//   dq_i = scale sum_j ds k_j,  dk_j = scale sum_i ds q_i,  dv_j = sum_i p do_i
-// with the query heads of a group summed into their kv head.
+// Backward of the attention with a sliding window and sinks:
+//   delta_i = o_i . do_i,  p_ij = exp(s_ij - lse_i),  ds_ij = p_ij (do_i . v_j - delta_i)
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij do_i
+// with the query heads of a group summed into their kv head.  Scores are
+// recomputed from q, k and the forward's lse.
 //
-// A warp owns a query (forward, dq) or a key (dk, dv); its lanes take 32 keys
-// (queries) at a time for the scores and the channels for the sums.
-#include <algorithm>
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
+// Two passes, one that keeps query rows (dQ, built like the forward) and one
+// that keeps key rows (dK, dV), so that every sum is taken by one CTA in a
+// fixed order: no atomics, the same bits every time, at the price of computing
+// S and dP twice (seven products in place of five).  Rounding: P and dS are
+// rounded once to the operand type, everything else is fp32.
+//
+// Sinks are seen by every later query.  The key tile that holds them sums the
+// queries that its window reaches; the queries past it are cut into chunks
+// that are items of their own, with fp32 partial sums that sink_sum_kernel adds
+// in ascending order.
 #include "window_host.h"
+#include "window_tile.cuh"
 
 namespace lsrm {
 namespace {
 
-template <typename T>
-__device__ __forceinline__ float dot_row(const float* a, const T* b, int d) {
-  float s = 0.f;
-  for (int c = 0; c < d; c += 8) {
-    const uint4 u = *reinterpret_cast<const uint4*>(b + c);
-    const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s = fmaf(a[c + i], (float)e[i], s);
-  }
-  return s;
-}
-
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
 struct WindowBwdParams : WindowParams {
-  const void* dout;  // [total_q, hq, D]
-  float* delta;      // [total_q, hq]
+  const void* dout;    // [total_q, hq, D]
+  float* delta;        // [total_q, hq]
   void *dq, *dk, *dv;
+  // sinks past the window's reach
+  int chunk;           // query tokens per partial sum (0: no sinks)
+  int chunk_slots;
+  float* part0;        // [num_seqs][hkv][sinks][2][D] fp32: dv, dk of the sinks' own tile
+  float* part;         // [chunk_slots][hkv][sinks][2][D]
 };
 
+// delta = rowsum(o * do), D / 8 lanes a row.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) window_dq_kernel(const WindowBwdParams p) {
-  __shared__ float sq[4][D], sdo[4][D];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * 4 + warp;
-  if (row >= (long long)p.total_q * p.hq) return;
-  const int tok = (int)(row / p.hq), h = (int)(row % p.hq), hk = h / p.g;
-  const int b = seq_of_token(p.cu_q, p.num_seqs, tok);
-  const Seq s_ = seq_of(p, b);
-  const int pos = tok - s_.q0 + s_.lk - s_.lq;
-  const Seen seen = keys_of(p, pos, s_.lk, b < p.num_seqs);
-  const T* q = static_cast<const T*>(p.q) + tok * p.q_stride + h * D;
-  const T* dout = static_cast<const T*>(p.dout) + row * D;
-  const T* out = static_cast<const T*>(p.out) + row * D;
-  float delta = 0.f;
-  for (int d = lane; d < D; d += 32) {
-    sq[warp][d] = (float)q[d] * p.scale;
-    sdo[warp][d] = (float)dout[d];
-    delta += (float)dout[d] * (float)out[d];
-  }
-  delta = warp_sum(delta);
-  if (lane == 0) p.delta[row] = delta;
-  __syncwarp();
-  const float lse = p.lse[row];
-  const T* k = static_cast<const T*>(p.k) + s_.k0 * p.k_stride + hk * D;
-  const T* v = static_cast<const T*>(p.v) + s_.k0 * p.v_stride + hk * D;
-  float acc[D / 32];
+__global__ void __launch_bounds__(256) window_delta_kernel(const uint4* __restrict__ o, const uint4* __restrict__ d,
+                                                           float* __restrict__ delta, long long rows) {
+  constexpr int GL = D / 8;
+  const long long stride = (long long)gridDim.x * blockDim.x;
+  const long long n = rows * GL, top = (n + 31) / 32 * 32;  // whole warps take part in the shuffles
+  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < top; i += stride) {
+    float s = 0.f;
+    if (i < n) {
+      const uint4 a = o[i], b = d[i];
+      const T *x = reinterpret_cast<const T*>(&a), *y = reinterpret_cast<const T*>(&b);
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
-  const int n = lse == -INFINITY ? 0 : seen.sink + seen.hi - seen.lo;
-  for (int base = 0; base < n; base += 32) {
-    const int idx = base + lane;
-    const int j = idx < seen.sink ? idx : seen.lo + idx - seen.sink;
-    float ds = 0.f;
-    if (idx < n) {
-      const float pr = expf(dot_row(sq[warp], k + j * p.k_stride, D) - lse);
-      ds = pr * (dot_row(sdo[warp], v + j * p.v_stride, D) - delta);
+      for (int j = 0; j < 8; ++j) s = fmaf((float)x[j], (float)y[j], s);
     }
-    const int cnt = min(32, n - base);
-    for (int t = 0; t < cnt; ++t) {
-      const float dt = __shfl_sync(0xffffffffu, ds, t);
-      const int jt = __shfl_sync(0xffffffffu, j, t);
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(dt, (float)k[jt * p.k_stride + lane + 32 * i], acc[i]);
-    }
+    for (int k = GL / 2; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
+    if (i < n && i % GL == 0) delta[i / GL] = s;
   }
-  T* dq = static_cast<T*>(p.dq) + row * D;
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) dq[lane + 32 * i] = (T)(acc[i] * p.scale);
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(128) window_dkv_kernel(const WindowBwdParams p) {
-  __shared__ float sk[4][D], sv[4][D];
+// ------------------------------- dQ ----------------------------------------
+// As the forward: a persistent CTA, two tiles of 128 packed query rows, key
+// tiles of 64 (S, dP and dQ of both row tiles fill TMEM at 128 channels).
+
+constexpr int kBwThreads = 352;
+constexpr int kDqKeys = 64;
+
+template <int D>
+struct DqSmem {
+  static constexpr int QT = TileShape<D>::bytes(128), KT = TileShape<D>::bytes(kDqKeys);
+  static constexpr int NQ = D == 128 ? 1 : 2;  // Q and dO buffers of each row tile
+  static constexpr int NS = D == 128 ? 6 : 8;  // K / V ring
+  static constexpr int OFF_KV = 4 * NQ * QT;   // [row tile][buffer][Q, dO]
+  static constexpr int OFF_ITEM = OFF_KV + NS * KT;
+  static constexpr int OFF_BAR = OFF_ITEM + kItems * (int)sizeof(RowItem);
+  // q_full[2][NQ], q_empty[2][NQ], kv_full[NS], kv_empty[NS], s_full[2], s_free[2], ds_full[2], dq_done[2],
+  // item_full[], item_empty[], mma_done[2]
+  static constexpr int NBAR = 4 * NQ + 2 * NS + 8 + 2 * kItems + 2;
+  static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
+  static constexpr int BYTES = OFF_MISC + 16 + 1024;
+  static constexpr int ALLOC = BYTES > kOneCtaPerSmSmem ? BYTES : kOneCtaPerSmSmem;
+  static_assert(OFF_BAR % 8 == 0 && ALLOC <= 227 * 1024, "shared memory budget");
+};
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kBwThreads, 1)
+    window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
+                     const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                     const WindowBwdParams p, const int n_items) {
+  using L = DqSmem<D>;
+  constexpr uint32_t AB = BF16 ? 1u : 0u;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sKV = smem + L::OFF_KV;
+  RowItem* items = reinterpret_cast<RowItem*>(smem + L::OFF_ITEM);
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
+  uint64_t* q_empty = q_full + 2 * L::NQ;
+  uint64_t* kv_full = q_empty + 2 * L::NQ;
+  uint64_t* kv_empty = kv_full + L::NS;
+  uint64_t* s_full = kv_empty + L::NS;
+  uint64_t* s_free = s_full + 2;
+  uint64_t* ds_full = s_free + 2;
+  uint64_t* dq_done = ds_full + 2;
+  uint64_t* item_full = dq_done + 2;
+  uint64_t* item_empty = item_full + kItems;
+  uint64_t* mma_done = item_empty + kItems;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
+
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long row = (long long)blockIdx.x * 4 + warp;
-  if (row >= (long long)p.total_k * p.hkv) return;
-  const int tok = (int)(row / p.hkv), hk = (int)(row % p.hkv);
-  const int b = seq_of_token(p.cu_k, p.num_seqs, tok);
-  const Seq s_ = seq_of(p, b);
-  const int j = tok - s_.k0, shift = s_.lk - s_.lq;
-  // queries at positions [j - right, j + left] see key j; a sink is seen by all (causal: from j on)
-  int i0 = max(0, j - p.right - shift), i1 = min(s_.lq, j + p.left + 1 - shift);
-  if (j < p.sinks) {
-    if (!p.causal) i0 = 0;
-    i1 = s_.lq;
+  const int G = p.g, TT = 128 / G;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2 * L::NQ; ++i) mbar_init(&q_full[i], 1), mbar_init(&q_empty[i], 1);
+    for (int i = 0; i < L::NS; ++i) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], 2);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_free[i], 4);
+      mbar_init(&ds_full[i], 4);
+      mbar_init(&dq_done[i], 1);
+      mbar_init(&mma_done[i], 1);
+    }
+    for (int i = 0; i < kItems; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 10);
+    *abort_flag = 0;
+    fence_mbar_init();
   }
-  if (b >= p.num_seqs) i1 = i0;
-  const T* k = static_cast<const T*>(p.k) + tok * p.k_stride + hk * D;
-  const T* v = static_cast<const T*>(p.v) + tok * p.v_stride + hk * D;
-  for (int d = lane; d < D; d += 32) sk[warp][d] = (float)k[d] * p.scale, sv[warp][d] = (float)v[d];
-  __syncwarp();
-  float dk[D / 32], dv[D / 32];
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i) dk[i] = dv[i] = 0.f;
-  for (int base = i0; base < i1; base += 32) {
-    const int i = base + lane, cnt = min(32, i1 - base);
-    for (int h = hk * p.g; h < (hk + 1) * p.g; ++h) {
-      float pr = 0.f, ds = 0.f;
-      if (i < i1) {
-        const long long r = (long long)(s_.q0 + i) * p.hq + h;
-        pr = expf(dot_row(sk[warp], static_cast<const T*>(p.q) + (s_.q0 + i) * p.q_stride + h * D, D) - p.lse[r]);
-        ds = pr * (dot_row(sv[warp], static_cast<const T*>(p.dout) + r * D, D) - p.delta[r]);
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // TMEM columns per row tile u: S [128 u, +64), dP [128 u + 64, +64), dQ [256 + u D, + D), and dS (32) in
+  // [384 + 32 u, +32) up to D = 64, else over S
+  constexpr bool kOwnDs = D <= 64;
+
+  if (warp == 10) {
+    // ------------------------------ producer ------------------------------
+    if (elect_one()) {
+      tma_prefetch_desc(&tm_q);
+      tma_prefetch_desc(&tm_do);
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+    }
+    const uint32_t q_bytes = (uint32_t)(2 * G * TT * D * 2);
+    int n_it = 0, J = 0, nq[2] = {0, 0};
+    bool ok = true;
+    for (int w = blockIdx.x; ok; w += gridDim.x) {
+      RowItem it;
+      it.stop = w >= n_items;
+      if (!it.stop && !row_item<kDqKeys>(p, w, TT, it)) continue;
+      const int r = n_it % kItems;
+      if (!wait_phase(&item_empty[r], ((n_it / kItems) & 1) ^ 1, abort_flag, p.err)) break;
+      if (lane == 0) {
+        items[r] = it;
+        mbar_arrive(&item_full[r]);
       }
-      for (int t = 0; t < cnt; ++t) {
-        const float pt = __shfl_sync(0xffffffffu, pr, t), dt = __shfl_sync(0xffffffffu, ds, t);
-        const T* q = static_cast<const T*>(p.q) + (s_.q0 + base + t) * p.q_stride + h * D;
-        const T* dout = static_cast<const T*>(p.dout) + ((long long)(s_.q0 + base + t) * p.hq + h) * D;
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          dk[c] = fmaf(dt, (float)q[lane + 32 * c], dk[c]);
-          dv[c] = fmaf(pt, (float)dout[lane + 32 * c], dv[c]);
+      __syncwarp();
+      ++n_it;
+      if (it.stop) break;
+      for (int u = 0; u < 2 && ok; ++u) {
+        if (it.b[u] <= it.a[u]) continue;
+        const int st = u * L::NQ + nq[u] % L::NQ;
+        if (!(ok = wait_phase(&q_empty[st], ((nq[u] / L::NQ) & 1) ^ 1, abort_flag, p.err))) break;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&q_full[st], q_bytes);
+          load_tile<D>(sQ + 2 * st * L::QT, 128, &tm_q, it.hk * G, it.tok + u * TT, &q_full[st]);
+          load_tile<D>(sQ + (2 * st + 1) * L::QT, 128, &tm_do, it.hk * G, it.tok + u * TT, &q_full[st]);
+        }
+        __syncwarp();
+        ++nq[u];
+      }
+      for (int t = 0; t < it.tiles && ok; ++t) {
+        const int key = it.key0 + it.key<kDqKeys>(t);
+        for (int kv = 0; kv < 2; ++kv) {
+          const int st = J % L::NS;
+          if (!(ok = wait_phase(&kv_empty[st], ((J / L::NS) & 1) ^ 1, abort_flag, p.err))) break;
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&kv_full[st], L::KT);
+            load_tile<D>(sKV + st * L::KT, kDqKeys, kv ? &tm_v : &tm_k, it.hk, key, &kv_full[st]);
+          }
+          __syncwarp();
+          ++J;
         }
       }
     }
-  }
+    if (lane == 0 && *abort_flag) {  // copies in flight land before the CTA exits
+      for (int u = 0; u < 2; ++u)
+        for (int k = max(0, nq[u] - L::NQ); k < nq[u]; ++k)
+          mbar_wait_drain(&q_full[u * L::NQ + k % L::NQ], (k / L::NQ) & 1);
+      for (int j = max(0, J - L::NS); j < J; ++j) mbar_wait_drain(&kv_full[j % L::NS], (j / L::NS) & 1);
+    }
+    __syncwarp();
+  } else if (warp >= 8) {
+    // --------------------------- tensor-core issue ---------------------------
+    const int u = warp - 8;
+    const uint32_t tm_s = tmem + u * 128, tm_dp = tm_s + 64, tm_dq = tmem + 256 + u * D;
+    const uint32_t tm_ds = kOwnDs ? tmem + 384 + 32 * u : tm_s;
+    const uint32_t idesc_s = make_idesc(AB, 0, 0, 128, kDqKeys), idesc_q = make_idesc(AB, 0, 1, 128, D);
+    int n_it = 0, J = 0, nq = 0, ns = 0, np = 0;  // items, ring slots, Q tiles, S and dQ products so far
+    while (true) {
+      const int r = n_it % kItems;
+      if (!wait_phase(&item_full[r], (n_it / kItems) & 1, abort_flag, p.err)) break;
+      const RowItem& it = items[r];
+      ++n_it;
+      if (it.stop) break;
+      const int st_q = u * L::NQ + nq % L::NQ;
+      const uint32_t q_base = smem_u32(sQ + 2 * st_q * L::QT), do_base = q_base + L::QT;
+      const int a = it.a[u], b = it.b[u];
+      auto wait_slot = [&](int j) { return wait_phase(&kv_full[j % L::NS], (j / L::NS) & 1, abort_flag, p.err); };
+      auto pass = [&](int t) {  // keys that only the other row tile sees
+        if (!wait_slot(J + 2 * t) || !wait_slot(J + 2 * t + 1)) return false;
+        if (lane == 0) {
+          mbar_arrive(&kv_empty[(J + 2 * t) % L::NS]);
+          mbar_arrive(&kv_empty[(J + 2 * t + 1) % L::NS]);
+        }
+        __syncwarp();
+        return true;
+      };
+      auto issue_s = [&](int t) {
+        const int sk = (J + 2 * t) % L::NS, sv = (J + 2 * t + 1) % L::NS;
+        if (!wait_slot(J + 2 * t) || !wait_slot(J + 2 * t + 1)) return false;
+        // the last S and dP have been read; where dS lies over S, the product that reads it is over
+        if (kOwnDs && ns > 0 && !wait_phase(&s_free[u], (ns - 1) & 1, abort_flag, p.err)) return false;
+        if (!kOwnDs && np > 0 && !wait_phase(&dq_done[u], (np - 1) & 1, abort_flag, p.err)) return false;
+        ++ns;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t k_base = smem_u32(sKV + sk * L::KT), v_base = smem_u32(sKV + sv * L::KT);
 #pragma unroll
-  for (int c = 0; c < D / 32; ++c) {
-    static_cast<T*>(p.dk)[row * D + lane + 32 * c] = (T)(dk[c] * p.scale);
-    static_cast<T*>(p.dv)[row * D + lane + 32 * c] = (T)dv[c];
+          for (int ks = 0; ks < D / 16; ++ks)
+            umma_f16(tm_s, desc_k<D>(q_base, 128, ks), desc_k<D>(k_base, kDqKeys, ks), idesc_s, ks > 0);
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks)
+            umma_f16(tm_dp, desc_k<D>(do_base, 128, ks), desc_k<D>(v_base, kDqKeys, ks), idesc_s, ks > 0);
+          umma_commit(&s_full[u]);
+          umma_commit(&kv_empty[sv]);
+          if (t == b - 1) umma_commit(&q_empty[st_q]);
+        }
+        __syncwarp();
+        return true;
+      };
+      bool ok = true;
+      for (int t = 0; t < a && ok; ++t) ok = pass(t);
+      if (ok && b > a) {
+        ok = wait_phase(&q_full[st_q], (nq / L::NQ) & 1, abort_flag, p.err) && issue_s(a);
+        ++nq;
+      }
+      for (int t = a; t < b && ok; ++t) {
+        if (kOwnDs && t + 1 < b && !(ok = issue_s(t + 1))) break;
+        const int st = (J + 2 * t) % L::NS, valid = it.valid<kDqKeys>(t);
+        if (valid < kDqKeys) zero_rows<D>(sKV + st * L::KT, kDqKeys, valid);
+        if (!(ok = wait_phase(&ds_full[u], np & 1, abort_flag, p.err))) break;
+        ++np;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t k_base = smem_u32(sKV + st * L::KT);
+#pragma unroll
+          for (int ks = 0; ks < kDqKeys / 16; ++ks)
+            umma_f16_ts(tm_dq, tm_ds + ks * 8, desc_mn<D>(k_base, kDqKeys, ks), idesc_q, (t > a || ks > 0) ? 1u : 0u);
+          umma_commit(&dq_done[u]);
+          umma_commit(&kv_empty[st]);
+        }
+        __syncwarp();
+        if (!kOwnDs && t + 1 < b) ok = issue_s(t + 1);
+      }
+      for (int t = b > a ? b : a; t < it.tiles && ok; ++t) ok = pass(t);
+      if (!ok) break;
+      J += 2 * it.tiles;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[r]);
+    }
+    if (elect_one()) {
+      umma_commit(&mma_done[u]);
+      mbar_wait_drain(&mma_done[u], 0);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------ dS -------------------------------------
+    // A thread owns a row: p = exp2(s - lse), ds = p (dp - delta).
+    const int u = warp >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const int t_row = row / G, g = row - t_row * G;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t tm_s = tmem + u * 128 + lanes, tm_dp = tm_s + 64, tm_dq = tmem + 256 + u * D + lanes;
+    const uint32_t tm_ds = (kOwnDs ? tmem + 384 + 32 * u : tmem + u * 128) + lanes;
+    const float sl2 = p.scale * 1.4426950408889634f;
+    int n_it = 0, ns = 0;
+    while (true) {
+      const int r = n_it % kItems;
+      if (!wait_phase(&item_full[r], (n_it / kItems) & 1, abort_flag, p.err)) break;
+      const RowItem& it = items[r];
+      ++n_it;
+      if (it.stop) break;
+      const int a = it.a[u], b = it.b[u];
+      const bool live = t_row < it.n[u] && t_row < TT;
+      const RowKeys keys = row_keys(p, it.pos + u * TT + t_row, it.lk);
+      const long long orow = (long long)(it.tok + u * TT + t_row) * p.hq + it.hk * G + g;
+      float lse2 = live ? p.lse[orow] * 1.4426950408889634f : 0.f;
+      if (lse2 == -INFINITY) lse2 = 0.f;  // a row that sees nothing: every column is masked
+      const float delta = live ? p.delta[orow] : 0.f;
+      const float2 sc = make_float2(sl2, sl2), nl = make_float2(-lse2, -lse2), nd = make_float2(-delta, -delta);
+      bool ok = true;
+      float s[32], d[32];
+      for (int t = a; t < b; ++t) {
+        const int key = it.key<kDqKeys>(t);
+        const bool sinks_only = t < it.sep;
+        const int lo = sinks_only ? 0 : keys.lo - key, hi = sinks_only ? 0 : keys.hi - key;
+        const int sink = it.sep && !sinks_only ? 0 : keys.sink - key;
+        uint32_t bits[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) bits[c] = live ? seen_bits(lo, hi, sink, 32 * c) : 0u;
+        if (!(ok = wait_phase(&s_full[u], ns & 1, abort_flag, p.err))) break;
+        ++ns;
+        tc_fence_after();
+        uint32_t w[2][16];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (__any_sync(0xffffffffu, bits[c] != 0u)) {
+            tmem_ld32(tm_s + 32 * c, s);
+            tmem_ld32(tm_dp + 32 * c, d);
+            tmem_wait_values<32>(s);
+            tmem_wait_values<32>(d);
+            const bool full = __all_sync(0xffffffffu, !live || bits[c] == 0xffffffffu);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float2 e = fma2(make_float2(s[i], s[i + 1]), sc, nl);
+              e.x = ex2(e.x);
+              e.y = ex2(e.y);
+              e = mul2(e, add2(make_float2(d[i], d[i + 1]), nd));
+              s[i] = e.x;
+              s[i + 1] = e.y;
+            }
+            if (!full) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) s[i] = (bits[c] >> i & 1u) ? s[i] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) w[c][i / 2] = pack2<BF16>(s[i], s[i + 1]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[c][i] = 0u;
+          }
+        }
+        if (kOwnDs) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[u]);
+          // dS's columns are free once the product of the tile before is over
+          if (t > a && !(ok = wait_phase(&dq_done[u], (ns - 2) & 1, abort_flag, p.err))) break;
+          tc_fence_after();
+        }
+        tmem_st16(tm_ds, w[0]);
+        tmem_st16(tm_ds + 16, w[1]);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ds_full[u]);
+      }
+      if (!ok) break;
+      if (b > a) {
+        if (!wait_phase(&dq_done[u], (ns - 1) & 1, abort_flag, p.err)) break;
+        tc_fence_after();
+      }
+      uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.dq) + orow * D);
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        if (b > a) {
+          tmem_ld32(tm_dq + c, s);
+          tmem_wait_values<32>(s);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+#pragma unroll
+          for (int j = i; j < i + 8; ++j) s[j] = b > a ? s[j] * p.scale : 0.f;
+          if (live)
+            out[(c + i) / 8] = make_uint4(pack2<BF16>(s[i], s[i + 1]), pack2<BF16>(s[i + 2], s[i + 3]),
+                                          pack2<BF16>(s[i + 4], s[i + 5]), pack2<BF16>(s[i + 6], s[i + 7]));
+        }
+      }
+      tc_fence_before();  // dQ is read before this warp's next dS lets the next item overwrite it
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[r]);
+    }
   }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+// ----------------------------- dK and dV ------------------------------------
+// A persistent CTA keeps 128 keys of a kv head and walks the queries that see
+// them, 64 packed rows at a time:
+//   S^T = K Q^T, dP^T = V dO^T (128 keys x 64 rows, two TMEM stages)
+//   warps 0-3 (even query tiles), 4-7 (odd ones): a key a thread, P^T and dS^T
+//   as 16-bit operands in TMEM;  dV += P^T dO, dK += dS^T Q
+//   warp 8 issues, warp 9 loads, warp 10 gathers the rows' lse and delta.
+
+constexpr int kKvRows = 64;  // packed query rows of a tile
+
+struct KvItem {
+  int stop;
+  int hk, key;         // kv head, first key (global)
+  int nk, j0;          // keys, position of the first
+  int tok, ntok, pos;  // first query token (global), their number, the position of the first
+  int sinks_only;      // 1: a chunk of queries past the window's reach, for the sinks alone
+  float* part;         // where the sinks' sums go (fp32), or null
+};
+
+template <int D>
+struct KvSmem {
+  static constexpr int KT = TileShape<D>::bytes(128), QT = TileShape<D>::bytes(kKvRows);
+  static constexpr int NK = D == 128 ? 1 : 2;  // K and V buffers
+  static constexpr int NS = 4;                 // ring of (Q, dO, lse, delta)
+  static constexpr int OFF_Q = 2 * NK * KT;
+  static constexpr int OFF_STAT = OFF_Q + 2 * NS * QT;
+  static constexpr int OFF_ITEM = OFF_STAT + NS * 2 * kKvRows * 4;
+  static constexpr int OFF_BAR = OFF_ITEM + kItems * (int)sizeof(KvItem);
+  // k_full[NK], k_empty[NK], q_full[NS], stat_full[NS], q_empty[NS], s_full[2], p_full[2], acc_done[2], acc_full,
+  // acc_free, item_full[], item_empty[], mma_done
+  static constexpr int NBAR = 2 * NK + 3 * NS + 6 + 2 + 2 * kItems + 1;
+  static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
+  static constexpr int BYTES = OFF_MISC + 16 + 1024;
+  static constexpr int ALLOC = BYTES > kOneCtaPerSmSmem ? BYTES : kOneCtaPerSmSmem;
+  static_assert(OFF_BAR % 8 == 0 && OFF_STAT % 16 == 0 && ALLOC <= 227 * 1024, "shared memory budget");
+};
+
+// The queries that the window of keys [j0, j0 + nk) reaches, as token range
+// [first, last) of the sequence; from token 0 on for the tile of the sinks
+// (queries ahead of its window see them too).
+__device__ __forceinline__ void window_queries(const WindowParams& p, const Seq& s, int j0, int nk, int& first,
+                                               int& last) {
+  const int shift = s.lk - s.lq;
+  first = max(0, j0 - p.right - shift);
+  last = min(s.lq, j0 + nk + p.left - shift);
+  if (j0 == 0 && p.sinks > 0) first = 0;
+  if (last < first) last = first;
+}
+
+// Query tokens of chunk `c` of a sequence that see nothing of it but the sinks.
+__device__ __forceinline__ void sink_queries(const WindowParams& p, const Seq& s, int chunk, int c, int& first,
+                                             int& last) {
+  int a, b;
+  window_queries(p, s, 0, min(128, s.lk), a, b);
+  first = max(c * chunk, b);
+  last = s.lk > 0 ? min(s.lq, (c + 1) * chunk) : 0;
+  if (last < first) last = first;
+}
+
+__device__ __forceinline__ bool kv_item(const WindowBwdParams& p, int w, int D, KvItem& it) {
+  const int n_sink = p.chunk_slots * p.hkv;
+  const long long row = (long long)p.sinks * 2 * D;
+  it.sinks_only = w < n_sink;
+  it.part = nullptr;
+  if (it.sinks_only) {
+    const int slot = w / p.hkv;
+    it.hk = w - slot * p.hkv;
+    const int b = seq_of_slot(p.cu_q, p.num_seqs, p.chunk, slot);
+    if (b >= p.num_seqs) return false;
+    const Seq s = seq_of(p, b);
+    int first, last;
+    sink_queries(p, s, p.chunk, slot - (p.cu_q[b] / p.chunk + b), first, last);
+    if (last <= first) return false;
+    it.key = s.k0;
+    it.nk = min(p.sinks, s.lk);
+    it.j0 = 0;
+    it.tok = s.q0 + first;
+    it.ntok = last - first;
+    it.pos = first + s.lk - s.lq;
+    it.part = p.part + w * row;
+    return true;
+  }
+  w -= n_sink;
+  const int slot = w / p.hkv;
+  it.hk = w - slot * p.hkv;
+  const int b = seq_of_slot(p.cu_k, p.num_seqs, 128, slot);
+  const Seq s = seq_of(p, b);
+  it.j0 = (slot - (p.cu_k[b] / 128 + b)) * 128;
+  if (it.j0 < 0 || it.j0 >= s.lk) return false;
+  it.key = s.k0 + it.j0;
+  it.nk = min(128, s.lk - it.j0);
+  int first = 0, last = 0;
+  if (b < p.num_seqs) window_queries(p, s, it.j0, it.nk, first, last);
+  it.tok = s.q0 + first;
+  it.ntok = last - first;
+  it.pos = first + s.lk - s.lq;
+  if (it.j0 == 0 && p.sinks > 0 && b < p.num_seqs) it.part = p.part0 + (long long)(b * p.hkv + it.hk) * row;
+  return true;
+}
+
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kBwThreads, 1)
+    window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
+                      const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                      const WindowBwdParams p, const int n_items) {
+  using L = KvSmem<D>;
+  constexpr uint32_t AB = BF16 ? 1u : 0u;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sK = smem;                 // [NK][K, V]
+  uint8_t* sQ = smem + L::OFF_Q;      // [NS][Q, dO]
+  float* stat = reinterpret_cast<float*>(smem + L::OFF_STAT);  // [NS][lse (log2), delta][64], negated
+  KvItem* items = reinterpret_cast<KvItem*>(smem + L::OFF_ITEM);
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
+  uint64_t* k_empty = k_full + L::NK;
+  uint64_t* q_full = k_empty + L::NK;
+  uint64_t* stat_full = q_full + L::NS;
+  uint64_t* q_empty = stat_full + L::NS;
+  uint64_t* s_full = q_empty + L::NS;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* acc_done = p_full + 2;
+  uint64_t* acc_full = acc_done + 2;
+  uint64_t* acc_free = acc_full + 1;
+  uint64_t* item_full = acc_free + 1;
+  uint64_t* item_empty = item_full + kItems;
+  uint64_t* mma_done = item_empty + kItems;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = p.g, TT = kKvRows / G;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::NK; ++i) mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1);
+    for (int i = 0; i < L::NS; ++i) mbar_init(&q_full[i], 1), mbar_init(&stat_full[i], 1), mbar_init(&q_empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&acc_done[i], 1);
+    mbar_init(acc_full, 1);
+    mbar_init(acc_free, 8);
+    for (int i = 0; i < kItems; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 10);
+    mbar_init(mma_done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // TMEM columns: stage st: S^T [128 st, +64), dP^T [128 st + 64, +64); dV [256, +D), dK [256 + D, +D); P^T and
+  // dS^T (32 each) of a stage in [384 + 64 st, +64) up to D = 64, else over its S^T and dP^T
+  constexpr bool kOwnP = D <= 64;
+
+  if (warp == 9) {
+    // ------------------------------ producer ------------------------------
+    if (elect_one()) {
+      tma_prefetch_desc(&tm_q);
+      tma_prefetch_desc(&tm_do);
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+    }
+    const uint32_t q_bytes = (uint32_t)(2 * G * TT * D * 2);
+    int n_it = 0, J = 0, nk = 0;
+    bool ok = true;
+    for (int w = blockIdx.x; ok; w += gridDim.x) {
+      KvItem it;
+      it.stop = w >= n_items;
+      if (!it.stop && !kv_item(p, w, D, it)) continue;
+      const int r = n_it % kItems;
+      if (!wait_phase(&item_empty[r], ((n_it / kItems) & 1) ^ 1, abort_flag, p.err)) break;
+      if (lane == 0) {
+        items[r] = it;
+        mbar_arrive(&item_full[r]);
+      }
+      __syncwarp();
+      ++n_it;
+      if (it.stop) break;
+      if (it.ntok <= 0) continue;
+      const int sk = nk % L::NK;
+      if (!(ok = wait_phase(&k_empty[sk], ((nk / L::NK) & 1) ^ 1, abort_flag, p.err))) break;
+      if (elect_one()) {
+        mbar_arrive_expect_tx(&k_full[sk], 2 * L::KT);
+        load_tile<D>(sK + 2 * sk * L::KT, 128, &tm_k, it.hk, it.key, &k_full[sk]);
+        load_tile<D>(sK + (2 * sk + 1) * L::KT, 128, &tm_v, it.hk, it.key, &k_full[sk]);
+      }
+      __syncwarp();
+      ++nk;
+      for (int t = 0; t * TT < it.ntok; ++t) {
+        const int st = J % L::NS;
+        if (!(ok = wait_phase(&q_empty[st], ((J / L::NS) & 1) ^ 1, abort_flag, p.err))) break;
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&q_full[st], q_bytes);
+          load_tile<D>(sQ + 2 * st * L::QT, kKvRows, &tm_q, it.hk * G, it.tok + t * TT, &q_full[st]);
+          load_tile<D>(sQ + (2 * st + 1) * L::QT, kKvRows, &tm_do, it.hk * G, it.tok + t * TT, &q_full[st]);
+        }
+        __syncwarp();
+        ++J;
+      }
+    }
+    if (lane == 0 && *abort_flag) {  // copies in flight land before the CTA exits
+      for (int k = max(0, nk - L::NK); k < nk; ++k) mbar_wait_drain(&k_full[k % L::NK], (k / L::NK) & 1);
+      for (int j = max(0, J - L::NS); j < J; ++j) mbar_wait_drain(&q_full[j % L::NS], (j / L::NS) & 1);
+    }
+    __syncwarp();
+  } else if (warp == 10) {
+    // -------------------- lse and delta of the query rows --------------------
+    int n_it = 0, J = 0;
+    bool ok = true;
+    while (ok) {
+      const int r = n_it % kItems;
+      if (!wait_phase(&item_full[r], (n_it / kItems) & 1, abort_flag, p.err)) break;
+      const KvItem& it = items[r];
+      ++n_it;
+      if (it.stop) break;
+      for (int t = 0; t * TT < it.ntok; ++t, ++J) {
+        float l[2], d[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = lane + 32 * i, tr = row / G, tok = t * TT + tr;
+          l[i] = d[i] = 0.f;
+          if (tr < TT && tok < it.ntok) {
+            const long long idx = (long long)(it.tok + tok) * p.hq + it.hk * G + row - tr * G;
+            l[i] = p.lse[idx] * -1.4426950408889634f;
+            d[i] = -p.delta[idx];
+            if (l[i] == INFINITY) l[i] = 0.f;  // sees nothing: every key is masked
+          }
+        }
+        const int st = J % L::NS;
+        if (!(ok = wait_phase(&q_empty[st], ((J / L::NS) & 1) ^ 1, abort_flag, p.err))) break;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          stat[(2 * st) * kKvRows + lane + 32 * i] = l[i];
+          stat[(2 * st + 1) * kKvRows + lane + 32 * i] = d[i];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&stat_full[st]);
+      }
+      if (!ok) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[r]);
+    }
+  } else if (warp == 8) {
+    // --------------------------- tensor-core issue ---------------------------
+    const uint32_t idesc_s = make_idesc(AB, 0, 0, 128, kKvRows), idesc_a = make_idesc(AB, 0, 1, 128, D);
+    const uint32_t tm_dv = tmem + 256, tm_dk = tmem + 256 + D;
+    int n_it = 0, J = 0, nk = 0, n_acc = 0;  // items, query tiles, K tiles, items with sums so far
+    while (true) {
+      const int r = n_it % kItems;
+      if (!wait_phase(&item_full[r], (n_it / kItems) & 1, abort_flag, p.err)) break;
+      const KvItem& it = items[r];
+      ++n_it;
+      if (it.stop) break;
+      const int n = (it.ntok + TT - 1) / TT;
+      bool ok = true;
+      if (n > 0) {
+        const int sk = nk % L::NK;
+        const uint32_t k_base = smem_u32(sK + 2 * sk * L::KT), v_base = k_base + L::KT;
+        if (!wait_phase(&k_full[sk], (nk / L::NK) & 1, abort_flag, p.err)) break;
+        ++nk;
+        auto issue_s = [&](int t) {
+          const int j = J + t, st = j % L::NS, stage = j & 1;
+          if (!wait_phase(&q_full[st], (j / L::NS) & 1, abort_flag, p.err)) return false;
+          // rows that hold no query of the sequence must not reach the sums, not even times zero
+          const int rows = min(TT, it.ntok - t * TT) * G;
+          if (rows < kKvRows) {
+            zero_rows<D>(sQ + 2 * st * L::QT, kKvRows, rows);
+            zero_rows<D>(sQ + (2 * st + 1) * L::QT, kKvRows, rows);
+          }
+          // S^T and dP^T of the stage's last tile were read before its P^T was announced; where P^T and dS^T lie
+          // over them, the sums that read those are over
+          if (!kOwnP && j >= 2 && !wait_phase(&acc_done[stage], ((j >> 1) & 1) ^ 1, abort_flag, p.err)) return false;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t q_base = smem_u32(sQ + 2 * st * L::QT), do_base = q_base + L::QT;
+            const uint32_t tm_s = tmem + stage * 128;
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks)
+              umma_f16(tm_s, desc_k<D>(k_base, 128, ks), desc_k<D>(q_base, kKvRows, ks), idesc_s, ks > 0);
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks)
+              umma_f16(tm_s + 64, desc_k<D>(v_base, 128, ks), desc_k<D>(do_base, kKvRows, ks), idesc_s, ks > 0);
+            umma_commit(&s_full[stage]);
+            if (t == n - 1) umma_commit(&k_empty[sk]);
+          }
+          __syncwarp();
+          return true;
+        };
+        ok = issue_s(0) && (n < 2 || issue_s(1));
+        for (int t = 0; t < n && ok; ++t) {
+          const int j = J + t, st = j % L::NS, stage = j & 1;
+          if (!(ok = wait_phase(&p_full[stage], (j >> 1) & 1, abort_flag, p.err))) break;
+          if (kOwnP && t + 2 < n && !(ok = issue_s(t + 2))) break;
+          // the last item's sums have been read
+          if (t == 0 && n_acc > 0 && !(ok = wait_phase(acc_free, (n_acc - 1) & 1, abort_flag, p.err))) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t q_base = smem_u32(sQ + 2 * st * L::QT), do_base = q_base + L::QT;
+            const uint32_t tm_p = kOwnP ? tmem + 384 + 64 * stage : tmem + 128 * stage;
+            const uint32_t tm_ds = kOwnP ? tm_p + 32 : tm_p + 64;
+#pragma unroll
+            for (int ks = 0; ks < kKvRows / 16; ++ks)
+              umma_f16_ts(tm_dv, tm_p + ks * 8, desc_mn<D>(do_base, kKvRows, ks), idesc_a, (t > 0 || ks > 0) ? 1u : 0u);
+#pragma unroll
+            for (int ks = 0; ks < kKvRows / 16; ++ks)
+              umma_f16_ts(tm_dk, tm_ds + ks * 8, desc_mn<D>(q_base, kKvRows, ks), idesc_a, (t > 0 || ks > 0) ? 1u : 0u);
+            umma_commit(&acc_done[stage]);
+            umma_commit(&q_empty[st]);
+            if (t == n - 1) umma_commit(acc_full);
+          }
+          __syncwarp();
+          if (!kOwnP && t + 2 < n) ok = issue_s(t + 2);
+        }
+        if (!ok) break;
+        ++n_acc;
+        J += n;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[r]);
+    }
+    if (elect_one()) {
+      umma_commit(mma_done);
+      mbar_wait_drain(mma_done, 0);
+    }
+    __syncwarp();
+  } else {
+    // --------------------------- P^T and dS^T --------------------------------
+    const int wg = warp >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t tm_s = tmem + wg * 128 + lanes, tm_dp = tm_s + 64;
+    const uint32_t tm_p = (kOwnP ? tmem + 384 + 64 * wg : tmem + 128 * wg) + lanes;
+    const uint32_t tm_ds = kOwnP ? tm_p + 32 : tm_p + 64;
+    const float sl2 = p.scale * 1.4426950408889634f;
+    const float2 sc = make_float2(sl2, sl2);
+    int n_it = 0, J = 0, n_acc = 0;
+    while (true) {
+      const int r = n_it % kItems;
+      if (!wait_phase(&item_full[r], (n_it / kItems) & 1, abort_flag, p.err)) break;
+      const KvItem& it = items[r];
+      ++n_it;
+      if (it.stop) break;
+      const int n = (it.ntok + TT - 1) / TT;
+      // queries that see this thread's key, as a token range of the item
+      const int j = it.j0 + row;
+      int lo = j - p.right - it.pos, hi = j + p.left + 1 - it.pos;
+      if (j < p.sinks) {
+        if (!p.causal) lo = 0;
+        hi = it.ntok;
+      } else if (it.sinks_only) {
+        hi = lo;
+      }
+      lo = max(lo, 0);
+      hi = min(hi, it.ntok);
+      const bool live = row < it.nk;
+      if (!live) hi = lo;
+      bool ok = true;
+      for (int t = (J & 1) ^ wg; t < n; t += 2) {
+        const int jt = J + t, st = jt % L::NS;
+        const int c_lo = (lo - t * TT) * G, c_hi = (min(hi, (t + 1) * TT) - t * TT) * G;
+        uint32_t bits[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) bits[c] = range_bits(c_lo - 32 * c, c_hi - 32 * c);
+        if (!(ok = wait_phase(&stat_full[st], (jt / L::NS) & 1, abort_flag, p.err))) break;
+        if (!(ok = wait_phase(&s_full[wg], (jt >> 1) & 1, abort_flag, p.err))) break;
+        tc_fence_after();
+        const float* nl = stat + (2 * st) * kKvRows;
+        const float* nd = nl + kKvRows;
+        if (kOwnP && jt >= 2) {  // P^T's and dS^T's columns are free once the sums of the stage's last tile are over
+          if (!(ok = wait_phase(&acc_done[wg], ((jt >> 1) & 1) ^ 1, abort_flag, p.err))) break;
+          tc_fence_after();
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t wp[16], wd[16];
+          if (__any_sync(0xffffffffu, bits[c] != 0u)) {
+            float s[32], d[32];
+            tmem_ld32(tm_s + 32 * c, s);
+            tmem_ld32(tm_dp + 32 * c, d);
+            tmem_wait_values<32>(s);
+            tmem_wait_values<32>(d);
+            const bool full = __all_sync(0xffffffffu, !live || bits[c] == 0xffffffffu);
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const float4 l4 = *reinterpret_cast<const float4*>(nl + 32 * c + i);
+              const float4 d4 = *reinterpret_cast<const float4*>(nd + 32 * c + i);
+              float2 e0 = fma2(make_float2(s[i], s[i + 1]), sc, make_float2(l4.x, l4.y));
+              float2 e1 = fma2(make_float2(s[i + 2], s[i + 3]), sc, make_float2(l4.z, l4.w));
+              e0.x = ex2(e0.x);
+              e0.y = ex2(e0.y);
+              e1.x = ex2(e1.x);
+              e1.y = ex2(e1.y);
+              float2 f0 = mul2(e0, add2(make_float2(d[i], d[i + 1]), make_float2(d4.x, d4.y)));
+              float2 f1 = mul2(e1, add2(make_float2(d[i + 2], d[i + 3]), make_float2(d4.z, d4.w)));
+              if (!full) {
+                const uint32_t b4 = bits[c] >> i;
+                e0.x = (b4 & 1u) ? e0.x : 0.f, f0.x = (b4 & 1u) ? f0.x : 0.f;
+                e0.y = (b4 & 2u) ? e0.y : 0.f, f0.y = (b4 & 2u) ? f0.y : 0.f;
+                e1.x = (b4 & 4u) ? e1.x : 0.f, f1.x = (b4 & 4u) ? f1.x : 0.f;
+                e1.y = (b4 & 8u) ? e1.y : 0.f, f1.y = (b4 & 8u) ? f1.y : 0.f;
+              }
+              wp[i / 2] = pack2<BF16>(e0.x, e0.y);
+              wp[i / 2 + 1] = pack2<BF16>(e1.x, e1.y);
+              wd[i / 2] = pack2<BF16>(f0.x, f0.y);
+              wd[i / 2 + 1] = pack2<BF16>(f1.x, f1.y);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) wp[i] = wd[i] = 0u;
+          }
+          tmem_st16(tm_p + 16 * c, wp);  // over S^T and dP^T, the columns are ones that have been read
+          tmem_st16(tm_ds + 16 * c, wd);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[wg]);
+      }
+      if (!ok) break;
+      J += n;
+      if (n > 0) {
+        if (!wait_phase(acc_full, n_acc & 1, abort_flag, p.err)) break;
+        ++n_acc;
+        tc_fence_after();
+      }
+      // warps 0-3 write dV, warps 4-7 dK
+      const bool to_part = it.part && j < p.sinks;
+      const bool to_out = live && !it.sinks_only && !to_part;
+      const float mul = wg ? p.scale : 1.f;
+      uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(wg ? p.dk : p.dv) +
+                                            ((long long)(it.key + row) * p.hkv + it.hk) * D);
+      float4* part = to_part ? reinterpret_cast<float4*>(it.part + (long long)(j * 2 + wg) * D) : nullptr;
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        float s[32];
+        if (n > 0) {
+          tmem_ld32(tmem + 256 + wg * D + c + lanes, s);
+          tmem_wait_values<32>(s);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) s[i] = n > 0 ? s[i] * mul : 0.f;
+        if (to_out) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+            out[(c + i) / 8] = make_uint4(pack2<BF16>(s[i], s[i + 1]), pack2<BF16>(s[i + 2], s[i + 3]),
+                                          pack2<BF16>(s[i + 4], s[i + 5]), pack2<BF16>(s[i + 6], s[i + 7]));
+        } else if (to_part && live) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) part[(c + i) / 4] = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (n > 0) mbar_arrive(acc_free);
+        mbar_arrive(&item_empty[r]);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+// dv and dk of the sinks: their own tile's sum, then the chunks' in ascending
+// order (four interleaved runs, joined in order).  A block a sink.
+template <typename T, int D>
+__global__ void __launch_bounds__(4 * 2 * D) sink_sum_kernel(const WindowBwdParams p) {
+  __shared__ float sum[4][2 * D];
+  const int j = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, e = threadIdx.x;
+  const Seq s = seq_of(p, b);
+  if (j >= min(p.sinks, s.lk)) return;
+  const long long row = (long long)p.sinks * 2 * D;
+  const int slot0 = p.cu_q[b] / p.chunk + b;
+  float a = 0.f;
+  for (int c = threadIdx.y; c * p.chunk < s.lq; c += 4) {
+    int first, last;
+    sink_queries(p, s, p.chunk, c, first, last);
+    if (last > first) a += p.part[((long long)(slot0 + c) * p.hkv + hk) * row + j * 2 * D + e];
+  }
+  sum[threadIdx.y][e] = a;
+  __syncthreads();
+  if (threadIdx.y) return;
+  a = p.part0[(long long)(b * p.hkv + hk) * row + j * 2 * D + e];
+  for (int i = 0; i < 4; ++i) a += sum[i][e];
+  T* out = static_cast<T*>(e < D ? p.dv : p.dk);
+  out[((long long)(s.k0 + j) * p.hkv + hk) * D + e % D] = (T)a;
+}
+
+// Query tokens of a sink chunk: at least as many as a key tile's window
+// reaches, so that its item is no longer than they are, and never under 1024,
+// which bounds the partial sums' memory.
+int sink_chunk(const WindowParams& p) { return std::max(1024, 128 + p.left + p.right); }
+
+struct BwdLayout {
+  size_t delta, part0, part, bytes;
+  int chunk, slots;
+};
+
+BwdLayout bwd_layout(const WindowParams& p, int D) {
+  BwdLayout l{};
+  l.delta = 0;
+  size_t at = align_up((size_t)p.total_q * p.hq * sizeof(float), 256);
+  if (p.sinks > 0 && p.num_seqs > 0) {
+    l.chunk = sink_chunk(p);
+    l.slots = tile_slots(p.total_q, p.num_seqs, l.chunk);
+    const size_t row = (size_t)p.hkv * p.sinks * 2 * D * sizeof(float);
+    l.part0 = at;
+    at = align_up(at + p.num_seqs * row, 256);
+    l.part = at;
+    at = align_up(at + l.slots * row, 256);
+  }
+  l.bytes = at + 256;
+  return l;
+}
+
+template <int D, bool BF16>
+int launch_bwd(const WindowBwdParams& p, cudaStream_t s) {
+  using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
+  using S = TileShape<D>;
+  const int tt = 128 / p.g, tk = kKvRows / p.g;
+  int rc;
+  if (p.total_q > 0) {
+    ProfScope ps("window_attn_delta", s);
+    const long long rows = (long long)p.total_q * p.hq;
+    const int grid = (int)std::min<long long>((rows * (D / 8) + 255) / 256, (long long)num_sms() * 8);
+    window_delta_kernel<T, D><<<grid, 256, 0, s>>>(static_cast<const uint4*>(p.out), static_cast<const uint4*>(p.dout),
+                                                   p.delta, rows);
+    LSRM_LAUNCH_CHECK();
+  }
+  // no query or no key at all: the maps are never read
+  const void* q = p.total_q ? p.q : p.k;
+  const void* d = p.total_q ? p.dout : p.k;
+  const void* k = p.total_k ? p.k : p.q;
+  const void* v = p.total_k ? p.v : p.q;
+  const long long qs = p.total_q ? p.q_stride : p.k_stride, ds = p.total_q ? (long long)p.hq * D : p.k_stride;
+  const long long ks = p.total_k ? p.k_stride : p.q_stride, vs = p.total_k ? p.v_stride : p.q_stride;
+  CUtensorMap mq, md, mk, mv;
+  if (p.total_q > 0) {
+    if ((rc = make_tmap_3d(&mq, q, D, p.hq, p.total_q, qs, p.g, tt, S::kCols))) return rc;
+    if ((rc = make_tmap_3d(&md, d, D, p.hq, p.total_q, ds, p.g, tt, S::kCols))) return rc;
+    if ((rc = make_tmap_3d(&mk, k, D, p.hkv, p.total_k, ks, 1, kDqKeys, S::kCols))) return rc;
+    if ((rc = make_tmap_3d(&mv, v, D, p.hkv, p.total_k, vs, 1, kDqKeys, S::kCols))) return rc;
+    ProfScope ps("window_attn_dq", s);
+    const int n_items = tile_slots(p.total_q, p.num_seqs, 2 * tt) * p.hkv;
+    LSRM_CUDA_TRY(cudaFuncSetAttribute(window_dq_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       DqSmem<D>::ALLOC));
+    window_dq_kernel<D, BF16><<<std::min(n_items, num_sms()), kBwThreads, DqSmem<D>::ALLOC, s>>>(mq, md, mk, mv, p,
+                                                                                                 n_items);
+    LSRM_LAUNCH_CHECK();
+  }
+  if (p.total_k > 0) {
+    if ((rc = make_tmap_3d(&mq, q, D, p.hq, p.total_q, qs, p.g, tk, S::kCols))) return rc;
+    if ((rc = make_tmap_3d(&md, d, D, p.hq, p.total_q, ds, p.g, tk, S::kCols))) return rc;
+    if ((rc = make_tmap_3d(&mk, k, D, p.hkv, p.total_k, ks, 1, 128, S::kCols))) return rc;
+    if ((rc = make_tmap_3d(&mv, v, D, p.hkv, p.total_k, vs, 1, 128, S::kCols))) return rc;
+    {
+      ProfScope ps("window_attn_dkv", s);
+      const int n_items = (tile_slots(p.total_k, p.num_seqs, 128) + p.chunk_slots) * p.hkv;
+      LSRM_CUDA_TRY(cudaFuncSetAttribute(window_dkv_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         KvSmem<D>::ALLOC));
+      window_dkv_kernel<D, BF16><<<std::min(n_items, num_sms()), kBwThreads, KvSmem<D>::ALLOC, s>>>(mq, md, mk, mv, p,
+                                                                                                    n_items);
+      LSRM_LAUNCH_CHECK();
+    }
+    if (p.chunk) {
+      ProfScope ps("window_attn_sinks", s);
+      sink_sum_kernel<T, D><<<dim3(p.sinks, p.hkv, p.num_seqs), dim3(2 * D, 4), 0, s>>>(p);
+      LSRM_LAUNCH_CHECK();
+    }
+  }
+  return LSRM_OK;
 }
 
 }  // namespace
@@ -152,8 +968,12 @@ __global__ void __launch_bounds__(128) window_dkv_kernel(const WindowBwdParams p
 using namespace lsrm;
 
 extern "C" size_t lsrm_window_attn_workspace_bytes(const lsrm_window_shape* shape) {
-  if (!shape || shape->total_q < 0 || shape->num_q_heads < 1) return 0;
-  return align_up((size_t)shape->total_q * shape->num_q_heads * sizeof(float), 256) + 256;
+  if (!shape || shape->total_q < 0 || shape->total_k < 0 || shape->num_seqs < 0 || shape->num_kv_heads < 1 ||
+      shape->num_q_heads < 1 || shape->window < 1)
+    return 0;
+  return bwd_layout(window_params(shape, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr),
+                    shape->head_dim)
+      .bytes;
 }
 
 extern "C" int lsrm_window_attn_bwd(const lsrm_window_shape* shape, const int32_t* cu_seqlens_q,
@@ -166,31 +986,25 @@ extern "C" int lsrm_window_attn_bwd(const lsrm_window_shape* shape, const int32_
                  "out, lse, dout and the gradients must not be NULL");
   LSRM_CHECK_ARG((((uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) == 0,
                  "out, dout and the gradients must be 16-byte aligned");
+  LSRM_CHECK_ARG(shape->num_seqs <= 65535, "at most 65535 sequences");
   if (!workspace || workspace_bytes < lsrm_window_attn_workspace_bytes(shape)) {
     set_error("workspace too small: %zu bytes, %zu needed", workspace_bytes, lsrm_window_attn_workspace_bytes(shape));
     return LSRM_ERR_WORKSPACE;
   }
+  LSRM_CHECK_ARG(((uintptr_t)workspace & 255) == 0, "the workspace must be 256-byte aligned");
+  if (shape->total_q == 0 && shape->total_k == 0) return LSRM_OK;
   WindowBwdParams p;
   static_cast<WindowParams&>(p) = window_params(shape, cu_seqlens_q, cu_seqlens_k, q, k, v, const_cast<void*>(out),
                                                 const_cast<float*>(lse), err_flags);
   p.dout = dout, p.dq = dq, p.dk = dk, p.dv = dv;
-  p.delta = static_cast<float*>(workspace);
+  const BwdLayout l = bwd_layout(p, shape->head_dim);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.delta = reinterpret_cast<float*>(ws + l.delta);
+  p.chunk = l.chunk, p.chunk_slots = l.slots;
+  p.part0 = reinterpret_cast<float*>(ws + l.part0);
+  p.part = reinterpret_cast<float*>(ws + l.part);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (p.total_q > 0) {
-    ProfScope ps("window_attn_dq", s);
-    const unsigned grid = (unsigned)(((long long)p.total_q * p.hq + 3) / 4);
-#define CALL(BF, D) window_dq_kernel<std::conditional_t<BF, __nv_bfloat16, __half>, D><<<grid, 128, 0, s>>>(p);
-    WINDOW_TYPES(CALL)
+#define CALL(BF, D) return launch_bwd<D, BF>(p, s);
+  WINDOW_TYPES(CALL)
 #undef CALL
-    LSRM_LAUNCH_CHECK();
-  }
-  if (p.total_k > 0) {
-    ProfScope ps("window_attn_dkv", s);
-    const unsigned grid = (unsigned)(((long long)p.total_k * p.hkv + 3) / 4);
-#define CALL(BF, D) window_dkv_kernel<std::conditional_t<BF, __nv_bfloat16, __half>, D><<<grid, 128, 0, s>>>(p);
-    WINDOW_TYPES(CALL)
-#undef CALL
-    LSRM_LAUNCH_CHECK();
-  }
-  return LSRM_OK;
 }

@@ -25,19 +25,6 @@ namespace lsrm {
 namespace {
 
 constexpr int kFwThreads = 352;
-constexpr int kFwItems = 4;  // work items in flight between the producer and the other warps
-
-struct FwItem {
-  int stop;         // 1: no more items
-  int tok;          // first query token (global)
-  int n[2];         // query tokens of each row tile
-  int hk, pos, lk;  // kv head, position of the first query, keys of the sequence
-  int key0;         // first key of the sequence (global)
-  int tiles, sep;   // key tiles; 1: tile 0 holds the sinks alone, ahead of the window
-  int w0;           // first key of the window's first tile
-  int a[2], b[2];   // key tiles [a, b) of each row tile
-};
-
 template <int D>
 struct FwSmem {
   static constexpr int TILE = TileShape<D>::bytes(128);
@@ -45,51 +32,15 @@ struct FwSmem {
   static constexpr int NS = D == 128 ? 5 : 8;  // K / V ring
   static constexpr int OFF_KV = 2 * NQ * TILE;
   static constexpr int OFF_ITEM = OFF_KV + NS * TILE;
-  static constexpr int OFF_BAR = OFF_ITEM + kFwItems * (int)sizeof(FwItem);
+  static constexpr int OFF_BAR = OFF_ITEM + kItems * (int)sizeof(RowItem);
   // q_full[2][NQ], q_empty[2][NQ], kv_full[NS], kv_empty[NS], s_full[2], s_free[2], p_full[2], pv_done[2],
   // item_full[], item_empty[], mma_done[2]
-  static constexpr int NBAR = 4 * NQ + 2 * NS + 8 + 2 * kFwItems + 2;
+  static constexpr int NBAR = 4 * NQ + 2 * NS + 8 + 2 * kItems + 2;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int BYTES = OFF_MISC + 16 + 1024;
   static constexpr int ALLOC = BYTES > kOneCtaPerSmSmem ? BYTES : kOneCtaPerSmSmem;
   static_assert(OFF_BAR % 8 == 0 && ALLOC <= 227 * 1024, "shared memory budget");
 };
-
-// First key of key tile t.
-__device__ __forceinline__ int tile_key(const FwItem& it, int t) {
-  return it.sep ? (t == 0 ? 0 : it.w0 + 128 * (t - 1)) : it.w0 + 128 * t;
-}
-// Keys of tile t that exist (the rest of the tile lies past the sequence).
-__device__ __forceinline__ int tile_valid(const FwItem& it, int t) { return min(128, it.lk - tile_key(it, t)); }
-
-// The keys that the row tiles of an item see, as key tiles.
-__device__ __forceinline__ void plan_tiles(const WindowParams& p, FwItem& it, int tt) {
-  int lo[2], hi[2], sink[2], first = 0x7fffffff, end = 0, top = 0;
-  for (int u = 0; u < 2; ++u) {
-    lo[u] = hi[u] = sink[u] = 0;
-    if (it.n[u] <= 0) continue;
-    const RowKeys r0 = row_keys(p, it.pos + u * tt, it.lk), r1 = row_keys(p, it.pos + u * tt + it.n[u] - 1, it.lk);
-    lo[u] = r0.lo;
-    hi[u] = max(r1.hi, 0);
-    sink[u] = max(r1.sink, 0);
-    if (hi[u] > lo[u]) first = min(first, lo[u]), end = max(end, hi[u]);
-    else lo[u] = hi[u] = 0;
-    top = max(top, sink[u]);
-  }
-  it.sep = top > 0 && end > 0 && first > top;  // window and sinks apart: the sinks get a tile of their own
-  if (end == 0) first = 0;
-  if (!it.sep && top > 0) first = 0, end = max(end, top);
-  it.w0 = first;
-  const int wt = (end - first + 127) / 128;
-  it.tiles = wt + it.sep;
-  for (int u = 0; u < 2; ++u) {
-    int a = it.tiles, b = 0;
-    if (hi[u] > lo[u]) a = (lo[u] - first) / 128 + it.sep, b = (hi[u] - first + 127) / 128 + it.sep;
-    if (sink[u] > 0) a = 0, b = max(b, it.sep ? 1 : (sink[u] + 127) / 128);
-    it.a[u] = b > a ? a : 0;
-    it.b[u] = b > a ? b : 0;
-  }
-}
 
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kFwThreads, 1)
@@ -101,7 +52,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sQ = smem;
   uint8_t* sKV = smem + L::OFF_KV;
-  FwItem* items = reinterpret_cast<FwItem*>(smem + L::OFF_ITEM);
+  RowItem* items = reinterpret_cast<RowItem*>(smem + L::OFF_ITEM);
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* q_empty = q_full + 2 * L::NQ;
   uint64_t* kv_full = q_empty + 2 * L::NQ;
@@ -111,8 +62,8 @@ __global__ void __launch_bounds__(kFwThreads, 1)
   uint64_t* p_full = s_free + 2;
   uint64_t* pv_done = p_full + 2;
   uint64_t* item_full = pv_done + 2;
-  uint64_t* item_empty = item_full + kFwItems;
-  uint64_t* mma_done = item_empty + kFwItems;
+  uint64_t* item_empty = item_full + kItems;
+  uint64_t* mma_done = item_empty + kItems;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
 
@@ -129,7 +80,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       mbar_init(&pv_done[i], 1);
       mbar_init(&mma_done[i], 1);
     }
-    for (int i = 0; i < kFwItems; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 10);
+    for (int i = 0; i < kItems; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 10);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -159,25 +110,13 @@ __global__ void __launch_bounds__(kFwThreads, 1)
     int n_it = 0, J = 0, nq[2] = {0, 0};
     bool ok = true;
     for (int w = blockIdx.x; ok; w += gridDim.x) {
-      FwItem it;
+      RowItem it;
       it.stop = w >= n_items;
       if (!it.stop) {
-        const int slot = w / p.hkv;
-        it.hk = w - slot * p.hkv;
-        const int b = seq_of_slot(p.cu_q, p.num_seqs, 2 * TT, slot);
-        const Seq s = seq_of(p, b);
-        const int i0 = (slot - (p.cu_q[b] / (2 * TT) + b)) * 2 * TT;
-        if (i0 < 0 || i0 >= s.lq) continue;
-        it.tok = s.q0 + i0;
-        it.n[0] = min(TT, s.lq - i0);
-        it.n[1] = max(0, min(TT, s.lq - i0 - TT));
-        it.lk = b < p.num_seqs ? s.lk : 0;
-        it.pos = i0 + s.lk - s.lq;
-        it.key0 = s.k0;
-        plan_tiles(p, it, TT);
+        if (!row_item<128>(p, w, TT, it)) continue;
       }
-      const int r = n_it % kFwItems;
-      if (!wait_phase(&item_empty[r], ((n_it / kFwItems) & 1) ^ 1, abort_flag, p.err)) break;
+      const int r = n_it % kItems;
+      if (!wait_phase(&item_empty[r], ((n_it / kItems) & 1) ^ 1, abort_flag, p.err)) break;
       if (lane == 0) {
         items[r] = it;
         mbar_arrive(&item_full[r]);
@@ -197,7 +136,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
         ++nq[u];
       }
       for (int t = 0; t < it.tiles && ok; ++t) {
-        const int key = it.key0 + tile_key(it, t);
+        const int key = it.key0 + it.key<128>(t);
         for (int kv = 0; kv < 2; ++kv) {
           const int st = J % L::NS;
           if (!(ok = wait_phase(&kv_empty[st], ((J / L::NS) & 1) ^ 1, abort_flag, p.err))) break;
@@ -225,16 +164,16 @@ __global__ void __launch_bounds__(kFwThreads, 1)
     const uint32_t idesc_o = make_idesc(AB, 0, 1, 128, D);
     int n_it = 0, J = 0, nq = 0, ns = 0, np = 0;  // items, ring slots, Q tiles, S and P V products so far
     while (true) {
-      const int r = n_it % kFwItems;
-      if (!wait_phase(&item_full[r], (n_it / kFwItems) & 1, abort_flag, p.err)) break;
-      const FwItem& it = items[r];
+      const int r = n_it % kItems;
+      if (!wait_phase(&item_full[r], (n_it / kItems) & 1, abort_flag, p.err)) break;
+      const RowItem& it = items[r];
       ++n_it;
       if (it.stop) break;
       const int st_q = u * L::NQ + nq % L::NQ;
       const uint32_t q_base = smem_u32(sQ + st_q * L::TILE);
       const int a = it.a[u], b = it.b[u];
       // sinks of their own tile: only as many columns as they need
-      auto cols_of = [&](int t) { return it.sep && t == 0 ? (p.sinks + 31) / 32 * 32 : 128; };
+      auto cols_of = [&](int t) { return t < it.sep ? (p.sinks + 31) / 32 * 32 : 128; };
       auto wait_slot = [&](int j) { return wait_phase(&kv_full[j % L::NS], (j / L::NS) & 1, abort_flag, p.err); };
       // keys that only the other row tile sees
       auto pass = [&](int t) {
@@ -275,7 +214,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       }
       for (int t = a; t < b && ok; ++t) {
         if (kOwnP && t + 1 < b && !(ok = issue_s(t + 1))) break;
-        const int j = J + 2 * t + 1, st = j % L::NS, cols = cols_of(t), valid = tile_valid(it, t);
+        const int j = J + 2 * t + 1, st = j % L::NS, cols = cols_of(t), valid = it.valid<128>(t);
         if (!(ok = wait_slot(j))) break;
         if (valid < cols) zero_rows<D>(sKV + st * L::TILE, 128, valid);
         if (!(ok = wait_phase(&p_full[u], np & 1, abort_flag, p.err))) break;
@@ -324,9 +263,9 @@ __global__ void __launch_bounds__(kFwThreads, 1)
     const float sl2 = p.scale * 1.4426950408889634f;
     int n_it = 0, ns = 0;  // items, tiles so far
     while (true) {
-      const int r = n_it % kFwItems;
-      if (!wait_phase(&item_full[r], (n_it / kFwItems) & 1, abort_flag, p.err)) break;
-      const FwItem& it = items[r];
+      const int r = n_it % kItems;
+      if (!wait_phase(&item_full[r], (n_it / kItems) & 1, abort_flag, p.err)) break;
+      const RowItem& it = items[r];
       ++n_it;
       if (it.stop) break;
       const int a = it.a[u], b = it.b[u];
@@ -337,10 +276,10 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       bool ok = true;
       float s[2][32];
       for (int t = a; t < b; ++t) {
-        const int key = tile_key(it, t);
-        const bool sinks_only = it.sep && t == 0;
+        const int key = it.key<128>(t);
+        const bool sinks_only = t < it.sep;
         const int lo = sinks_only ? 0 : keys.lo - key, hi = sinks_only ? 0 : keys.hi - key;
-        const int sink = it.sep && t > 0 ? 0 : keys.sink - key;
+        const int sink = it.sep && !sinks_only ? 0 : keys.sink - key;
         // columns 32 c .. + 31: which of them this row sees; per warp, chunks that some and that all rows see
         uint32_t some = 0u, all = 0u;
         uint32_t bits[4];

@@ -165,6 +165,80 @@ __device__ __forceinline__ void tmem_wait_values(float* v) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+f"(v[i]));
 }
 
+// ---------------------------------------------------------------------------
+// Work items of the kernels that keep query rows (forward, dQ): two tiles of
+// TT tokens x G heads, one kv head, and the key tiles (KT keys) that either
+// sees.  The producer plans them; the other warps read them from a ring.
+// ---------------------------------------------------------------------------
+constexpr int kItems = 4;
+
+struct RowItem {
+  int stop;         // 1: no more items
+  int tok;          // first query token (global)
+  int n[2];         // query tokens of each row tile
+  int hk, pos, lk;  // kv head, position of the first query, keys of the sequence
+  int key0;         // first key of the sequence (global)
+  int tiles, sep;   // key tiles; the first `sep` of them hold the sinks alone, apart from the window
+  int w0;           // first key of the window's first tile
+  int a[2], b[2];   // key tiles [a, b) of each row tile
+
+  template <int KT>
+  __device__ __forceinline__ int key(int t) const {
+    return t < sep ? KT * t : w0 + KT * (t - sep);
+  }
+  // Keys of tile t that exist (the rest of the tile lies past the sequence).
+  template <int KT>
+  __device__ __forceinline__ int valid(int t) const {
+    return min(KT, lk - key<KT>(t));
+  }
+};
+
+// Plans work item `w`; false when it holds no query.
+template <int KT>
+__device__ __forceinline__ bool row_item(const WindowParams& p, int w, int tt, RowItem& it) {
+  const int slot = w / p.hkv;
+  it.hk = w - slot * p.hkv;
+  const int b = seq_of_slot(p.cu_q, p.num_seqs, 2 * tt, slot);
+  const Seq s = seq_of(p, b);
+  const int i0 = (slot - (p.cu_q[b] / (2 * tt) + b)) * 2 * tt;
+  if (i0 < 0 || i0 >= s.lq) return false;
+  it.tok = s.q0 + i0;
+  it.n[0] = min(tt, s.lq - i0);
+  it.n[1] = max(0, min(tt, s.lq - i0 - tt));
+  it.lk = b < p.num_seqs ? s.lk : 0;
+  it.pos = i0 + s.lk - s.lq;
+  it.key0 = s.k0;
+  int lo[2], hi[2], sink[2], first = 0x7fffffff, end = 0, top = 0;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    lo[u] = hi[u] = sink[u] = 0;
+    if (it.n[u] <= 0) continue;
+    const RowKeys r0 = row_keys(p, it.pos + u * tt, it.lk), r1 = row_keys(p, it.pos + u * tt + it.n[u] - 1, it.lk);
+    sink[u] = max(r1.sink, 0);
+    top = max(top, sink[u]);
+    if (r1.hi <= r0.lo) continue;
+    lo[u] = r0.lo;
+    hi[u] = r1.hi;
+    first = min(first, lo[u]);
+    end = max(end, hi[u]);
+  }
+  const bool apart = top > 0 && end > 0 && first > top;
+  it.sep = apart ? (top + KT - 1) / KT : 0;
+  if (end == 0) first = 0;
+  if (!apart && top > 0) first = 0, end = max(end, top);
+  it.w0 = first;
+  it.tiles = (end - first + KT - 1) / KT + it.sep;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    int x = it.tiles, y = 0;
+    if (hi[u] > lo[u]) x = (lo[u] - first) / KT + it.sep, y = (hi[u] - first + KT - 1) / KT + it.sep;
+    if (sink[u] > 0) x = 0, y = max(y, (sink[u] + KT - 1) / KT);
+    it.a[u] = y > x ? x : 0;
+    it.b[u] = y > x ? y : 0;
+  }
+  return true;
+}
+
 template <int N>
 __device__ __forceinline__ void tmem_store_cols(uint32_t taddr, const uint32_t* v) {
   static_assert(N % 16 == 0, "whole sixteens");
