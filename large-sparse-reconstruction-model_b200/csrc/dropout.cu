@@ -16,23 +16,36 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, T
   const long long full = n >> 3;
   const long long stride = (long long)gridDim.x * blockDim.x;
   long long c = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  for (; c < full; c += stride) {
-    float f[8];
+  for (; c + stride < full; c += 2 * stride) {  // two loads in flight
+    float f[8], g[8];
     load8(x, c, f);
-    const uint32_t keep = dropout_keep8(d, c);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = (keep >> i & 1u) ? f[i] * d.scale : 0.f;
+    load8(x, c + stride, g);
+    dropout8(d, c, f);
     store8(y, c, f);
+    dropout8(d, c + stride, g);
+    store8(y, c + stride, g);
   }
-  if (c == full && (n & 7)) {
+  for (; c <= full; c += stride) {
     float f[8];
-    const int rest = (int)(n & 7);
-    load8_part(x, c, 0, rest, f);
-    const uint32_t keep = dropout_keep8(d, c);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = (keep >> i & 1u) ? f[i] * d.scale : 0.f;
-    store8_part(y, c, 0, rest, f);
+    if (c < full) {
+      load8(x, c, f);
+      dropout8(d, c, f);
+      store8(y, c, f);
+    } else if (n & 7) {
+      load8_part(x, c, 0, (int)(n & 7), f);
+      dropout8(d, c, f);
+      store8_part(y, c, 0, (int)(n & 7), f);
+    }
   }
+}
+
+template <typename T>
+int launch_dropout(const void* x, void* y, long long n, const DropoutParams& d, cudaStream_t s) {
+  const int grid = (int)std::min<long long>((n / 8 + 256) / 256,
+                                            (long long)num_sms() * resident_blocks<dropout_kernel<T>>(256));
+  dropout_kernel<<<grid, 256, 0, s>>>(static_cast<const T*>(x), static_cast<T*>(y), n, d);
+  LSRM_LAUNCH_CHECK();
+  return LSRM_OK;
 }
 
 }  // namespace
@@ -52,13 +65,7 @@ extern "C" int lsrm_dropout(int64_t n, int32_t dtype, double p, uint64_t seed, u
   const DropoutParams d = make_dropout(p, seed, offset);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   ProfScope ps("dropout", s);
-  const int grid = (int)std::min<long long>((n / 8 + 256) / 256, (long long)num_sms() * 8);
-  if (dtype == LSRM_DTYPE_BF16)
-    dropout_kernel<<<grid, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(x), static_cast<__nv_bfloat16*>(y), n, d);
-  else if (dtype == LSRM_DTYPE_F16)
-    dropout_kernel<<<grid, 256, 0, s>>>(static_cast<const __half*>(x), static_cast<__half*>(y), n, d);
-  else
-    dropout_kernel<<<grid, 256, 0, s>>>(static_cast<const float*>(x), static_cast<float*>(y), n, d);
-  LSRM_LAUNCH_CHECK();
-  return LSRM_OK;
+  return dtype == LSRM_DTYPE_BF16  ? launch_dropout<__nv_bfloat16>(x, y, n, d, s)
+         : dtype == LSRM_DTYPE_F16 ? launch_dropout<__half>(x, y, n, d, s)
+                                   : launch_dropout<float>(x, y, n, d, s);
 }

@@ -82,6 +82,23 @@ inline T ceil_div(T a, T b) {
   return (a + b - 1) / b;
 }
 
+// Blocks of `threads` threads of a kernel that are resident on a
+// multiprocessor at once (asked once per kernel and power-of-two size): the
+// grid of a grid-stride kernel is a whole number of such rounds, so that none
+// is left for a short last one.
+template <auto Kernel>
+int resident_blocks(int threads) {
+  static std::atomic<int> cache[12];
+  int i = 0;
+  while ((32 << i) < threads && i < 11) ++i;
+  int n = cache[i].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kernel, threads, 0) != cudaSuccess || n < 1) n = 1;
+    cache[i].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 }  // namespace lsrm

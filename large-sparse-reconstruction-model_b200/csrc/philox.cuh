@@ -39,14 +39,13 @@ __device__ __forceinline__ uint4 philox4x32(uint64_t block, uint32_t k0, uint32_
   return make_uint4(x0, x1, x2, x3);
 }
 
-// Keep bits of the eight elements 8 * chunk .. 8 * chunk + 7 (bit i: element i).
-__device__ __forceinline__ uint32_t dropout_keep8(const DropoutParams& d, long long chunk) {
+// Drops and scales the eight elements 8 * chunk .. 8 * chunk + 7 in place.
+__device__ __forceinline__ void dropout8(const DropoutParams& d, long long chunk, float* f) {
   const uint4 a = philox4x32(d.offset + 2 * (uint64_t)chunk, d.key0, d.key1);
   const uint4 b = philox4x32(d.offset + 2 * (uint64_t)chunk + 1, d.key0, d.key1);
-  const uint32_t t = d.threshold;
-  return (uint32_t)(a.x >= t) | (uint32_t)(a.y >= t) << 1 | (uint32_t)(a.z >= t) << 2 | (uint32_t)(a.w >= t) << 3 |
-         (uint32_t)(b.x >= t) << 4 | (uint32_t)(b.y >= t) << 5 | (uint32_t)(b.z >= t) << 6 |
-         (uint32_t)(b.w >= t) << 7;
+  const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = w[i] >= d.threshold ? f[i] * d.scale : 0.f;
 }
 
 }  // namespace lsrm

@@ -28,6 +28,11 @@ namespace {
 
 constexpr int kNormMaxCols = 16384;  // 512 threads x 4 chunks x 8 elements
 constexpr int kRowWarps = 8;         // rows per block when a warp owns a row
+#ifndef FC
+#define FC 4
+#define BC 2
+#endif
+constexpr int kFwdChunks = FC, kBwdChunks = BC;
 
 struct NormParams {
   long long rows;
@@ -155,16 +160,6 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const NormParams p) 
   S* hs = static_cast<S*>(p.h);
   const long long team = (long long)blockIdx.x * blockDim.y + threadIdx.y;
   const long long teams = (long long)gridDim.x * blockDim.y;
-  float w[EVEN ? NV : 1][8];
-  if (EVEN) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = t + tpr * i;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[i][j] = 1.f;
-      if (p.w && c < p.cols8) read_w8<T>(p, 8 * c, w[i]);
-    }
-  }
   for (long long row = team; row < p.rows; row += teams) {
     const long long e0 = row * p.cols, c0 = e0 >> 3;
     const int n8 = EVEN ? p.cols8 : (int)(((e0 + p.cols - 1) >> 3) - c0 + 1);
@@ -179,11 +174,7 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const NormParams p) 
         const long long c = c0 + k;
         const Part pt = EVEN ? Part{0, 8} : part_of(c, e0, p.cols);
         read_chunk<EVEN>(x, c, p.total8, pt, v[i]);
-        if (DROP) {
-          const uint32_t keep = dropout_keep8(p.drop, c);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[i][j] = (keep >> j & 1u) ? v[i][j] * p.drop.scale : 0.f;
-        }
+        if (DROP) dropout8(p.drop, c, v[i]);
         if (res) {
           float r[8];
           read_chunk<EVEN>(res, c, p.total8, pt, r);
@@ -216,8 +207,10 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const NormParams p) 
           if (p.w && col >= 0 && col < p.cols) v[i][j] *= read_w(p, col, kBf16);
         }
       } else {
+        float w[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+        if (p.w && k < n8) read_w8<T>(p, 8 * k, w);  // from L1: registers are better spent on more rows in flight
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] *= rstd * w[i][j];
+        for (int j = 0; j < 8; ++j) v[i][j] *= rstd * w[j];
       }
       if (OUT == kOutPlain) {
         if (k < n8) write_chunk<EVEN>(y, c0 + k, EVEN ? Part{0, 8} : part_of(c0 + k, e0, p.cols), v[i]);
@@ -300,17 +293,12 @@ __global__ void __launch_bounds__(512) residual_norm_bwd_kernel(const NormParams
   const long long team = (long long)blockIdx.x * blockDim.y + threadIdx.y;
   const long long teams = (long long)gridDim.x * blockDim.y;
   float dw[EVEN ? NV : 1][8];
-  float w[EVEN ? NV : 1][8];
   float* s_row = s_dw + (EVEN ? 0 : threadIdx.y * p.cols);
 #pragma unroll
   for (int i = 0; i < (EVEN ? NV : 1); ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) dw[i][j] = 0.f, w[i][j] = 1.f;
-  if (EVEN) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (p.w && t + tpr * i < p.cols8) read_w8<T>(p, 8 * (t + tpr * i), w[i]);
-  } else if (p.dw_part) {
+    for (int j = 0; j < 8; ++j) dw[i][j] = 0.f;
+  if (!EVEN && p.dw_part) {
     for (int c = t; c < p.cols; c += tpr) s_row[c] = 0.f;
     if (tpr == 32) __syncwarp();
     else __syncthreads();
@@ -332,6 +320,8 @@ __global__ void __launch_bounds__(512) residual_norm_bwd_kernel(const NormParams
         read_chunk<EVEN>(dy, c, p.total8, pt, g[i]);
         read_chunk<EVEN>(hs, c, p.total8, pt, h[i]);
         const int col0 = (int)(8 * c - e0);
+        float w[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+        if (EVEN && p.w) read_w8<T>(p, 8 * k, w);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if (!EVEN && (j < pt.lo || j >= pt.hi)) {
@@ -340,7 +330,7 @@ __global__ void __launch_bounds__(512) residual_norm_bwd_kernel(const NormParams
           }
           if (EVEN) {
             dw[i][j] = fmaf(g[i][j] * h[i][j], rstd, dw[i][j]);
-            g[i][j] *= w[i][j];
+            g[i][j] *= w[j];
           } else {
             // a column belongs to one thread of the team in a row; the team meets between rows
             if (p.dw_part) s_row[col0 + j] = fmaf(g[i][j] * h[i][j], rstd, s_row[col0 + j]);
@@ -366,11 +356,7 @@ __global__ void __launch_bounds__(512) residual_norm_bwd_kernel(const NormParams
         for (int j = 0; j < 8; ++j) d[j] = fmaf(rstd, g[i][j] - h[i][j] * k2, d[j]);
         write_chunk<EVEN>(dres, c, pt, d);
         if (dx) {
-          if (DROP) {
-            const uint32_t keep = dropout_keep8(p.drop, c);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) d[j] = (keep >> j & 1u) ? d[j] * p.drop.scale : 0.f;
-          }
+          if (DROP) dropout8(p.drop, c, d);
           write_chunk<EVEN>(dx, c, pt, d);
         }
       }
@@ -428,13 +414,41 @@ __global__ void __launch_bounds__(256) norm_dw_kernel(const float* __restrict__ 
   }
 }
 
-template <typename T, bool E4M3>
+// y = value * scale, eight elements a thread.  EVEN: rows and groups are whole
+// chunks, so that a chunk has one scale.
+template <typename T, bool E4M3, bool EVEN>
 __global__ void __launch_bounds__(256) dequantize8_kernel(const uint8_t* __restrict__ q, const float* __restrict__ sc,
                                                           T* __restrict__ y, long long rows, int cols, int group,
                                                           int groups) {
   const long long n = rows * cols, full = n >> 3, chunks = (n + 7) >> 3;
   const long long stride = (long long)gridDim.x * blockDim.x;
-  for (long long c = (long long)blockIdx.x * blockDim.x + threadIdx.x; c < chunks; c += stride) {
+  auto value = [](uint64_t u, int i) {
+    const uint32_t b = (uint32_t)(u >> (8 * i)) & 0xffu;
+    return E4M3 ? __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3)))
+                : (float)(int8_t)b;
+  };
+  long long c = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  if (EVEN) {
+    const int row8 = cols >> 3, group8 = group >> 3;
+    // row and chunk of the row advance without a division
+    long long row = c / row8;
+    int k = (int)(c - row * row8);
+    const long long step_row = stride / row8;
+    const int step_k = (int)(stride - step_row * row8);
+    for (; c < chunks; c += stride) {
+      const uint64_t u = reinterpret_cast<const uint64_t*>(q)[c];
+      const float s = sc[row * groups + (groups == 1 ? 0 : k / group8)];
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = value(u, i) * s;
+      store8(y, c, f);
+      row += step_row;
+      k += step_k;
+      if (k >= row8) k -= row8, ++row;
+    }
+    return;
+  }
+  for (; c < chunks; c += stride) {
     const int hi = c < full ? 8 : (int)(n & 7);
     uint64_t u = 0;
     if (hi == 8)
@@ -453,10 +467,7 @@ __global__ void __launch_bounds__(256) dequantize8_kernel(const uint8_t* __restr
         s = sc[row * groups + g];
         left = min(cols, (g + 1) * group) - col;
       }
-      const uint32_t b = (uint32_t)(u >> (8 * i)) & 0xffu;
-      const float val = E4M3 ? __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)b, __NV_E4M3)))
-                             : (float)(int8_t)b;
-      f[i] = val * s;
+      f[i] = value(u, i) * s;
       --left;
       ++col;
     }
@@ -467,36 +478,54 @@ __global__ void __launch_bounds__(256) dequantize8_kernel(const uint8_t* __restr
   }
 }
 
+template <typename T, bool E4M3>
+int launch_dequantize(const uint8_t* q, const float* scales, void* y, long long rows, int cols, int group, int groups,
+                      cudaStream_t s) {
+  const long long want = (rows * cols / 8 + 256) / 256;
+  constexpr auto k0 = dequantize8_kernel<T, E4M3, true>;
+  constexpr auto k1 = dequantize8_kernel<T, E4M3, false>;
+  if (cols % 8 == 0 && (groups == 1 || group % 8 == 0))
+    k0<<<(int)std::min<long long>(want, (long long)num_sms() * resident_blocks<k0>(256)), 256, 0, s>>>(
+        q, scales, static_cast<T*>(y), rows, cols, group, groups);
+  else
+    k1<<<(int)std::min<long long>(want, (long long)num_sms() * resident_blocks<k1>(256)), 256, 0, s>>>(
+        q, scales, static_cast<T*>(y), rows, cols, group, groups);
+  LSRM_LAUNCH_CHECK();
+  return LSRM_OK;
+}
+
 struct NormLaunch {
-  dim3 grid, block;
+  dim3 block;
+  long long teams;  // blocks that the rows can fill
   int nv;
   bool even;
 };
 
-// Threads per row: the narrowest team that holds the row in at most four
-// chunks a thread (a warp up to 1024 columns: the row's sums need no barrier).
-// Where there are not enough rows to fill the GPU (fewer teams than four a
+// Threads per row: the narrowest team that holds the row in at most `chunks`
+// chunks a thread (a warp where that suffices: the row's sums need no barrier).
+// Where there are not enough rows to fill the GPU (fewer than four a
 // multiprocessor), a thread takes one chunk so that a row's loads are in
 // flight at once.
-NormLaunch norm_launch(long long rows, int cols, bool block_teams) {
+NormLaunch norm_launch(long long rows, int cols, bool block_teams, int chunks) {
   const bool even = cols % 8 == 0;
   const int n8 = even ? cols / 8 : cols / 8 + 2;
-  const int most = rows <= 4LL * num_sms() ? 1 : 4;
+  const int most = rows <= 4LL * num_sms() ? 1 : chunks;
   int tpr = block_teams ? 64 : 32;
   while (tpr < 512 && tpr * most < n8) tpr *= 2;
   const int per = (n8 + tpr - 1) / tpr;
   NormLaunch l;
   l.nv = per <= 1 ? 1 : per <= 2 ? 2 : per <= 4 ? 4 : 5;
   l.even = even;
-  if (tpr == 32) {
-    l.block = dim3(32, kRowWarps);
-    l.grid = dim3((unsigned)std::min<long long>((rows + kRowWarps - 1) / kRowWarps, (long long)num_sms() * 4));
-  } else {
-    l.block = dim3(tpr, 1);
-    l.grid = dim3((unsigned)std::min<long long>(rows, (long long)num_sms() * (2048 / tpr)));
-  }
+  l.block = tpr == 32 ? dim3(32, kRowWarps) : dim3(tpr, 1);
+  l.teams = tpr == 32 ? (rows + kRowWarps - 1) / kRowWarps : rows;
   return l;
 }
+
+// Blocks of a launch, at most: what the multiprocessors hold at once.
+int norm_blocks(const NormLaunch& l, int resident) {
+  return (int)std::min<long long>(l.teams, (long long)num_sms() * resident);
+}
+int norm_blocks_most(const NormLaunch& l) { return norm_blocks(l, 2048 / (int)(l.block.x * l.block.y)); }
 
 #define NORM_NV(CALL)          \
   switch (l.nv) {              \
@@ -509,10 +538,15 @@ NormLaunch norm_launch(long long rows, int cols, bool block_teams) {
 template <typename T, typename S, int OUT, bool DROP>
 int launch_norm(const NormParams& p, const NormLaunch& l, size_t smem, cudaStream_t s) {
 #define NORM_CALL(NV)                                                                     \
-  if (l.even)                                                                             \
-    residual_norm_kernel<T, S, NV, true, OUT, DROP><<<l.grid, l.block, smem, s>>>(p);     \
-  else                                                                                    \
-    residual_norm_kernel<T, S, NV, false, OUT, DROP><<<l.grid, l.block, smem, s>>>(p);
+  {                                                                                       \
+    constexpr auto k0 = residual_norm_kernel<T, S, NV, true, OUT, DROP>;                  \
+    constexpr auto k1 = residual_norm_kernel<T, S, NV, false, OUT, DROP>;                 \
+    const int threads = l.block.x * l.block.y;                                            \
+    if (l.even)                                                                           \
+      k0<<<norm_blocks(l, resident_blocks<k0>(threads)), l.block, smem, s>>>(p);          \
+    else                                                                                  \
+      k1<<<norm_blocks(l, resident_blocks<k1>(threads)), l.block, smem, s>>>(p);          \
+  }
   NORM_NV(NORM_CALL)
 #undef NORM_CALL
   LSRM_LAUNCH_CHECK();
@@ -520,12 +554,16 @@ int launch_norm(const NormParams& p, const NormLaunch& l, size_t smem, cudaStrea
 }
 
 template <typename T, typename S, bool DROP>
-int launch_norm_bwd(const NormParams& p, const NormLaunch& l, size_t smem, cudaStream_t s) {
+int launch_norm_bwd(const NormParams& p, const NormLaunch& l, size_t smem, cudaStream_t s, int* blocks) {
 #define NORM_CALL(NV)                                                                                              \
   {                                                                                                                \
-    auto k = l.even ? residual_norm_bwd_kernel<T, S, NV, true, DROP> : residual_norm_bwd_kernel<T, S, NV, false, DROP>; \
+    constexpr auto k0 = residual_norm_bwd_kernel<T, S, NV, true, DROP>;                                            \
+    constexpr auto k1 = residual_norm_bwd_kernel<T, S, NV, false, DROP>;                                           \
+    const int threads = l.block.x * l.block.y;                                                                     \
+    *blocks = norm_blocks(l, l.even ? resident_blocks<k0>(threads) : resident_blocks<k1>(threads));                \
+    auto k = l.even ? k0 : k1;                                                                                     \
     if (smem > 48 * 1024) LSRM_CUDA_TRY(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); \
-    k<<<l.grid, l.block, smem, s>>>(p);                                                                            \
+    k<<<*blocks, l.block, smem, s>>>(p);                                                                           \
   }
   NORM_NV(NORM_CALL)
 #undef NORM_CALL
@@ -573,10 +611,12 @@ int launch_norm_t(bool s_f32, int out, bool drop, const NormParams& p, const Nor
 }
 
 template <typename T>
-int launch_norm_bwd_t(bool s_f32, bool drop, const NormParams& p, const NormLaunch& l, size_t smem, cudaStream_t s) {
+int launch_norm_bwd_t(bool s_f32, bool drop, const NormParams& p, const NormLaunch& l, size_t smem, cudaStream_t s,
+                      int* blocks) {
   if (s_f32)
-    return drop ? launch_norm_bwd<T, float, true>(p, l, smem, s) : launch_norm_bwd<T, float, false>(p, l, smem, s);
-  return drop ? launch_norm_bwd<T, T, true>(p, l, smem, s) : launch_norm_bwd<T, T, false>(p, l, smem, s);
+    return drop ? launch_norm_bwd<T, float, true>(p, l, smem, s, blocks)
+                : launch_norm_bwd<T, float, false>(p, l, smem, s, blocks);
+  return drop ? launch_norm_bwd<T, T, true>(p, l, smem, s, blocks) : launch_norm_bwd<T, T, false>(p, l, smem, s, blocks);
 }
 
 }  // namespace
@@ -600,7 +640,7 @@ extern "C" int lsrm_residual_rms_norm_fwd(int64_t rows, int32_t cols, int32_t dt
   p.drop = make_dropout(p_drop, seed, offset);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   ProfScope ps("residual_rms_norm", s);
-  const NormLaunch l = norm_launch(rows, cols, false);
+  const NormLaunch l = norm_launch(rows, cols, false, kFwdChunks);
   return dtype == LSRM_DTYPE_BF16
              ? launch_norm_t<__nv_bfloat16>(stream_dtype == LSRM_DTYPE_F32, kOutPlain, p_drop > 0, p, l, 0, s)
              : launch_norm_t<__half>(stream_dtype == LSRM_DTYPE_F32, kOutPlain, p_drop > 0, p, l, 0, s);
@@ -629,7 +669,7 @@ extern "C" int lsrm_residual_rms_norm_8bit(int64_t rows, int32_t cols, int32_t d
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   ProfScope ps("residual_rms_norm_8bit", s);
   const bool uneven_groups = cols % 8 != 0 && p.groups > 1;
-  const NormLaunch l = norm_launch(rows, cols, uneven_groups);
+  const NormLaunch l = norm_launch(rows, cols, uneven_groups, kFwdChunks);
   const size_t smem = uneven_groups ? p.groups * sizeof(int) : 0;
   const int out = out_dtype == LSRM_DTYPE_E4M3 ? kOutE4m3 : kOutInt8;
   return dtype == LSRM_DTYPE_BF16
@@ -640,7 +680,7 @@ extern "C" int lsrm_residual_rms_norm_8bit(int64_t rows, int32_t cols, int32_t d
 // The partial sums of dw: one row of fp32 per block of the backward kernel.
 extern "C" size_t lsrm_residual_rms_norm_workspace_bytes(int64_t rows, int32_t cols) {
   if (rows <= 0 || cols < 1 || cols > kNormMaxCols) return 0;
-  return (size_t)norm_launch(rows, cols, false).grid.x * cols * sizeof(float);
+  return (size_t)norm_blocks_most(norm_launch(rows, cols, false, kBwdChunks)) * cols * sizeof(float);
 }
 
 extern "C" int lsrm_residual_rms_norm_bwd(int64_t rows, int32_t cols, int32_t dtype, int32_t stream_dtype,
@@ -670,25 +710,26 @@ extern "C" int lsrm_residual_rms_norm_bwd(int64_t rows, int32_t cols, int32_t dt
   p.h = const_cast<void*>(h), p.rstd = const_cast<float*>(rstd), p.dy = dy, p.dh = dh, p.dx = dx, p.dres = dresidual;
   p.dw_part = dweight ? static_cast<float*>(workspace) : nullptr;
   p.drop = make_dropout(p_drop, seed, offset);
-  const NormLaunch l = norm_launch(rows, cols, false);
+  const NormLaunch l = norm_launch(rows, cols, false, kBwdChunks);
   size_t smem = 0;
   if (dweight && (!l.even || l.block.y > 1)) smem = (size_t)cols * (l.even ? 1 : l.block.y) * sizeof(float);
+  int blocks = 0;
   {
     ProfScope ps("residual_rms_norm_bwd", s);
     rc = dtype == LSRM_DTYPE_BF16
-             ? launch_norm_bwd_t<__nv_bfloat16>(stream_dtype == LSRM_DTYPE_F32, p_drop > 0, p, l, smem, s)
-             : launch_norm_bwd_t<__half>(stream_dtype == LSRM_DTYPE_F32, p_drop > 0, p, l, smem, s);
+             ? launch_norm_bwd_t<__nv_bfloat16>(stream_dtype == LSRM_DTYPE_F32, p_drop > 0, p, l, smem, s, &blocks)
+             : launch_norm_bwd_t<__half>(stream_dtype == LSRM_DTYPE_F32, p_drop > 0, p, l, smem, s, &blocks);
     if (rc) return rc;
   }
   if (!dweight) return LSRM_OK;
   ProfScope ps("residual_rms_norm_dw", s);
   const dim3 grid((cols + 31) / 32), block(32, 8);
   if (weight_dtype == LSRM_DTYPE_F32)
-    norm_dw_kernel<<<grid, block, 0, s>>>(p.dw_part, (int)l.grid.x, cols, static_cast<float*>(dweight));
+    norm_dw_kernel<<<grid, block, 0, s>>>(p.dw_part, blocks, cols, static_cast<float*>(dweight));
   else if (dtype == LSRM_DTYPE_BF16)
-    norm_dw_kernel<<<grid, block, 0, s>>>(p.dw_part, (int)l.grid.x, cols, static_cast<__nv_bfloat16*>(dweight));
+    norm_dw_kernel<<<grid, block, 0, s>>>(p.dw_part, blocks, cols, static_cast<__nv_bfloat16*>(dweight));
   else
-    norm_dw_kernel<<<grid, block, 0, s>>>(p.dw_part, (int)l.grid.x, cols, static_cast<__half*>(dweight));
+    norm_dw_kernel<<<grid, block, 0, s>>>(p.dw_part, blocks, cols, static_cast<__half*>(dweight));
   LSRM_LAUNCH_CHECK();
   return LSRM_OK;
 }
@@ -706,13 +747,10 @@ extern "C" int lsrm_dequantize_8bit(int64_t rows, int32_t cols, int32_t in_dtype
   const int g = group ? group : cols, groups = (cols + g - 1) / g;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   ProfScope ps("dequantize_8bit", s);
-  const int grid = (int)std::min<long long>((rows * cols / 8 + 256) / 256, (long long)num_sms() * 8);
   const uint8_t* q = static_cast<const uint8_t*>(values);
-#define DEQ(T)                                                                                                 \
-  if (in_dtype == LSRM_DTYPE_E4M3)                                                                             \
-    dequantize8_kernel<T, true><<<grid, 256, 0, s>>>(q, scales, static_cast<T*>(y), rows, cols, g, groups);    \
-  else                                                                                                         \
-    dequantize8_kernel<T, false><<<grid, 256, 0, s>>>(q, scales, static_cast<T*>(y), rows, cols, g, groups);
+#define DEQ(T)                                                                                               \
+  return in_dtype == LSRM_DTYPE_E4M3 ? launch_dequantize<T, true>(q, scales, y, rows, cols, g, groups, s)     \
+                                     : launch_dequantize<T, false>(q, scales, y, rows, cols, g, groups, s);
   if (out_dtype == LSRM_DTYPE_BF16) {
     DEQ(__nv_bfloat16)
   } else if (out_dtype == LSRM_DTYPE_F16) {
@@ -721,6 +759,4 @@ extern "C" int lsrm_dequantize_8bit(int64_t rows, int32_t cols, int32_t in_dtype
     DEQ(float)
   }
 #undef DEQ
-  LSRM_LAUNCH_CHECK();
-  return LSRM_OK;
 }
