@@ -10,23 +10,31 @@
 
 namespace lsrm {
 
+// The eight elements as loaded (a load in flight costs 4 or 8 registers).
 template <typename T>
-__device__ __forceinline__ float to_f32(T v) {
-  return (float)v;
+struct Raw8 {
+  uint4 u[sizeof(T) / 2];
+};
+
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8_raw(const T* base, long long chunk) {
+  Raw8<T> r;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+    r.u[i] = reinterpret_cast<const uint4*>(base)[chunk * (sizeof(T) / 2) + i];
+  return r;
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack8(const Raw8<T>& r, float* f) {
+  const T* e = reinterpret_cast<const T*>(r.u);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = (float)e[i];
 }
 
 template <typename T>
 __device__ __forceinline__ void load8(const T* base, long long chunk, float* f) {
-  if constexpr (sizeof(T) == 2) {
-    const uint4 u = reinterpret_cast<const uint4*>(base)[chunk];
-    const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = (float)e[i];
-  } else {
-    const float4 a = reinterpret_cast<const float4*>(base)[2 * chunk];
-    const float4 b = reinterpret_cast<const float4*>(base)[2 * chunk + 1];
-    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-  }
+  unpack8(load8_raw(base, chunk), f);
 }
 
 template <typename T>
