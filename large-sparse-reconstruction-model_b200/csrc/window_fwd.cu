@@ -12,11 +12,11 @@
 //   warps 8, 9      tensor-core issue for row tile 0 and 1: S = Q K^T, O += P V
 //                   (P from TMEM)
 //   warp 10         producer: work items, TMA of Q, K and V
-// K and V tiles (128 keys) go through one ring and serve both row tiles, which
-// halves the L2 reads per product.  Up to 64 channels P has TMEM columns of its
-// own and the next S is computed while this one's softmax runs; at 128 channels
-// TMEM is full, P lies over S, and the row tiles' turns hide each other's
-// products.  Rounding: S, m, l and O are fp32; P is
+// K and V tiles (64 keys) go through one ring and serve both row tiles, which
+// halves the L2 reads per product.  S has two buffers of 64 columns a row tile
+// and P lies over its S, so that the products of the tiles before and after run
+// under a tile's softmax (at 128 keys a buffer TMEM holds one, and the two row
+// tiles fell into step: both in their softmax, then both waiting).  Rounding: S, m, l and O are fp32; P is
 // rounded to the operand type (the sum l takes it unrounded), O once at the end.
 #include "window_host.h"
 #include "window_tile.cuh"
@@ -25,17 +25,18 @@ namespace lsrm {
 namespace {
 
 constexpr int kFwThreads = 352;
+constexpr int kFwKeys = 64;
 template <int D>
 struct FwSmem {
-  static constexpr int TILE = TileShape<D>::bytes(128);
+  static constexpr int QT = TileShape<D>::bytes(128), KT = TileShape<D>::bytes(kFwKeys);
   static constexpr int NQ = D == 128 ? 1 : 2;  // Q buffers of each row tile
-  static constexpr int NS = D == 128 ? 5 : 8;  // K / V ring
-  static constexpr int OFF_KV = 2 * NQ * TILE;
-  static constexpr int OFF_ITEM = OFF_KV + NS * TILE;
+  static constexpr int NS = D == 128 ? 9 : 12;  // K / V ring
+  static constexpr int OFF_KV = 2 * NQ * QT;
+  static constexpr int OFF_ITEM = OFF_KV + NS * KT;
   static constexpr int OFF_BAR = OFF_ITEM + kItems * (int)sizeof(RowItem);
-  // q_full[2][NQ], q_empty[2][NQ], kv_full[NS], kv_empty[NS], s_full[2], s_free[2], p_full[2], pv_done[2],
+  // q_full[2][NQ], q_empty[2][NQ], kv_full[NS], kv_empty[NS], s_full[2][2], p_full[2][2], pv_done[2][2],
   // item_full[], item_empty[], mma_done[2]
-  static constexpr int NBAR = 4 * NQ + 2 * NS + 8 + 2 * kItems + 2;
+  static constexpr int NBAR = 4 * NQ + 2 * NS + 12 + 2 * kItems + 2;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int BYTES = OFF_MISC + 16 + 1024;
   static constexpr int ALLOC = BYTES > kOneCtaPerSmSmem ? BYTES : kOneCtaPerSmSmem;
@@ -58,10 +59,10 @@ __global__ void __launch_bounds__(kFwThreads, 1)
   uint64_t* kv_full = q_empty + 2 * L::NQ;
   uint64_t* kv_empty = kv_full + L::NS;
   uint64_t* s_full = kv_empty + L::NS;
-  uint64_t* s_free = s_full + 2;
-  uint64_t* p_full = s_free + 2;
-  uint64_t* pv_done = p_full + 2;
-  uint64_t* item_full = pv_done + 2;
+  // [row tile][buffer]: two tiles are under way, so each has its own phases
+  uint64_t* p_full = s_full + 4;
+  uint64_t* pv_done = p_full + 4;
+  uint64_t* item_full = pv_done + 4;
   uint64_t* item_empty = item_full + kItems;
   uint64_t* mma_done = item_empty + kItems;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
@@ -74,10 +75,12 @@ __global__ void __launch_bounds__(kFwThreads, 1)
     for (int i = 0; i < 2 * L::NQ; ++i) mbar_init(&q_full[i], 1), mbar_init(&q_empty[i], 1);
     for (int i = 0; i < L::NS; ++i) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], 2);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&s_full[i], 1);
-      mbar_init(&s_free[i], 4);
-      mbar_init(&p_full[i], 4);
-      mbar_init(&pv_done[i], 1);
+      mbar_init(&s_full[2 * i], 1);
+      mbar_init(&s_full[2 * i + 1], 1);
+      mbar_init(&p_full[2 * i], 4);
+      mbar_init(&p_full[2 * i + 1], 4);
+      mbar_init(&pv_done[2 * i], 1);
+      mbar_init(&pv_done[2 * i + 1], 1);
       mbar_init(&mma_done[i], 1);
     }
     for (int i = 0; i < kItems; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 10);
@@ -92,8 +95,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // TMEM columns: S [0, 256), O [256, 256 + 2 D), P (64 a row tile) in [384, 512) up to D = 64, else over S
-  constexpr bool kOwnP = D <= 64;
+  // TMEM columns: S of row tile u, buffer i [128 u + 64 i, +64) with P over its first half; O [256 + u D, +D)
 
   if (warp == 10) {
     // ------------------------------ producer ------------------------------
@@ -113,7 +115,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       RowItem it;
       it.stop = w >= n_items;
       if (!it.stop) {
-        if (!row_item<128>(p, w, TT, it)) continue;
+        if (!row_item<kFwKeys>(p, w, TT, it)) continue;
       }
       const int r = n_it % kItems;
       if (!wait_phase(&item_empty[r], ((n_it / kItems) & 1) ^ 1, abort_flag, p.err)) break;
@@ -130,19 +132,19 @@ __global__ void __launch_bounds__(kFwThreads, 1)
         if (!(ok = wait_phase(&q_empty[st], ((nq[u] / L::NQ) & 1) ^ 1, abort_flag, p.err))) break;
         if (elect_one()) {
           mbar_arrive_expect_tx(&q_full[st], q_bytes);
-          load_tile<D>(sQ + st * L::TILE, 128, &tm_q, it.hk * G, it.tok + u * TT, &q_full[st]);
+          load_tile<D>(sQ + st * L::QT, 128, &tm_q, it.hk * G, it.tok + u * TT, &q_full[st]);
         }
         __syncwarp();
         ++nq[u];
       }
       for (int t = 0; t < it.tiles && ok; ++t) {
-        const int key = it.key0 + it.key<128>(t);
+        const int key = it.key0 + it.key<kFwKeys>(t);
         for (int kv = 0; kv < 2; ++kv) {
           const int st = J % L::NS;
           if (!(ok = wait_phase(&kv_empty[st], ((J / L::NS) & 1) ^ 1, abort_flag, p.err))) break;
           if (elect_one()) {
-            mbar_arrive_expect_tx(&kv_full[st], L::TILE);
-            load_tile<D>(sKV + st * L::TILE, 128, kv ? &tm_v : &tm_k, it.hk, key, &kv_full[st]);
+            mbar_arrive_expect_tx(&kv_full[st], L::KT);
+            load_tile<D>(sKV + st * L::KT, kFwKeys, kv ? &tm_v : &tm_k, it.hk, key, &kv_full[st]);
           }
           __syncwarp();
           ++J;
@@ -160,9 +162,10 @@ __global__ void __launch_bounds__(kFwThreads, 1)
   } else if (warp >= 8) {
     // --------------------------- tensor-core issue ---------------------------
     const int u = warp - 8;
-    const uint32_t tm_s = tmem + u * 128, tm_o = tmem + 256 + u * D, tm_p = kOwnP ? tmem + 384 + u * 64 : tm_s;
+    const uint32_t tm_s = tmem + u * 128, tm_o = tmem + 256 + u * D;
     const uint32_t idesc_o = make_idesc(AB, 0, 1, 128, D);
-    int n_it = 0, J = 0, nq = 0, ns = 0, np = 0;  // items, ring slots, Q tiles, S and P V products so far
+    int n_it = 0, J = 0, nq = 0;         // items, ring slots, Q tiles so far
+    int ns = 0, np = 0;                  // S and P V products issued
     while (true) {
       const int r = n_it % kItems;
       if (!wait_phase(&item_full[r], (n_it / kItems) & 1, abort_flag, p.err)) break;
@@ -170,10 +173,10 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       ++n_it;
       if (it.stop) break;
       const int st_q = u * L::NQ + nq % L::NQ;
-      const uint32_t q_base = smem_u32(sQ + st_q * L::TILE);
+      const uint32_t q_base = smem_u32(sQ + st_q * L::QT);
       const int a = it.a[u], b = it.b[u];
       // sinks of their own tile: only as many columns as they need
-      auto cols_of = [&](int t) { return t < it.sep ? (p.sinks + 31) / 32 * 32 : 128; };
+      auto cols_of = [&](int t) { return t < it.sep ? min(kFwKeys, (p.sinks - t * kFwKeys + 31) / 32 * 32) : kFwKeys; };
       auto wait_slot = [&](int j) { return wait_phase(&kv_full[j % L::NS], (j / L::NS) & 1, abort_flag, p.err); };
       // keys that only the other row tile sees
       auto pass = [&](int t) {
@@ -186,20 +189,19 @@ __global__ void __launch_bounds__(kFwThreads, 1)
         return true;
       };
       auto issue_s = [&](int t) {
-        const int j = J + 2 * t, st = j % L::NS;
+        const int j = J + 2 * t, st = j % L::NS, buf = ns & 1;
         if (!wait_slot(j)) return false;
-        // the last S has been read; where P lies over S, the product that reads P is over
-        if (kOwnP && ns > 0 && !wait_phase(&s_free[u], (ns - 1) & 1, abort_flag, p.err)) return false;
-        if (!kOwnP && np > 0 && !wait_phase(&pv_done[u], (np - 1) & 1, abort_flag, p.err)) return false;
+        // the product that reads the buffer's last P is over
+        if (ns >= 2 && !wait_phase(&pv_done[2 * u + buf], ((ns >> 1) & 1) ^ 1, abort_flag, p.err)) return false;
         ++ns;
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t k_base = smem_u32(sKV + st * L::TILE);
+          const uint32_t k_base = smem_u32(sKV + st * L::KT);
           const uint32_t idesc_s = make_idesc(AB, 0, 0, 128, cols_of(t));
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks)
-            umma_f16(tm_s, desc_k<D>(q_base, 128, ks), desc_k<D>(k_base, 128, ks), idesc_s, ks > 0);
-          umma_commit(&s_full[u]);
+            umma_f16(tm_s + 64 * buf, desc_k<D>(q_base, 128, ks), desc_k<D>(k_base, kFwKeys, ks), idesc_s, ks > 0);
+          umma_commit(&s_full[2 * u + buf]);
           umma_commit(&kv_empty[st]);
           if (t == b - 1) umma_commit(&q_empty[st_q]);
         }
@@ -209,28 +211,28 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       bool ok = true;
       for (int t = 0; t < a && ok; ++t) ok = pass(t);
       if (ok && b > a) {
-        ok = wait_phase(&q_full[st_q], (nq / L::NQ) & 1, abort_flag, p.err) && issue_s(a);
+        ok = wait_phase(&q_full[st_q], (nq / L::NQ) & 1, abort_flag, p.err) && issue_s(a) && (b < a + 2 || issue_s(a + 1));
         ++nq;
       }
       for (int t = a; t < b && ok; ++t) {
-        if (kOwnP && t + 1 < b && !(ok = issue_s(t + 1))) break;
-        const int j = J + 2 * t + 1, st = j % L::NS, cols = cols_of(t), valid = it.valid<128>(t);
+        const int j = J + 2 * t + 1, st = j % L::NS, cols = cols_of(t), valid = it.valid<kFwKeys>(t);
         if (!(ok = wait_slot(j))) break;
-        if (valid < cols) zero_rows<D>(sKV + st * L::TILE, 128, valid);
-        if (!(ok = wait_phase(&p_full[u], np & 1, abort_flag, p.err))) break;
-        ++np;
+        if (valid < cols) zero_rows<D>(sKV + st * L::KT, kFwKeys, valid);
+        if (!(ok = wait_phase(&p_full[2 * u + (np & 1)], (np >> 1) & 1, abort_flag, p.err))) break;
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t v_base = smem_u32(sKV + st * L::TILE);
+          const uint32_t v_base = smem_u32(sKV + st * L::KT);
 #pragma unroll
-          for (int ks = 0; ks < 8; ++ks)
+          for (int ks = 0; ks < kFwKeys / 16; ++ks)
             if (ks < cols / 16)
-              umma_f16_ts(tm_o, tm_p + ks * 8, desc_mn<D>(v_base, 128, ks), idesc_o, (t > a || ks > 0) ? 1u : 0u);
-          umma_commit(&pv_done[u]);
+              umma_f16_ts(tm_o, tm_s + 64 * (np & 1) + ks * 8, desc_mn<D>(v_base, kFwKeys, ks), idesc_o,
+                          (t > a || ks > 0) ? 1u : 0u);
+          umma_commit(&pv_done[2 * u + (np & 1)]);
           umma_commit(&kv_empty[st]);
         }
         __syncwarp();
-        if (!kOwnP && t + 1 < b) ok = issue_s(t + 1);
+        ++np;
+        if (t + 2 < b) ok = issue_s(t + 2);
       }
       for (int t = b > a ? b : a; t < it.tiles && ok; ++t) ok = pass(t);
       if (!ok) break;
@@ -248,18 +250,15 @@ __global__ void __launch_bounds__(kFwThreads, 1)
     // A thread owns a row.  The maximum is lazy: P = exp2(s - m) may reach 2^8
     // before O and l are rescaled to a new one (fp32 sums, and a 16-bit P keeps
     // its relative precision), so after a row's first tiles O is hardly ever
-    // touched.  S is swept twice in chunks of 32 columns, the next chunk in
-    // flight: once for the maximum, once for P (holding a row's 128 scores
-    // between the two spills).  A chunk that no row of the warp sees is skipped
-    // and one that all see is not masked, which leaves one masked chunk of a
-    // window's slanted edge.
+    // touched.  A chunk of 32 columns that no row of the warp sees is skipped and
+    // one that all see is not masked, which leaves one masked chunk of a window's
+    // slanted edge.
     constexpr float kLazy = 8.f;
     const int u = warp >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const int t_row = row / G, g = row - t_row * G;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const uint32_t tm_s = tmem + u * 128 + lanes, tm_o = tmem + 256 + u * D + lanes;
-    const uint32_t tm_p = (kOwnP ? tmem + 384 + u * 64 : tmem + u * 128) + lanes;
+    const uint32_t tm_s0 = tmem + u * 128 + lanes, tm_o = tmem + 256 + u * D + lanes;
     const float sl2 = p.scale * 1.4426950408889634f;
     int n_it = 0, ns = 0;  // items, tiles so far
     while (true) {
@@ -276,37 +275,36 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       bool ok = true;
       float s[2][32];
       for (int t = a; t < b; ++t) {
-        const int key = it.key<128>(t);
+        const int key = it.key<kFwKeys>(t);
         const bool sinks_only = t < it.sep;
         const int lo = sinks_only ? 0 : keys.lo - key, hi = sinks_only ? 0 : keys.hi - key;
         const int sink = it.sep && !sinks_only ? 0 : keys.sink - key;
-        // columns 32 c .. + 31: which of them this row sees; per warp, chunks that some and that all rows see
-        uint32_t some = 0u, all = 0u;
-        uint32_t bits[4];
+        // columns 32 c .. + 31: which of them this row sees; per warp, whether some and whether all rows see them
+        uint32_t bits[2];
+        bool some[2], all[2];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           bits[c] = live ? seen_bits(lo, hi, sink, 32 * c) : 0u;
-          some |= (__any_sync(0xffffffffu, bits[c] != 0u) ? 1u : 0u) << c;
-          all |= (__all_sync(0xffffffffu, !live || bits[c] == 0xffffffffu) ? 1u : 0u) << c;
+          some[c] = __any_sync(0xffffffffu, bits[c] != 0u);
+          all[c] = __all_sync(0xffffffffu, !live || bits[c] == 0xffffffffu);
         }
-        if (!(ok = wait_phase(&s_full[u], ns & 1, abort_flag, p.err))) break;
+        const uint32_t tm_s = tm_s0 + 64 * (ns & 1);
+        if (!(ok = wait_phase(&s_full[2 * u + (ns & 1)], (ns >> 1) & 1, abort_flag, p.err))) break;
         ++ns;
         tc_fence_after();
+        if (some[0]) tmem_ld32(tm_s, s[0]);
+        if (some[1]) tmem_ld32(tm_s + 32, s[1]);
+        tmem_wait_values<32>(s[0]);
+        tmem_wait_values<32>(s[1]);
         float mt = -INFINITY;
-        if (some & 1u) tmem_ld32(tm_s, s[0]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_wait_values<32>(s[c & 1]);
-          if (c < 3 && (some >> (c + 1) & 1u)) tmem_ld32(tm_s + 32 * (c + 1), s[(c + 1) & 1]);
-          if (some >> c & 1u) {
-            if (!(all >> c & 1u)) mask32(s[c & 1], bits[c]);
-            mt = fmaxf(mt, max32(s[c & 1]));
+        for (int c = 0; c < 2; ++c) {
+          if (some[c]) {
+            if (!all[c]) mask32(s[c], bits[c]);
+            mt = fmaxf(mt, max32(s[c]));
           }
         }
-        if (some & 1u) tmem_ld32(tm_s, s[0]);  // in flight over what follows
         mt *= sl2;
-        // P's columns and O are free once the product of the tile before is over
-        if (t > a && !wait_phase(&pv_done[u], (ns - 2) & 1, abort_flag, p.err)) { ok = false; break; }
         const bool move = mt > m + kLazy || (m == -INFINITY && mt > -INFINITY);
         if (__any_sync(0xffffffffu, move)) {
           const float m_new = move ? mt : m;
@@ -315,6 +313,8 @@ __global__ void __launch_bounds__(kFwThreads, 1)
 #pragma unroll
           for (int j = 0; j < 2; ++j) l2[j] = mul2(l2[j], make_float2(f, f));
           if (t > a) {
+            // O is whole once the product of the tile before is over
+            if (!(ok = wait_phase(&pv_done[2 * u + (ns & 1)], ((ns - 2) >> 1) & 1, abort_flag, p.err))) break;
             tc_fence_after();
 #pragma unroll
             for (int c = 0; c < D; c += 16) {
@@ -330,20 +330,12 @@ __global__ void __launch_bounds__(kFwThreads, 1)
         const float off = m == -INFINITY ? 0.f : m;
         const float2 sc = make_float2(sl2, sl2), no2 = make_float2(-off, -off);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tmem_wait_values<32>(s[c & 1]);
-          if (c < 3 && (some >> (c + 1) & 1u)) tmem_ld32(tm_s + 32 * (c + 1), s[(c + 1) & 1]);
-          if (c == 3 && kOwnP) {  // S is in registers: the next one may be computed
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_free[u]);
-          }
+        for (int c = 0; c < 2; ++c) {
           uint32_t w[16];
-          if (some >> c & 1u) {
-            if (!(all >> c & 1u)) mask32(s[c & 1], bits[c]);
+          if (some[c]) {
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
-              float2 e = fma2(make_float2(s[c & 1][i], s[c & 1][i + 1]), sc, no2);
+              float2 e = fma2(make_float2(s[c][i], s[c][i + 1]), sc, no2);
               e.x = ex2(e.x);
               e.y = ex2(e.y);
               l2[(i >> 1) & 1] = add2(l2[(i >> 1) & 1], e);
@@ -353,16 +345,16 @@ __global__ void __launch_bounds__(kFwThreads, 1)
 #pragma unroll
             for (int i = 0; i < 16; ++i) w[i] = 0u;
           }
-          tmem_st16(tm_p + 16 * c, w);  // over S, its columns are ones that this sweep has passed
+          tmem_st16(tm_s + 16 * c, w);
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[u]);
+        if (lane == 0) mbar_arrive(&p_full[2 * u + ((ns - 1) & 1)]);
       }
       if (!ok) break;
       if (b > a) {
-        if (!wait_phase(&pv_done[u], (ns - 1) & 1, abort_flag, p.err)) break;
+        if (!wait_phase(&pv_done[2 * u + ((ns - 1) & 1)], ((ns - 1) >> 1) & 1, abort_flag, p.err)) break;
         tc_fence_after();
       }
       const float l = l2[0].x + l2[0].y + l2[1].x + l2[1].y;
@@ -408,8 +400,8 @@ int launch_fwd(const WindowParams& p, cudaStream_t s) {
   // no key at all: the maps are never read
   const void* k = p.total_k ? p.k : p.q;
   const void* v = p.total_k ? p.v : p.q;
-  if ((rc = make_tmap_3d(&mk, k, D, p.hkv, p.total_k, p.total_k ? p.k_stride : p.q_stride, 1, 128, S::kCols))) return rc;
-  if ((rc = make_tmap_3d(&mv, v, D, p.hkv, p.total_k, p.total_k ? p.v_stride : p.q_stride, 1, 128, S::kCols))) return rc;
+  if ((rc = make_tmap_3d(&mk, k, D, p.hkv, p.total_k, p.total_k ? p.k_stride : p.q_stride, 1, kFwKeys, S::kCols))) return rc;
+  if ((rc = make_tmap_3d(&mv, v, D, p.hkv, p.total_k, p.total_k ? p.v_stride : p.q_stride, 1, kFwKeys, S::kCols))) return rc;
   const int n_items = tile_slots(p.total_q, p.num_seqs, 2 * tt) * p.hkv;
   const int grid = std::min(n_items, num_sms());
   LSRM_CUDA_TRY(cudaFuncSetAttribute(window_fwd_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC));
