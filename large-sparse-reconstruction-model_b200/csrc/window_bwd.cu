@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kBwThreads, 1)
     for (int w = blockIdx.x; ok; w += gridDim.x) {
       RowItem it;
       it.stop = w >= n_items;
-      if (!it.stop && !row_item<kDqKeys>(p, w, TT, it)) continue;
+      if (!it.stop && !row_item<kDqKeys, 2>(p, w, TT, it)) continue;
       const int r = n_it % kItems;
       if (!wait_phase(&item_empty[r], ((n_it / kItems) & 1) ^ 1, abort_flag, p.err)) break;
       if (lane == 0) {
@@ -224,12 +224,8 @@ __global__ void __launch_bounds__(kBwThreads, 1)
         tc_fence_after();
         if (elect_one()) {
           const uint32_t k_base = smem_u32(sKV + sk * L::KT), v_base = smem_u32(sKV + sv * L::KT);
-#pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks)
-            umma_f16(tm_s, desc_k<D>(q_base, 128, ks), desc_k<D>(k_base, kDqKeys, ks), idesc_s, ks > 0);
-#pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks)
-            umma_f16(tm_dp, desc_k<D>(do_base, 128, ks), desc_k<D>(v_base, kDqKeys, ks), idesc_s, ks > 0);
+          mma_rows<D, 128, kDqKeys>(tm_s, q_base, k_base, idesc_s);
+          mma_rows<D, 128, kDqKeys>(tm_dp, do_base, v_base, idesc_s);
           umma_commit(&s_full[u]);
           umma_commit(&kv_empty[sv]);
           if (t == b - 1) umma_commit(&q_empty[st_q]);
@@ -252,9 +248,7 @@ __global__ void __launch_bounds__(kBwThreads, 1)
         tc_fence_after();
         if (elect_one()) {
           const uint32_t k_base = smem_u32(sKV + st * L::KT);
-#pragma unroll
-          for (int ks = 0; ks < kDqKeys / 16; ++ks)
-            umma_f16_ts(tm_dq, tm_ds + ks * 8, desc_mn<D>(k_base, kDqKeys, ks), idesc_q, (t > a || ks > 0) ? 1u : 0u);
+          mma_sum<D, kDqKeys>(tm_dq, tm_ds, k_base, idesc_q, t > a);
           umma_commit(&dq_done[u]);
           umma_commit(&kv_empty[st]);
         }
@@ -663,12 +657,8 @@ __global__ void __launch_bounds__(kBwThreads, 1)
           if (elect_one()) {
             const uint32_t q_base = smem_u32(sQ + 2 * st * L::QT), do_base = q_base + L::QT;
             const uint32_t tm_s = tmem + stage * 128;
-#pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks)
-              umma_f16(tm_s, desc_k<D>(k_base, 128, ks), desc_k<D>(q_base, kKvRows, ks), idesc_s, ks > 0);
-#pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks)
-              umma_f16(tm_s + 64, desc_k<D>(v_base, 128, ks), desc_k<D>(do_base, kKvRows, ks), idesc_s, ks > 0);
+            mma_rows<D, 128, kKvRows>(tm_s, k_base, q_base, idesc_s);
+            mma_rows<D, 128, kKvRows>(tm_s + 64, v_base, do_base, idesc_s);
             umma_commit(&s_full[stage]);
             if (t == n - 1) umma_commit(&k_empty[sk]);
           }
@@ -687,12 +677,8 @@ __global__ void __launch_bounds__(kBwThreads, 1)
             const uint32_t q_base = smem_u32(sQ + 2 * st * L::QT), do_base = q_base + L::QT;
             const uint32_t tm_p = kOwnP ? tmem + 384 + 64 * stage : tmem + 128 * stage;
             const uint32_t tm_ds = kOwnP ? tm_p + 32 : tm_p + 64;
-#pragma unroll
-            for (int ks = 0; ks < kKvRows / 16; ++ks)
-              umma_f16_ts(tm_dv, tm_p + ks * 8, desc_mn<D>(do_base, kKvRows, ks), idesc_a, (t > 0 || ks > 0) ? 1u : 0u);
-#pragma unroll
-            for (int ks = 0; ks < kKvRows / 16; ++ks)
-              umma_f16_ts(tm_dk, tm_ds + ks * 8, desc_mn<D>(q_base, kKvRows, ks), idesc_a, (t > 0 || ks > 0) ? 1u : 0u);
+            mma_sum<D, kKvRows>(tm_dv, tm_p, do_base, idesc_a, t > 0);
+            mma_sum<D, kKvRows>(tm_dk, tm_ds, q_base, idesc_a, t > 0);
             umma_commit(&acc_done[stage]);
             umma_commit(&q_empty[st]);
             if (t == n - 1) umma_commit(acc_full);

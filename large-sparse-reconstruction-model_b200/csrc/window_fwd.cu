@@ -4,39 +4,45 @@
 //   o_i = sum_j exp(s_ij - lse_i) v_j      (no key: o = 0, lse = -inf)
 //
 // One pass over a query's keys with a running maximum and sum.  A persistent
-// CTA per multiprocessor walks work items (two tiles of 128 packed query rows
-// of one kv head and the keys that either sees):
+// CTA per multiprocessor has two tiles of 128 packed query rows under way:
 //   warps 0-3, 4-7  softmax of row tile 0 and 1, a row a thread: S from TMEM,
 //                   mask, running maximum, P = exp2(S - m) to TMEM as 16-bit
 //                   operand, at the end O / l to global memory
 //   warps 8, 9      tensor-core issue for row tile 0 and 1: S = Q K^T, O += P V
 //                   (P from TMEM)
-//   warp 10         producer: work items, TMA of Q, K and V
-// K and V tiles (64 keys) go through one ring and serve both row tiles, which
-// halves the L2 reads per product.  S has two buffers of 64 columns a row tile
-// and P lies over its S, so that the products of the tiles before and after run
-// under a tile's softmax (at 128 keys a buffer TMEM holds one, and the two row
-// tiles fell into step: both in their softmax, then both waiting).  Rounding: S, m, l and O are fp32; P is
-// rounded to the operand type (the sum l takes it unrounded), O once at the end.
+//   warps 10, 11    producers: work items, TMA of Q, K and V
+// S has two buffers of 64 columns a row tile and P lies over its S, so that the
+// products of the tiles before and after run under a tile's softmax (at 128 keys
+// a buffer TMEM holds one, and the two row tiles fell into step: both in their
+// softmax, then both waiting).  At 128 channels an item is two neighbouring row
+// tiles, and each K and V tile (64 keys) of its ring serves both, which halves
+// the L2 reads that would bound it.  Up to 64 channels each row tile is an item
+// of its own with its own ring and producer: sharing made the one ahead wait
+// for the other at every item's end.  Rounding: S, m, l and O are fp32; P is
+// rounded to the operand type (the sum l takes it unrounded), O once at the
+// end.
 #include "window_host.h"
 #include "window_tile.cuh"
 
 namespace lsrm {
 namespace {
 
-constexpr int kFwThreads = 352;
+constexpr int kFwThreads = 384;
 constexpr int kFwKeys = 64;
+
 template <int D>
 struct FwSmem {
   static constexpr int QT = TileShape<D>::bytes(128), KT = TileShape<D>::bytes(kFwKeys);
   static constexpr int NQ = D == 128 ? 1 : 2;  // Q buffers of each row tile
-  static constexpr int NS = D == 128 ? 9 : 12;  // K / V ring
+  static constexpr int RINGS = D == 128 ? 1 : 2;    // rings of work items and of K / V tiles
+  static constexpr int ROWS = 2 / RINGS;            // row tiles of an item
+  static constexpr int NS = D == 128 ? 9 : 10;      // K / V tiles of a ring
   static constexpr int OFF_KV = 2 * NQ * QT;
-  static constexpr int OFF_ITEM = OFF_KV + NS * KT;
-  static constexpr int OFF_BAR = OFF_ITEM + kItems * (int)sizeof(RowItem);
-  // q_full[2][NQ], q_empty[2][NQ], kv_full[NS], kv_empty[NS], s_full[2][2], p_full[2][2], pv_done[2][2],
-  // item_full[], item_empty[], mma_done[2]
-  static constexpr int NBAR = 4 * NQ + 2 * NS + 12 + 2 * kItems + 2;
+  static constexpr int OFF_ITEM = OFF_KV + RINGS * NS * KT;
+  static constexpr int OFF_BAR = OFF_ITEM + RINGS * kItems * (int)sizeof(RowItem);
+  // q_full[2][NQ], q_empty[2][NQ], kv_full[RINGS][NS], kv_empty[RINGS][NS], s_full[2][2], p_full[2][2],
+  // pv_done[2][2], item_full[RINGS][], item_empty[RINGS][], mma_done[2]
+  static constexpr int NBAR = 4 * NQ + 2 * RINGS * NS + 12 + 2 * RINGS * kItems + 2;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int BYTES = OFF_MISC + 16 + 1024;
   static constexpr int ALLOC = BYTES > kOneCtaPerSmSmem ? BYTES : kOneCtaPerSmSmem;
@@ -57,14 +63,14 @@ __global__ void __launch_bounds__(kFwThreads, 1)
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* q_empty = q_full + 2 * L::NQ;
   uint64_t* kv_full = q_empty + 2 * L::NQ;
-  uint64_t* kv_empty = kv_full + L::NS;
-  uint64_t* s_full = kv_empty + L::NS;
+  uint64_t* kv_empty = kv_full + L::RINGS * L::NS;
+  uint64_t* s_full = kv_empty + L::RINGS * L::NS;
   // [row tile][buffer]: two tiles are under way, so each has its own phases
   uint64_t* p_full = s_full + 4;
   uint64_t* pv_done = p_full + 4;
   uint64_t* item_full = pv_done + 4;
-  uint64_t* item_empty = item_full + kItems;
-  uint64_t* mma_done = item_empty + kItems;
+  uint64_t* item_empty = item_full + L::RINGS * kItems;
+  uint64_t* mma_done = item_empty + L::RINGS * kItems;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
 
@@ -73,7 +79,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * L::NQ; ++i) mbar_init(&q_full[i], 1), mbar_init(&q_empty[i], 1);
-    for (int i = 0; i < L::NS; ++i) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], 2);
+    for (int i = 0; i < L::RINGS * L::NS; ++i) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], L::ROWS);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[2 * i], 1);
       mbar_init(&s_full[2 * i + 1], 1);
@@ -83,7 +89,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       mbar_init(&pv_done[2 * i + 1], 1);
       mbar_init(&mma_done[i], 1);
     }
-    for (int i = 0; i < kItems; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 10);
+    for (int i = 0; i < L::RINGS * kItems; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 5 * L::ROWS);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -97,7 +103,17 @@ __global__ void __launch_bounds__(kFwThreads, 1)
   const uint32_t tmem = *tmem_slot;
   // TMEM columns: S of row tile u, buffer i [128 u + 64 i, +64) with P over its first half; O [256 + u D, +D)
 
-  if (warp == 10) {
+  // this warp's row tile (of the CTA, and of its item) and ring
+  const int u = warp >= 10 ? warp - 10 : warp >= 8 ? warp - 8 : warp >> 2;
+  const int ring = L::RINGS == 1 ? 0 : u, ui = L::RINGS == 1 ? u : 0;
+  items += ring * kItems;
+  item_full += ring * kItems;
+  item_empty += ring * kItems;
+  sKV += ring * L::NS * L::KT;
+  kv_full += ring * L::NS;
+  kv_empty += ring * L::NS;
+
+  if (warp >= 10) {
     // ------------------------------ producer ------------------------------
     // The whole warp walks the items; one elected lane issues (under elect.sync
     // the compiler knows that one lane is active and issues TMA and tensor-core
@@ -109,13 +125,13 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       tma_prefetch_desc(&tm_v);
     }
     const uint32_t q_bytes = (uint32_t)(G * TT * D * 2);
-    int n_it = 0, J = 0, nq[2] = {0, 0};
-    bool ok = true;
-    for (int w = blockIdx.x; ok; w += gridDim.x) {
+    int n_it = 0, J = 0, nq[L::ROWS] = {};
+    bool ok = u < L::RINGS;
+    for (int w = blockIdx.x * L::RINGS + ring; ok; w += gridDim.x * L::RINGS) {
       RowItem it;
       it.stop = w >= n_items;
       if (!it.stop) {
-        if (!row_item<kFwKeys>(p, w, TT, it)) continue;
+        if (!row_item<kFwKeys, L::ROWS>(p, w, TT, it)) continue;
       }
       const int r = n_it % kItems;
       if (!wait_phase(&item_empty[r], ((n_it / kItems) & 1) ^ 1, abort_flag, p.err)) break;
@@ -126,16 +142,17 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       __syncwarp();
       ++n_it;
       if (it.stop) break;
-      for (int u = 0; u < 2 && ok; ++u) {
-        if (it.b[u] <= it.a[u]) continue;
-        const int st = u * L::NQ + nq[u] % L::NQ;
-        if (!(ok = wait_phase(&q_empty[st], ((nq[u] / L::NQ) & 1) ^ 1, abort_flag, p.err))) break;
+#pragma unroll
+      for (int i = 0; i < L::ROWS; ++i) {
+        if (!ok || it.b[i] <= it.a[i]) continue;
+        const int st = (ring + i) * L::NQ + nq[i] % L::NQ;
+        if (!(ok = wait_phase(&q_empty[st], ((nq[i] / L::NQ) & 1) ^ 1, abort_flag, p.err))) continue;
         if (elect_one()) {
           mbar_arrive_expect_tx(&q_full[st], q_bytes);
-          load_tile<D>(sQ + st * L::QT, 128, &tm_q, it.hk * G, it.tok + u * TT, &q_full[st]);
+          load_tile<D>(sQ + st * L::QT, 128, &tm_q, it.hk * G, it.tok + i * TT, &q_full[st]);
         }
         __syncwarp();
-        ++nq[u];
+        ++nq[i];
       }
       for (int t = 0; t < it.tiles && ok; ++t) {
         const int key = it.key0 + it.key<kFwKeys>(t);
@@ -153,15 +170,14 @@ __global__ void __launch_bounds__(kFwThreads, 1)
     }
     // after an abort: copies in flight land before the CTA exits
     if (lane == 0 && *abort_flag) {
-      for (int u = 0; u < 2; ++u)
-        for (int k = max(0, nq[u] - L::NQ); k < nq[u]; ++k)
-          mbar_wait_drain(&q_full[u * L::NQ + k % L::NQ], (k / L::NQ) & 1);
+      for (int i = 0; i < L::ROWS; ++i)
+        for (int k = max(0, nq[i] - L::NQ); k < nq[i]; ++k)
+          mbar_wait_drain(&q_full[(ring + i) * L::NQ + k % L::NQ], (k / L::NQ) & 1);
       for (int j = max(0, J - L::NS); j < J; ++j) mbar_wait_drain(&kv_full[j % L::NS], (j / L::NS) & 1);
     }
     __syncwarp();
   } else if (warp >= 8) {
     // --------------------------- tensor-core issue ---------------------------
-    const int u = warp - 8;
     const uint32_t tm_s = tmem + u * 128, tm_o = tmem + 256 + u * D;
     const uint32_t idesc_o = make_idesc(AB, 0, 1, 128, D);
     int n_it = 0, J = 0, nq = 0;         // items, ring slots, Q tiles so far
@@ -174,7 +190,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       if (it.stop) break;
       const int st_q = u * L::NQ + nq % L::NQ;
       const uint32_t q_base = smem_u32(sQ + st_q * L::QT);
-      const int a = it.a[u], b = it.b[u];
+      const int a = it.a[ui], b = it.b[ui];
       // sinks of their own tile: only as many columns as they need
       auto cols_of = [&](int t) { return t < it.sep ? min(kFwKeys, (p.sinks - t * kFwKeys + 31) / 32 * 32) : kFwKeys; };
       auto wait_slot = [&](int j) { return wait_phase(&kv_full[j % L::NS], (j / L::NS) & 1, abort_flag, p.err); };
@@ -198,9 +214,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
         if (elect_one()) {
           const uint32_t k_base = smem_u32(sKV + st * L::KT);
           const uint32_t idesc_s = make_idesc(AB, 0, 0, 128, cols_of(t));
-#pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks)
-            umma_f16(tm_s + 64 * buf, desc_k<D>(q_base, 128, ks), desc_k<D>(k_base, kFwKeys, ks), idesc_s, ks > 0);
+          mma_rows<D, 128, kFwKeys>(tm_s + 64 * buf, q_base, k_base, idesc_s);
           umma_commit(&s_full[2 * u + buf]);
           umma_commit(&kv_empty[st]);
           if (t == b - 1) umma_commit(&q_empty[st_q]);
@@ -222,11 +236,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
         tc_fence_after();
         if (elect_one()) {
           const uint32_t v_base = smem_u32(sKV + st * L::KT);
-#pragma unroll
-          for (int ks = 0; ks < kFwKeys / 16; ++ks)
-            if (ks < cols / 16)
-              umma_f16_ts(tm_o, tm_s + 64 * (np & 1) + ks * 8, desc_mn<D>(v_base, kFwKeys, ks), idesc_o,
-                          (t > a || ks > 0) ? 1u : 0u);
+          mma_sum<D, kFwKeys>(tm_o, tm_s + 64 * (np & 1), v_base, idesc_o, t > a, cols / 16);
           umma_commit(&pv_done[2 * u + (np & 1)]);
           umma_commit(&kv_empty[st]);
         }
@@ -254,7 +264,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
     // one that all see is not masked, which leaves one masked chunk of a window's
     // slanted edge.
     constexpr float kLazy = 8.f;
-    const int u = warp >> 2, quarter = warp & 3;
+    const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const int t_row = row / G, g = row - t_row * G;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
@@ -267,26 +277,31 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       const RowItem& it = items[r];
       ++n_it;
       if (it.stop) break;
-      const int a = it.a[u], b = it.b[u];
-      const bool live = t_row < it.n[u] && t_row < TT;
-      const RowKeys keys = row_keys(p, it.pos + u * TT + t_row, it.lk);
+      const int a = it.a[ui], b = it.b[ui];
+      const bool live = t_row < it.n[ui] && t_row < TT;
+      const RowKeys keys = row_keys(p, it.pos + ui * TT + t_row, it.lk);
+      const WarpKeys wk = warp_keys(keys, live);
       float m = -INFINITY;
       float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       bool ok = true;
       float s[2][32];
       for (int t = a; t < b; ++t) {
+        // columns 32 c .. + 31: which of them this row sees; per warp, whether some and whether all rows see them.
+        // Between a window's edges all see all, which two comparisons tell (spelling the bits out took longer than
+        // the exponentials).
         const int key = it.key<kFwKeys>(t);
-        const bool sinks_only = t < it.sep;
-        const int lo = sinks_only ? 0 : keys.lo - key, hi = sinks_only ? 0 : keys.hi - key;
-        const int sink = it.sep && !sinks_only ? 0 : keys.sink - key;
-        // columns 32 c .. + 31: which of them this row sees; per warp, whether some and whether all rows see them
-        uint32_t bits[2];
-        bool some[2], all[2];
+        uint32_t bits[2] = {0xffffffffu, 0xffffffffu};
+        bool some[2] = {true, true}, all[2] = {true, true};
+        if (key < wk.all_lo || key + kFwKeys > wk.all_hi || t < it.sep) {
+          const bool sinks_only = t < it.sep;
+          const int lo = sinks_only ? 0 : keys.lo - key, hi = sinks_only ? 0 : keys.hi - key;
+          const int sink = it.sep && !sinks_only ? 0 : keys.sink - key;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          bits[c] = live ? seen_bits(lo, hi, sink, 32 * c) : 0u;
-          some[c] = __any_sync(0xffffffffu, bits[c] != 0u);
-          all[c] = __all_sync(0xffffffffu, !live || bits[c] == 0xffffffffu);
+          for (int c = 0; c < 2; ++c) {
+            bits[c] = live ? seen_bits(lo, hi, sink, 32 * c) : 0u;
+            some[c] = __any_sync(0xffffffffu, bits[c] != 0u);
+            all[c] = __all_sync(0xffffffffu, !live || bits[c] == 0xffffffffu);
+          }
         }
         const uint32_t tm_s = tm_s0 + 64 * (ns & 1);
         if (!(ok = wait_phase(&s_full[2 * u + (ns & 1)], (ns >> 1) & 1, abort_flag, p.err))) break;
@@ -359,7 +374,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       }
       const float l = l2[0].x + l2[0].y + l2[1].x + l2[1].y;
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      const long long orow = (long long)(it.tok + u * TT + t_row) * p.hq + it.hk * G + g;
+      const long long orow = (long long)(it.tok + ui * TT + t_row) * p.hq + it.hk * G + g;
       uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + orow * D);
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
@@ -402,8 +417,8 @@ int launch_fwd(const WindowParams& p, cudaStream_t s) {
   const void* v = p.total_k ? p.v : p.q;
   if ((rc = make_tmap_3d(&mk, k, D, p.hkv, p.total_k, p.total_k ? p.k_stride : p.q_stride, 1, kFwKeys, S::kCols))) return rc;
   if ((rc = make_tmap_3d(&mv, v, D, p.hkv, p.total_k, p.total_k ? p.v_stride : p.q_stride, 1, kFwKeys, S::kCols))) return rc;
-  const int n_items = tile_slots(p.total_q, p.num_seqs, 2 * tt) * p.hkv;
-  const int grid = std::min(n_items, num_sms());
+  const int n_items = tile_slots(p.total_q, p.num_seqs, L::ROWS * tt) * p.hkv;
+  const int grid = std::min((n_items + L::RINGS - 1) / L::RINGS, num_sms());
   LSRM_CUDA_TRY(cudaFuncSetAttribute(window_fwd_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC));
   window_fwd_kernel<D, BF16><<<grid, kFwThreads, L::ALLOC, s>>>(mq, mk, mv, p, n_items);
   LSRM_LAUNCH_CHECK();

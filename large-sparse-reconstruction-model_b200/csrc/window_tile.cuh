@@ -44,19 +44,76 @@ __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volat
   return __all_sync(0xffffffffu, ok);
 }
 
-// Descriptors of a [rows][D] tile at shared address `base`: as a K-major
-// operand (the contraction runs over D; step ks takes 16 channels), and as an
-// MN-major one (the contraction runs over the rows; step ks takes 16 of them).
+// Operand descriptors of a [ROWS][D] tile, as their two words.  The upper one is
+// a constant, and the lower one of a later step is the first one's plus a
+// constant, so that one thread issues a product in a few instructions (building
+// each descriptor from its fields took some 60 cycles a product, and the
+// issuing warp bounded the kernels).
 template <int D>
-__device__ __forceinline__ uint64_t desc_k(uint32_t base, int rows, int ks) {
+__device__ __forceinline__ constexpr uint32_t desc_hi() {
+  using S = TileShape<D>;
+  return (uint32_t)((8 * S::RB) >> 4) | (1u << 14) | ((uint32_t)S::SWZ << 29);
+}
+// K-major (the contraction runs over D, step ks takes 16 channels).
+template <int D>
+__device__ __forceinline__ uint32_t desc_k(uint32_t base) {
+  return (base >> 4) | (1u << 16);
+}
+template <int D, int ROWS>
+__device__ __forceinline__ constexpr uint32_t step_k(int ks) {
   using S = TileShape<D>;
   constexpr int per = S::kCols / 16;
-  return make_sdesc(base + (ks / per) * rows * S::RB + (ks % per) * 32, 16, 8 * S::RB, S::SWZ);
+  return (uint32_t)((ks / per) * ROWS * S::RB + (ks % per) * 32) >> 4;
+}
+// MN-major (the contraction runs over the rows, step ks takes 16 of them).
+template <int D, int ROWS>
+__device__ __forceinline__ uint32_t desc_mn(uint32_t base) {
+  return (base >> 4) | ((uint32_t)(ROWS * TileShape<D>::RB >> 4) << 16);
 }
 template <int D>
-__device__ __forceinline__ uint64_t desc_mn(uint32_t base, int rows, int ks) {
-  using S = TileShape<D>;
-  return make_sdesc(base + ks * 16 * S::RB, rows * S::RB, 8 * S::RB, S::SWZ);
+__device__ __forceinline__ constexpr uint32_t step_mn(int ks) {
+  return (uint32_t)(ks * 16 * TileShape<D>::RB) >> 4;
+}
+
+// D[tmem] (+)= A B, as umma_f16 / umma_f16_ts of common.cuh; ACC is known at
+// compile time, or `acc` says.
+template <int HI>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %4};\n\tmov.b64 db, {%2, %4};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "n"(HI), "r"((uint32_t)acc)
+      : "memory");
+}
+template <int HI>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint32_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %4};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "r"(b), "r"(idesc), "n"(HI), "r"((uint32_t)acc)
+      : "memory");
+}
+
+// D = A B^T over the D channels of an [A_ROWS][D] and a [B_ROWS][D] tile.
+template <int D, int A_ROWS, int B_ROWS>
+__device__ __forceinline__ void mma_rows(uint32_t d, uint32_t a_base, uint32_t b_base, uint32_t idesc) {
+  const uint32_t a = desc_k<D>(a_base), b = desc_k<D>(b_base);
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks)
+    mma_ss<(int)desc_hi<D>()>(d, a + step_k<D, A_ROWS>(ks), b + step_k<D, B_ROWS>(ks), idesc, ks > 0);
+}
+// D (+)= A B for A [128][16 steps] in TMEM and B a [ROWS][D] tile.
+template <int D, int ROWS>
+__device__ __forceinline__ void mma_sum(uint32_t d, uint32_t a_tmem, uint32_t b_base, uint32_t idesc, bool acc,
+                                        int steps = ROWS / 16) {
+  const uint32_t b = desc_mn<D, ROWS>(b_base);
+#pragma unroll
+  for (int ks = 0; ks < ROWS / 16; ++ks)
+    if (ks < steps) mma_ts<(int)desc_hi<D>()>(d, a_tmem + ks * 8, b + step_mn<D>(ks), idesc, acc || ks > 0);
 }
 
 // TMA of one operand tile: rows of `heads` heads x tokens from (head, token).
@@ -165,10 +222,25 @@ __device__ __forceinline__ void tmem_wait_values(float* v) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+f"(v[i]));
 }
 
+// Where the rows of a warp stand to the window's keys: keys in [all_lo, all_hi)
+// are seen by every row, keys outside [any_lo, any_hi) by none (rows that are
+// not live do not count).
+struct WarpKeys {
+  int any_lo, any_hi, all_lo, all_hi;
+};
+__device__ __forceinline__ WarpKeys warp_keys(const RowKeys& r, bool live) {
+  WarpKeys w;
+  w.any_lo = __reduce_min_sync(0xffffffffu, live ? r.lo : 0x7fffffff);
+  w.any_hi = __reduce_max_sync(0xffffffffu, live ? r.hi : 0);
+  w.all_lo = __reduce_max_sync(0xffffffffu, live ? r.lo : 0);
+  w.all_hi = __reduce_min_sync(0xffffffffu, live ? r.hi : 0x7fffffff);
+  return w;
+}
+
 // ---------------------------------------------------------------------------
-// Work items of the kernels that keep query rows (forward, dQ): two tiles of
-// TT tokens x G heads, one kv head, and the key tiles (KT keys) that either
-// sees.  The producer plans them; the other warps read them from a ring.
+// Work items of the kernels that keep query rows (forward, dQ): one or two
+// tiles of TT tokens x G heads, one kv head, and the key tiles (KT keys) that
+// either sees.  The producer plans them; the other warps read them from a ring.
 // ---------------------------------------------------------------------------
 constexpr int kItems = 4;
 
@@ -193,18 +265,18 @@ struct RowItem {
   }
 };
 
-// Plans work item `w`; false when it holds no query.
-template <int KT>
+// Plans work item `w` of ROWS row tiles; false when it holds no query.
+template <int KT, int ROWS>
 __device__ __forceinline__ bool row_item(const WindowParams& p, int w, int tt, RowItem& it) {
   const int slot = w / p.hkv;
   it.hk = w - slot * p.hkv;
-  const int b = seq_of_slot(p.cu_q, p.num_seqs, 2 * tt, slot);
+  const int b = seq_of_slot(p.cu_q, p.num_seqs, ROWS * tt, slot);
   const Seq s = seq_of(p, b);
-  const int i0 = (slot - (p.cu_q[b] / (2 * tt) + b)) * 2 * tt;
+  const int i0 = (slot - (p.cu_q[b] / (ROWS * tt) + b)) * ROWS * tt;
   if (i0 < 0 || i0 >= s.lq) return false;
   it.tok = s.q0 + i0;
   it.n[0] = min(tt, s.lq - i0);
-  it.n[1] = max(0, min(tt, s.lq - i0 - tt));
+  it.n[1] = ROWS > 1 ? max(0, min(tt, s.lq - i0 - tt)) : 0;
   it.lk = b < p.num_seqs ? s.lk : 0;
   it.pos = i0 + s.lk - s.lq;
   it.key0 = s.k0;
