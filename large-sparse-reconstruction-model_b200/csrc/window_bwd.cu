@@ -386,9 +386,12 @@ __global__ void __launch_bounds__(kBwThreads, 1)
 //   S^T = K Q^T, dP^T = V dO^T (128 keys x 64 rows, two TMEM stages)
 //   warps 0-3 (even query tiles), 4-7 (odd ones): a key a thread, P^T and dS^T
 //   as 16-bit operands in TMEM;  dV += P^T dO, dK += dS^T Q
-//   warp 8 issues, warp 9 loads, warp 10 gathers the rows' lse and delta.
+//   warp 8 issues the first two products, warp 11 the sums (one warp for all
+//   four spends longer on issuing than they take), warp 9 loads, warp 10 gathers
+//   the rows' lse and delta.
 
 constexpr int kKvRows = 64;  // packed query rows of a tile
+constexpr int kKvThreads = 384;
 
 struct KvItem {
   int stop;
@@ -409,8 +412,8 @@ struct KvSmem {
   static constexpr int OFF_ITEM = OFF_STAT + NS * 2 * kKvRows * 4;
   static constexpr int OFF_BAR = OFF_ITEM + kItems * (int)sizeof(KvItem);
   // k_full[NK], k_empty[NK], q_full[NS], stat_full[NS], q_empty[NS], s_full[2], p_full[2], acc_done[2], acc_full,
-  // acc_free, item_full[], item_empty[], mma_done
-  static constexpr int NBAR = 2 * NK + 3 * NS + 6 + 2 + 2 * kItems + 1;
+  // acc_free, item_full[], item_empty[], mma_done[2]
+  static constexpr int NBAR = 2 * NK + 3 * NS + 6 + 2 + 2 * kItems + 2;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int BYTES = OFF_MISC + 16 + 1024;
   static constexpr int ALLOC = BYTES > kOneCtaPerSmSmem ? BYTES : kOneCtaPerSmSmem;
@@ -481,7 +484,7 @@ __device__ __forceinline__ bool kv_item(const WindowBwdParams& p, int w, int D, 
 }
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kBwThreads, 1)
+__global__ void __launch_bounds__(kKvThreads, 1)
     window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                       const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                       const WindowBwdParams p, const int n_items) {
@@ -518,8 +521,9 @@ __global__ void __launch_bounds__(kBwThreads, 1)
     for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&acc_done[i], 1);
     mbar_init(acc_full, 1);
     mbar_init(acc_free, 8);
-    for (int i = 0; i < kItems; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 10);
-    mbar_init(mma_done, 1);
+    for (int i = 0; i < kItems; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 11);
+    mbar_init(&mma_done[0], 1);
+    mbar_init(&mma_done[1], 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -624,10 +628,62 @@ __global__ void __launch_bounds__(kBwThreads, 1)
       if (lane == 0) mbar_arrive(&item_empty[r]);
     }
   } else if (warp == 8) {
-    // --------------------------- tensor-core issue ---------------------------
-    const uint32_t idesc_s = make_idesc(AB, 0, 0, 128, kKvRows), idesc_a = make_idesc(AB, 0, 1, 128, D);
+    // --------------------- tensor-core issue: S^T and dP^T -------------------
+    const uint32_t idesc = make_idesc(AB, 0, 0, 128, kKvRows);
+    int n_it = 0, J = 0, nk = 0;  // items, query tiles, K tiles so far
+    while (true) {
+      const int r = n_it % kItems;
+      if (!wait_phase(&item_full[r], (n_it / kItems) & 1, abort_flag, p.err)) break;
+      const KvItem& it = items[r];
+      ++n_it;
+      if (it.stop) break;
+      const int n = (it.ntok + TT - 1) / TT, ntok = it.ntok;
+      bool ok = true;
+      if (n > 0) {
+        const int sk = nk % L::NK;
+        const uint32_t k_base = smem_u32(sK + 2 * sk * L::KT), v_base = k_base + L::KT;
+        if (!wait_phase(&k_full[sk], (nk / L::NK) & 1, abort_flag, p.err)) break;
+        ++nk;
+        for (int t = 0; t < n; ++t, ++J) {
+          const int st = J % L::NS, stage = J & 1;
+          if (!(ok = wait_phase(&q_full[st], (J / L::NS) & 1, abort_flag, p.err))) break;
+          // rows that hold no query of the sequence must not reach the sums, not even times zero
+          const int rows = min(TT, ntok - t * TT) * G;
+          if (rows < kKvRows) {
+            zero_rows<D>(sQ + 2 * st * L::QT, kKvRows, rows);
+            zero_rows<D>(sQ + (2 * st + 1) * L::QT, kKvRows, rows);
+          }
+          // the stage's last S^T and dP^T have been read; where P^T and dS^T lie over them, the sums that read those
+          // are over
+          if (J >= 2 && !(ok = wait_phase(kOwnP ? &p_full[stage] : &acc_done[stage], ((J >> 1) & 1) ^ 1, abort_flag, p.err)))
+            break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t q_base = smem_u32(sQ + 2 * st * L::QT), do_base = q_base + L::QT;
+            const uint32_t tm_s = tmem + stage * 128;
+            mma_rows<D, 128, kKvRows>(tm_s, k_base, q_base, idesc);
+            mma_rows<D, 128, kKvRows>(tm_s + 64, v_base, do_base, idesc);
+            umma_commit(&s_full[stage]);
+            if (t == n - 1) umma_commit(&k_empty[sk]);
+          }
+          __syncwarp();
+        }
+      }
+      if (!ok) break;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[r]);
+    }
+    if (elect_one()) {
+      umma_commit(&mma_done[0]);
+      mbar_wait_drain(&mma_done[0], 0);
+    }
+    __syncwarp();
+  } else if (warp == 11) {
+    // ------------------------ tensor-core issue: dV and dK --------------------
+    // (S^T's issue has seen the tile's Q and dO, and zeroed what is no query, before P^T can be announced)
+    const uint32_t idesc = make_idesc(AB, 0, 1, 128, D);
     const uint32_t tm_dv = tmem + 256, tm_dk = tmem + 256 + D;
-    int n_it = 0, J = 0, nk = 0, n_acc = 0;  // items, query tiles, K tiles, items with sums so far
+    int n_it = 0, J = 0, n_acc = 0;  // items, query tiles, items with sums so far
     while (true) {
       const int r = n_it % kItems;
       if (!wait_phase(&item_full[r], (n_it / kItems) & 1, abort_flag, p.err)) break;
@@ -636,66 +692,33 @@ __global__ void __launch_bounds__(kBwThreads, 1)
       if (it.stop) break;
       const int n = (it.ntok + TT - 1) / TT;
       bool ok = true;
-      if (n > 0) {
-        const int sk = nk % L::NK;
-        const uint32_t k_base = smem_u32(sK + 2 * sk * L::KT), v_base = k_base + L::KT;
-        if (!wait_phase(&k_full[sk], (nk / L::NK) & 1, abort_flag, p.err)) break;
-        ++nk;
-        auto issue_s = [&](int t) {
-          const int j = J + t, st = j % L::NS, stage = j & 1;
-          if (!wait_phase(&q_full[st], (j / L::NS) & 1, abort_flag, p.err)) return false;
-          // rows that hold no query of the sequence must not reach the sums, not even times zero
-          const int rows = min(TT, it.ntok - t * TT) * G;
-          if (rows < kKvRows) {
-            zero_rows<D>(sQ + 2 * st * L::QT, kKvRows, rows);
-            zero_rows<D>(sQ + (2 * st + 1) * L::QT, kKvRows, rows);
-          }
-          // S^T and dP^T of the stage's last tile were read before its P^T was announced; where P^T and dS^T lie
-          // over them, the sums that read those are over
-          if (!kOwnP && j >= 2 && !wait_phase(&acc_done[stage], ((j >> 1) & 1) ^ 1, abort_flag, p.err)) return false;
-          tc_fence_after();
-          if (elect_one()) {
-            const uint32_t q_base = smem_u32(sQ + 2 * st * L::QT), do_base = q_base + L::QT;
-            const uint32_t tm_s = tmem + stage * 128;
-            mma_rows<D, 128, kKvRows>(tm_s, k_base, q_base, idesc_s);
-            mma_rows<D, 128, kKvRows>(tm_s + 64, v_base, do_base, idesc_s);
-            umma_commit(&s_full[stage]);
-            if (t == n - 1) umma_commit(&k_empty[sk]);
-          }
-          __syncwarp();
-          return true;
-        };
-        ok = issue_s(0) && (n < 2 || issue_s(1));
-        for (int t = 0; t < n && ok; ++t) {
-          const int j = J + t, st = j % L::NS, stage = j & 1;
-          if (!(ok = wait_phase(&p_full[stage], (j >> 1) & 1, abort_flag, p.err))) break;
-          if (kOwnP && t + 2 < n && !(ok = issue_s(t + 2))) break;
-          // the last item's sums have been read
-          if (t == 0 && n_acc > 0 && !(ok = wait_phase(acc_free, (n_acc - 1) & 1, abort_flag, p.err))) break;
-          tc_fence_after();
-          if (elect_one()) {
-            const uint32_t q_base = smem_u32(sQ + 2 * st * L::QT), do_base = q_base + L::QT;
-            const uint32_t tm_p = kOwnP ? tmem + 384 + 64 * stage : tmem + 128 * stage;
-            const uint32_t tm_ds = kOwnP ? tm_p + 32 : tm_p + 64;
-            mma_sum<D, kKvRows>(tm_dv, tm_p, do_base, idesc_a, t > 0);
-            mma_sum<D, kKvRows>(tm_dk, tm_ds, q_base, idesc_a, t > 0);
-            umma_commit(&acc_done[stage]);
-            umma_commit(&q_empty[st]);
-            if (t == n - 1) umma_commit(acc_full);
-          }
-          __syncwarp();
-          if (!kOwnP && t + 2 < n) ok = issue_s(t + 2);
+      for (int t = 0; t < n; ++t, ++J) {
+        const int st = J % L::NS, stage = J & 1;
+        // the last item's sums have been read
+        if (t == 0 && n_acc > 0 && !(ok = wait_phase(acc_free, (n_acc - 1) & 1, abort_flag, p.err))) break;
+        if (!(ok = wait_phase(&q_full[st], (J / L::NS) & 1, abort_flag, p.err))) break;
+        if (!(ok = wait_phase(&p_full[stage], (J >> 1) & 1, abort_flag, p.err))) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t q_base = smem_u32(sQ + 2 * st * L::QT), do_base = q_base + L::QT;
+          const uint32_t tm_p = kOwnP ? tmem + 384 + 64 * stage : tmem + 128 * stage;
+          const uint32_t tm_ds = kOwnP ? tm_p + 32 : tm_p + 64;
+          mma_sum<D, kKvRows>(tm_dv, tm_p, do_base, idesc, t > 0);
+          mma_sum<D, kKvRows>(tm_dk, tm_ds, q_base, idesc, t > 0);
+          umma_commit(&acc_done[stage]);
+          umma_commit(&q_empty[st]);
+          if (t == n - 1) umma_commit(acc_full);
         }
-        if (!ok) break;
-        ++n_acc;
-        J += n;
+        __syncwarp();
       }
+      if (!ok) break;
+      if (n > 0) ++n_acc;
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[r]);
     }
     if (elect_one()) {
-      umma_commit(mma_done);
-      mbar_wait_drain(mma_done, 0);
+      umma_commit(&mma_done[1]);
+      mbar_wait_drain(&mma_done[1], 0);
     }
     __syncwarp();
   } else {
@@ -935,7 +958,7 @@ int launch_bwd(const WindowBwdParams& p, cudaStream_t s) {
       const int n_items = (tile_slots(p.total_k, p.num_seqs, 128) + p.chunk_slots) * p.hkv;
       LSRM_CUDA_TRY(cudaFuncSetAttribute(window_dkv_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          KvSmem<D>::ALLOC));
-      window_dkv_kernel<D, BF16><<<std::min(n_items, num_sms()), kBwThreads, KvSmem<D>::ALLOC, s>>>(mq, md, mk, mv, p,
+      window_dkv_kernel<D, BF16><<<std::min(n_items, num_sms()), kKvThreads, KvSmem<D>::ALLOC, s>>>(mq, md, mk, mv, p,
                                                                                                     n_items);
       LSRM_LAUNCH_CHECK();
     }
