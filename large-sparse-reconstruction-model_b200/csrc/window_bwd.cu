@@ -55,8 +55,14 @@ __global__ void __launch_bounds__(256) window_delta_kernel(const uint4* __restri
 // ------------------------------- dQ ----------------------------------------
 // As the forward: a persistent CTA, two tiles of 128 packed query rows, key
 // tiles of 64 (S, dP and dQ of both row tiles fill TMEM at 128 channels).
+//   warps 0-7, 8-15  dS of row tile 0 and 1: two threads a row, 32 keys each.  What a
+//                    thread does between two waits is a chain of short latencies,
+//                    so a multiprocessor needs many of them (with one thread a row
+//                    the same code took 1.4 times as long).
+//   warps 16, 17     tensor-core issue for row tile 0 and 1
+//   warp 18          producer
 
-constexpr int kBwThreads = 352;
+constexpr int kBwThreads = 608;
 constexpr int kDqKeys = 64;
 
 template <int D>
@@ -110,12 +116,12 @@ __global__ void __launch_bounds__(kBwThreads, 1)
     for (int i = 0; i < L::NS; ++i) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], 2);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&s_free[i], 4);
-      mbar_init(&ds_full[i], 4);
+      mbar_init(&s_free[i], 8);
+      mbar_init(&ds_full[i], 8);
       mbar_init(&dq_done[i], 1);
       mbar_init(&mma_done[i], 1);
     }
-    for (int i = 0; i < kItems; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 10);
+    for (int i = 0; i < kItems; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 18);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -131,7 +137,7 @@ __global__ void __launch_bounds__(kBwThreads, 1)
   // [384 + 32 u, +32) up to D = 64, else over S
   constexpr bool kOwnDs = D <= 64;
 
-  if (warp == 10) {
+  if (warp == 18) {
     // ------------------------------ producer ------------------------------
     if (elect_one()) {
       tma_prefetch_desc(&tm_q);
@@ -188,9 +194,9 @@ __global__ void __launch_bounds__(kBwThreads, 1)
       for (int j = max(0, J - L::NS); j < J; ++j) mbar_wait_drain(&kv_full[j % L::NS], (j / L::NS) & 1);
     }
     __syncwarp();
-  } else if (warp >= 8) {
+  } else if (warp >= 16) {
     // --------------------------- tensor-core issue ---------------------------
-    const int u = warp - 8;
+    const int u = warp - 16;
     const uint32_t tm_s = tmem + u * 128, tm_dp = tm_s + 64, tm_dq = tmem + 256 + u * D;
     const uint32_t tm_ds = kOwnDs ? tmem + 384 + 32 * u : tm_s;
     const uint32_t idesc_s = make_idesc(AB, 0, 0, 128, kDqKeys), idesc_q = make_idesc(AB, 0, 1, 128, D);
@@ -248,7 +254,7 @@ __global__ void __launch_bounds__(kBwThreads, 1)
         tc_fence_after();
         if (elect_one()) {
           const uint32_t k_base = smem_u32(sKV + st * L::KT);
-          mma_sum<D, kDqKeys>(tm_dq, tm_ds, k_base, idesc_q, t > a);
+          mma_sum<D, kDqKeys, kOwnDs ? 0 : 16>(tm_dq, tm_ds, k_base, idesc_q, t > a);
           umma_commit(&dq_done[u]);
           umma_commit(&kv_empty[st]);
         }
@@ -268,13 +274,15 @@ __global__ void __launch_bounds__(kBwThreads, 1)
     __syncwarp();
   } else {
     // ------------------------------ dS -------------------------------------
-    // A thread owns a row: p = exp2(s - lse), ds = p (dp - delta).
-    const int u = warp >> 2, quarter = warp & 3;
+    // p = exp2(s - lse), ds = p (dp - delta)
+    const int u = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const int t_row = row / G, g = row - t_row * G;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const uint32_t tm_s = tmem + u * 128 + lanes, tm_dp = tm_s + 64, tm_dq = tmem + 256 + u * D + lanes;
-    const uint32_t tm_ds = (kOwnDs ? tmem + 384 + 32 * u : tmem + u * 128) + lanes;
+    const uint32_t tm_s = tmem + u * 128 + 32 * half + lanes, tm_dp = tm_s + 64;
+    const uint32_t tm_dq = tmem + 256 + u * D + half * (D / 2) + lanes;
+    // over S: the halves' places do not touch what the other one may still read
+    const uint32_t tm_ds = (kOwnDs ? tmem + 384 + 32 * u + 16 * half : tmem + u * 128 + 32 * half) + lanes;
     const float sl2 = p.scale * 1.4426950408889634f;
     int n_it = 0, ns = 0;
     while (true) {
@@ -286,63 +294,63 @@ __global__ void __launch_bounds__(kBwThreads, 1)
       const int a = it.a[u], b = it.b[u];
       const bool live = t_row < it.n[u] && t_row < TT;
       const RowKeys keys = row_keys(p, it.pos + u * TT + t_row, it.lk);
+      const WarpKeys wk = warp_keys(keys, live);
       const long long orow = (long long)(it.tok + u * TT + t_row) * p.hq + it.hk * G + g;
       float lse2 = live ? p.lse[orow] * 1.4426950408889634f : 0.f;
       if (lse2 == -INFINITY) lse2 = 0.f;  // a row that sees nothing: every column is masked
       const float delta = live ? p.delta[orow] : 0.f;
       const float2 sc = make_float2(sl2, sl2), nl = make_float2(-lse2, -lse2), nd = make_float2(-delta, -delta);
       bool ok = true;
-      float s[32], d[32];
       for (int t = a; t < b; ++t) {
-        const int key = it.key<kDqKeys>(t);
-        const bool sinks_only = t < it.sep;
-        const int lo = sinks_only ? 0 : keys.lo - key, hi = sinks_only ? 0 : keys.hi - key;
-        const int sink = it.sep && !sinks_only ? 0 : keys.sink - key;
-        uint32_t bits[2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) bits[c] = live ? seen_bits(lo, hi, sink, 32 * c) : 0u;
+        // this thread's 32 columns: which of them the row sees
+        const int key = it.key<kDqKeys>(t) + 32 * half;
+        uint32_t bits = 0xffffffffu;
+        bool some = true, all = true;
+        if (key < wk.all_lo || key + 32 > wk.all_hi || t < it.sep) {
+          const bool sinks_only = t < it.sep;
+          bits = live ? seen_bits(sinks_only ? 0 : keys.lo - key, sinks_only ? 0 : keys.hi - key,
+                                  it.sep && !sinks_only ? 0 : keys.sink - key, 0)
+                      : 0u;
+          some = __any_sync(0xffffffffu, bits != 0u);
+          all = __all_sync(0xffffffffu, !live || bits == 0xffffffffu);
+        }
         if (!(ok = wait_phase(&s_full[u], ns & 1, abort_flag, p.err))) break;
         ++ns;
         tc_fence_after();
-        uint32_t w[2][16];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          if (__any_sync(0xffffffffu, bits[c] != 0u)) {
-            tmem_ld32(tm_s + 32 * c, s);
-            tmem_ld32(tm_dp + 32 * c, d);
-            tmem_wait_values<32>(s);
-            tmem_wait_values<32>(d);
-            const bool full = __all_sync(0xffffffffu, !live || bits[c] == 0xffffffffu);
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float2 e = fma2(make_float2(s[i], s[i + 1]), sc, nl);
-              e.x = ex2(e.x);
-              e.y = ex2(e.y);
-              e = mul2(e, add2(make_float2(d[i], d[i + 1]), nd));
-              s[i] = e.x;
-              s[i + 1] = e.y;
-            }
-            if (!full) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) s[i] = (bits[c] >> i & 1u) ? s[i] : 0.f;
-            }
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) w[c][i / 2] = pack2<BF16>(s[i], s[i + 1]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) w[c][i] = 0u;
+        uint32_t w[16];
+        if (some) {
+          float s[32], d[32];
+          tmem_ld32(tm_s, s);
+          tmem_ld32(tm_dp, d);
+          tmem_wait_values<32>(s);
+          tmem_wait_values<32>(d);
+          if (kOwnDs) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_free[u]);
           }
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float2 e = fma2(make_float2(s[i], s[i + 1]), sc, nl);
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            e = mul2(e, add2(make_float2(d[i], d[i + 1]), nd));
+            if (!all) {
+              e.x = (bits >> i & 1u) ? e.x : 0.f;
+              e.y = (bits >> i & 2u) ? e.y : 0.f;
+            }
+            w[i / 2] = pack2<BF16>(e.x, e.y);
+          }
+        } else {
+          if (kOwnDs && lane == 0) mbar_arrive(&s_free[u]);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = 0u;
         }
-        if (kOwnDs) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_free[u]);
-          // dS's columns are free once the product of the tile before is over
-          if (t > a && !(ok = wait_phase(&dq_done[u], (ns - 2) & 1, abort_flag, p.err))) break;
+        if (kOwnDs && t > a) {  // dS's columns are free once the product of the tile before is over
+          if (!(ok = wait_phase(&dq_done[u], (ns - 2) & 1, abort_flag, p.err))) break;
           tc_fence_after();
         }
-        tmem_st16(tm_ds, w[0]);
-        tmem_st16(tm_ds + 16, w[1]);
+        tmem_st16(tm_ds, w);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -353,15 +361,16 @@ __global__ void __launch_bounds__(kBwThreads, 1)
         if (!wait_phase(&dq_done[u], (ns - 1) & 1, abort_flag, p.err)) break;
         tc_fence_after();
       }
-      uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.dq) + orow * D);
+      uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.dq) + orow * D + half * (D / 2));
 #pragma unroll
-      for (int c = 0; c < D; c += 32) {
+      for (int c = 0; c < D / 2; c += 16) {
+        float s[16];
         if (b > a) {
-          tmem_ld32(tm_dq + c, s);
-          tmem_wait_values<32>(s);
+          tmem_ld16(tm_dq + c, s);
+          tmem_wait_values<16>(s);
         }
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) {
+        for (int i = 0; i < 16; i += 8) {
 #pragma unroll
           for (int j = i; j < i + 8; ++j) s[j] = b > a ? s[j] * p.scale : 0.f;
           if (live)
@@ -384,14 +393,14 @@ __global__ void __launch_bounds__(kBwThreads, 1)
 // A persistent CTA keeps 128 keys of a kv head and walks the queries that see
 // them, 64 packed rows at a time:
 //   S^T = K Q^T, dP^T = V dO^T (128 keys x 64 rows, two TMEM stages)
-//   warps 0-3 (even query tiles), 4-7 (odd ones): a key a thread, P^T and dS^T
-//   as 16-bit operands in TMEM;  dV += P^T dO, dK += dS^T Q
-//   warp 8 issues the first two products, warp 11 the sums (one warp for all
-//   four spends longer on issuing than they take), warp 9 loads, warp 10 gathers
+//   warps 0-7 (even query tiles), 8-15 (odd ones): two threads a key, 32 rows each;
+//   P^T and dS^T as 16-bit operands in TMEM;  dV += P^T dO, dK += dS^T Q
+//   warp 16 issues the first two products, warp 19 the sums (one warp for all
+//   four spends longer on issuing than they take), warp 17 loads, warp 18 gathers
 //   the rows' lse and delta.
 
 constexpr int kKvRows = 64;  // packed query rows of a tile
-constexpr int kKvThreads = 384;
+constexpr int kKvThreads = 640;
 
 struct KvItem {
   int stop;
@@ -518,10 +527,10 @@ __global__ void __launch_bounds__(kKvThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::NK; ++i) mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1);
     for (int i = 0; i < L::NS; ++i) mbar_init(&q_full[i], 1), mbar_init(&stat_full[i], 1), mbar_init(&q_empty[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&acc_done[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 8), mbar_init(&acc_done[i], 1);
     mbar_init(acc_full, 1);
-    mbar_init(acc_free, 8);
-    for (int i = 0; i < kItems; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 11);
+    mbar_init(acc_free, 16);
+    for (int i = 0; i < kItems; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 19);
     mbar_init(&mma_done[0], 1);
     mbar_init(&mma_done[1], 1);
     *abort_flag = 0;
@@ -539,7 +548,7 @@ __global__ void __launch_bounds__(kKvThreads, 1)
   // dS^T (32 each) of a stage in [384 + 64 st, +64) up to D = 64, else over its S^T and dP^T
   constexpr bool kOwnP = D <= 64;
 
-  if (warp == 9) {
+  if (warp == 17) {
     // ------------------------------ producer ------------------------------
     if (elect_one()) {
       tma_prefetch_desc(&tm_q);
@@ -590,7 +599,7 @@ __global__ void __launch_bounds__(kKvThreads, 1)
       for (int j = max(0, J - L::NS); j < J; ++j) mbar_wait_drain(&q_full[j % L::NS], (j / L::NS) & 1);
     }
     __syncwarp();
-  } else if (warp == 10) {
+  } else if (warp == 18) {
     // -------------------- lse and delta of the query rows --------------------
     int n_it = 0, J = 0;
     bool ok = true;
@@ -627,7 +636,7 @@ __global__ void __launch_bounds__(kKvThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[r]);
     }
-  } else if (warp == 8) {
+  } else if (warp == 16) {
     // --------------------- tensor-core issue: S^T and dP^T -------------------
     const uint32_t idesc = make_idesc(AB, 0, 0, 128, kKvRows);
     int n_it = 0, J = 0, nk = 0;  // items, query tiles, K tiles so far
@@ -678,7 +687,7 @@ __global__ void __launch_bounds__(kKvThreads, 1)
       mbar_wait_drain(&mma_done[0], 0);
     }
     __syncwarp();
-  } else if (warp == 11) {
+  } else if (warp == 19) {
     // ------------------------ tensor-core issue: dV and dK --------------------
     // (S^T's issue has seen the tile's Q and dO, and zeroed what is no query, before P^T can be announced)
     const uint32_t idesc = make_idesc(AB, 0, 1, 128, D);
@@ -703,8 +712,9 @@ __global__ void __launch_bounds__(kKvThreads, 1)
           const uint32_t q_base = smem_u32(sQ + 2 * st * L::QT), do_base = q_base + L::QT;
           const uint32_t tm_p = kOwnP ? tmem + 384 + 64 * stage : tmem + 128 * stage;
           const uint32_t tm_ds = kOwnP ? tm_p + 32 : tm_p + 64;
-          mma_sum<D, kKvRows>(tm_dv, tm_p, do_base, idesc, t > 0);
-          mma_sum<D, kKvRows>(tm_dk, tm_ds, q_base, idesc, t > 0);
+          constexpr int kGap = kOwnP ? 0 : 16;
+          mma_sum<D, kKvRows, kGap>(tm_dv, tm_p, do_base, idesc, t > 0);
+          mma_sum<D, kKvRows, kGap>(tm_dk, tm_ds, q_base, idesc, t > 0);
           umma_commit(&acc_done[stage]);
           umma_commit(&q_empty[st]);
           if (t == n - 1) umma_commit(acc_full);
@@ -723,11 +733,12 @@ __global__ void __launch_bounds__(kKvThreads, 1)
     __syncwarp();
   } else {
     // --------------------------- P^T and dS^T --------------------------------
-    const int wg = warp >> 2, quarter = warp & 3;
+    const int wg = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const uint32_t tm_s = tmem + wg * 128 + lanes, tm_dp = tm_s + 64;
-    const uint32_t tm_p = (kOwnP ? tmem + 384 + 64 * wg : tmem + 128 * wg) + lanes;
+    const uint32_t tm_s = tmem + wg * 128 + 32 * half + lanes, tm_dp = tm_s + 64;
+    // over S^T and dP^T: the halves' places do not touch what the other one may still read
+    const uint32_t tm_p = (kOwnP ? tmem + 384 + 64 * wg + 16 * half : tmem + 128 * wg + 32 * half) + lanes;
     const uint32_t tm_ds = kOwnP ? tm_p + 32 : tm_p + 64;
     const float sl2 = p.scale * 1.4426950408889634f;
     const float2 sc = make_float2(sl2, sl2);
@@ -755,33 +766,31 @@ __global__ void __launch_bounds__(kKvThreads, 1)
       bool ok = true;
       for (int t = (J & 1) ^ wg; t < n; t += 2) {
         const int jt = J + t, st = jt % L::NS;
-        const int c_lo = (lo - t * TT) * G, c_hi = (min(hi, (t + 1) * TT) - t * TT) * G;
-        uint32_t bits[2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) bits[c] = range_bits(c_lo - 32 * c, c_hi - 32 * c);
+        const uint32_t bits = range_bits((lo - t * TT) * G - 32 * half, (min(hi, (t + 1) * TT) - t * TT) * G - 32 * half);
+        const bool some = __any_sync(0xffffffffu, bits != 0u);
+        const bool full = __all_sync(0xffffffffu, !live || bits == 0xffffffffu);
         if (!(ok = wait_phase(&stat_full[st], (jt / L::NS) & 1, abort_flag, p.err))) break;
         if (!(ok = wait_phase(&s_full[wg], (jt >> 1) & 1, abort_flag, p.err))) break;
         tc_fence_after();
-        const float* nl = stat + (2 * st) * kKvRows;
+        const float* nl = stat + (2 * st) * kKvRows + 32 * half;
         const float* nd = nl + kKvRows;
         if (kOwnP && jt >= 2) {  // P^T's and dS^T's columns are free once the sums of the stage's last tile are over
           if (!(ok = wait_phase(&acc_done[wg], ((jt >> 1) & 1) ^ 1, abort_flag, p.err))) break;
           tc_fence_after();
         }
+        if (some) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t wp[16], wd[16];
-          if (__any_sync(0xffffffffu, bits[c] != 0u)) {
-            float s[32], d[32];
-            tmem_ld32(tm_s + 32 * c, s);
-            tmem_ld32(tm_dp + 32 * c, d);
-            tmem_wait_values<32>(s);
-            tmem_wait_values<32>(d);
-            const bool full = __all_sync(0xffffffffu, !live || bits[c] == 0xffffffffu);
+          for (int c = 0; c < 32; c += 16) {
+            float s[16], d[16];
+            uint32_t wp[8], wd[8];
+            tmem_ld16(tm_s + c, s);
+            tmem_ld16(tm_dp + c, d);
+            tmem_wait_values<16>(s);
+            tmem_wait_values<16>(d);
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float4 l4 = *reinterpret_cast<const float4*>(nl + 32 * c + i);
-              const float4 d4 = *reinterpret_cast<const float4*>(nd + 32 * c + i);
+            for (int i = 0; i < 16; i += 4) {
+              const float4 l4 = *reinterpret_cast<const float4*>(nl + c + i);
+              const float4 d4 = *reinterpret_cast<const float4*>(nd + c + i);
               float2 e0 = fma2(make_float2(s[i], s[i + 1]), sc, make_float2(l4.x, l4.y));
               float2 e1 = fma2(make_float2(s[i + 2], s[i + 3]), sc, make_float2(l4.z, l4.w));
               e0.x = ex2(e0.x);
@@ -791,7 +800,7 @@ __global__ void __launch_bounds__(kKvThreads, 1)
               float2 f0 = mul2(e0, add2(make_float2(d[i], d[i + 1]), make_float2(d4.x, d4.y)));
               float2 f1 = mul2(e1, add2(make_float2(d[i + 2], d[i + 3]), make_float2(d4.z, d4.w)));
               if (!full) {
-                const uint32_t b4 = bits[c] >> i;
+                const uint32_t b4 = bits >> (c + i);
                 e0.x = (b4 & 1u) ? e0.x : 0.f, f0.x = (b4 & 1u) ? f0.x : 0.f;
                 e0.y = (b4 & 2u) ? e0.y : 0.f, f0.y = (b4 & 2u) ? f0.y : 0.f;
                 e1.x = (b4 & 4u) ? e1.x : 0.f, f1.x = (b4 & 4u) ? f1.x : 0.f;
@@ -802,12 +811,13 @@ __global__ void __launch_bounds__(kKvThreads, 1)
               wd[i / 2] = pack2<BF16>(f0.x, f0.y);
               wd[i / 2 + 1] = pack2<BF16>(f1.x, f1.y);
             }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) wp[i] = wd[i] = 0u;
+            tmem_st8(tm_p + c / 2, wp);  // over S^T and dP^T, the columns are ones that have been read
+            tmem_st8(tm_ds + c / 2, wd);
           }
-          tmem_st16(tm_p + 16 * c, wp);  // over S^T and dP^T, the columns are ones that have been read
-          tmem_st16(tm_ds + 16 * c, wd);
+        } else {
+          const uint32_t z[16] = {};
+          tmem_st16(tm_p, z);
+          tmem_st16(tm_ds, z);
         }
         tmem_wait_st();
         tc_fence_before();
@@ -821,30 +831,31 @@ __global__ void __launch_bounds__(kKvThreads, 1)
         ++n_acc;
         tc_fence_after();
       }
-      // warps 0-3 write dV, warps 4-7 dK
+      // warps 0-7 write dV, warps 8-15 dK, a half of the channels each
       const bool to_part = it.part && j < p.sinks;
       const bool to_out = live && !it.sinks_only && !to_part;
       const float mul = wg ? p.scale : 1.f;
+      constexpr int DH = D / 2;
       uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(wg ? p.dk : p.dv) +
-                                            ((long long)(it.key + row) * p.hkv + it.hk) * D);
-      float4* part = to_part ? reinterpret_cast<float4*>(it.part + (long long)(j * 2 + wg) * D) : nullptr;
+                                            ((long long)(it.key + row) * p.hkv + it.hk) * D + half * DH);
+      float4* part = to_part ? reinterpret_cast<float4*>(it.part + (long long)(j * 2 + wg) * D + half * DH) : nullptr;
 #pragma unroll
-      for (int c = 0; c < D; c += 32) {
-        float s[32];
+      for (int c = 0; c < DH; c += 16) {
+        float s[16];
         if (n > 0) {
-          tmem_ld32(tmem + 256 + wg * D + c + lanes, s);
-          tmem_wait_values<32>(s);
+          tmem_ld16(tmem + 256 + wg * D + half * DH + c + lanes, s);
+          tmem_wait_values<16>(s);
         }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) s[i] = n > 0 ? s[i] * mul : 0.f;
+        for (int i = 0; i < 16; ++i) s[i] = n > 0 ? s[i] * mul : 0.f;
         if (to_out) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 8)
+          for (int i = 0; i < 16; i += 8)
             out[(c + i) / 8] = make_uint4(pack2<BF16>(s[i], s[i + 1]), pack2<BF16>(s[i + 2], s[i + 3]),
                                           pack2<BF16>(s[i + 4], s[i + 5]), pack2<BF16>(s[i + 6], s[i + 7]));
         } else if (to_part && live) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) part[(c + i) / 4] = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
+          for (int i = 0; i < 16; i += 4) part[(c + i) / 4] = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
         }
       }
       tc_fence_before();
