@@ -293,8 +293,7 @@ __global__ void __launch_bounds__(kBwThreads, 1)
       if (it.stop) break;
       const int a = it.a[u], b = it.b[u];
       const bool live = t_row < it.n[u] && t_row < TT;
-      const RowKeys keys = row_keys(p, it.pos + u * TT + t_row, it.lk);
-      const WarpKeys wk = warp_keys(keys, live);
+      const RowView<kDqKeys> view(p, it, it.pos + u * TT + t_row, live, 32 * half, 32);
       const long long orow = (long long)(it.tok + u * TT + t_row) * p.hq + it.hk * G + g;
       float lse2 = live ? p.lse[orow] * 1.4426950408889634f : 0.f;
       if (lse2 == -INFINITY) lse2 = 0.f;  // a row that sees nothing: every column is masked
@@ -303,14 +302,10 @@ __global__ void __launch_bounds__(kBwThreads, 1)
       bool ok = true;
       for (int t = a; t < b; ++t) {
         // this thread's 32 columns: which of them the row sees
-        const int key = it.key<kDqKeys>(t) + 32 * half;
-        uint32_t bits = 0xffffffffu;
+        uint32_t bits = 0u;
         bool some = true, all = true;
-        if (key < wk.all_lo || key + 32 > wk.all_hi || t < it.sep) {
-          const bool sinks_only = t < it.sep;
-          bits = live ? seen_bits(sinks_only ? 0 : keys.lo - key, sinks_only ? 0 : keys.hi - key,
-                                  it.sep && !sinks_only ? 0 : keys.sink - key, 0)
-                      : 0u;
+        if (!view.full(t)) {
+          bits = view.bits(t, 32 * half);
           some = __any_sync(0xffffffffu, bits != 0u);
           all = __all_sync(0xffffffffu, !live || bits == 0xffffffffu);
         }

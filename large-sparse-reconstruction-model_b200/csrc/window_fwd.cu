@@ -279,26 +279,19 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       if (it.stop) break;
       const int a = it.a[ui], b = it.b[ui];
       const bool live = t_row < it.n[ui] && t_row < TT;
-      const RowKeys keys = row_keys(p, it.pos + ui * TT + t_row, it.lk);
-      const WarpKeys wk = warp_keys(keys, live);
+      const RowView<kFwKeys> view(p, it, it.pos + ui * TT + t_row, live, 0, kFwKeys);
       float m = -INFINITY;
       float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       bool ok = true;
       float s[2][32];
       for (int t = a; t < b; ++t) {
-        // columns 32 c .. + 31: which of them this row sees; per warp, whether some and whether all rows see them.
-        // Between a window's edges all see all, which two comparisons tell (spelling the bits out took longer than
-        // the exponentials).
-        const int key = it.key<kFwKeys>(t);
-        uint32_t bits[2] = {0xffffffffu, 0xffffffffu};
+        // columns 32 c .. + 31: which of them this row sees; per warp, whether some and whether all rows see them
+        uint32_t bits[2];
         bool some[2] = {true, true}, all[2] = {true, true};
-        if (key < wk.all_lo || key + kFwKeys > wk.all_hi || t < it.sep) {
-          const bool sinks_only = t < it.sep;
-          const int lo = sinks_only ? 0 : keys.lo - key, hi = sinks_only ? 0 : keys.hi - key;
-          const int sink = it.sep && !sinks_only ? 0 : keys.sink - key;
+        if (!view.full(t)) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            bits[c] = live ? seen_bits(lo, hi, sink, 32 * c) : 0u;
+            bits[c] = view.bits(t, 32 * c);
             some[c] = __any_sync(0xffffffffu, bits[c] != 0u);
             all[c] = __all_sync(0xffffffffu, !live || bits[c] == 0xffffffffu);
           }

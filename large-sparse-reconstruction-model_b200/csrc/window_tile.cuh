@@ -174,16 +174,12 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int rows, int from) {
   __syncwarp();
 }
 
-// 32 visibility bits (columns c0 .. c0 + 31 of a key tile): columns [lo, hi)
-// and [0, sink).
+// Bits [lo, hi) of 32.
 __device__ __forceinline__ uint32_t range_bits(int lo, int hi) {
   lo = max(lo, 0);
   hi = min(hi, 32);
   if (hi <= lo) return 0u;
   return (0xffffffffu >> (32 - (hi - lo))) << lo;
-}
-__device__ __forceinline__ uint32_t seen_bits(int lo, int hi, int sink, int c0) {
-  return range_bits(lo - c0, hi - c0) | range_bits(-1, sink - c0);
 }
 
 // Two-lane fp32 arithmetic (one issue slot for two results).
@@ -253,21 +249,6 @@ __device__ __forceinline__ void tmem_wait_values(float* v) {
   tmem_wait_ld();
 #pragma unroll
   for (int i = 0; i < N; ++i) asm volatile("" : "+f"(v[i]));
-}
-
-// Where the rows of a warp stand to the window's keys: keys in [all_lo, all_hi)
-// are seen by every row, keys outside [any_lo, any_hi) by none (rows that are
-// not live do not count).
-struct WarpKeys {
-  int any_lo, any_hi, all_lo, all_hi;
-};
-__device__ __forceinline__ WarpKeys warp_keys(const RowKeys& r, bool live) {
-  WarpKeys w;
-  w.any_lo = __reduce_min_sync(0xffffffffu, live ? r.lo : 0x7fffffff);
-  w.any_hi = __reduce_max_sync(0xffffffffu, live ? r.hi : 0);
-  w.all_lo = __reduce_max_sync(0xffffffffu, live ? r.lo : 0);
-  w.all_hi = __reduce_min_sync(0xffffffffu, live ? r.hi : 0x7fffffff);
-  return w;
 }
 
 // ---------------------------------------------------------------------------
@@ -343,6 +324,38 @@ __device__ __forceinline__ bool row_item(const WindowParams& p, int w, int tt, R
   }
   return true;
 }
+
+// What one row of an item sees of its key tiles, and which of the tiles every
+// row of the warp sees whole (between a window's edges: two comparisons a tile;
+// spelling the masks out for each took longer than the exponentials).
+template <int KT>
+struct RowView {
+  int lo, hi, sink;  // columns of the window's first tile (`sink`: of the item's first tile)
+  int sep;
+  int full0, full1;  // tiles [full0, full1) need no mask
+  bool live;
+
+  __device__ __forceinline__ RowView(const WindowParams& p, const RowItem& it, int pos, bool is_live, int col0, int cols) {
+    const RowKeys k = row_keys(p, pos, it.lk);
+    live = is_live;
+    sep = it.sep;
+    lo = k.lo - it.w0;
+    hi = k.hi - it.w0;
+    sink = k.sink;
+    const int all_lo = __reduce_max_sync(0xffffffffu, live ? lo : 0) - col0;
+    const int all_hi = __reduce_min_sync(0xffffffffu, live ? hi : 0x3fffffff) - col0 - cols;
+    full0 = sep + (max(all_lo, 0) + KT - 1) / KT;
+    full1 = all_hi < 0 ? 0 : sep + all_hi / KT + 1;
+  }
+  __device__ __forceinline__ bool full(int t) const { return t >= full0 && t < full1; }
+  // Visibility of columns c0 .. c0 + 31 of tile t.
+  __device__ __forceinline__ uint32_t bits(int t, int c0) const {
+    if (!live) return 0u;
+    if (t < sep) return range_bits(-1, sink - KT * t - c0);
+    const int at = KT * (t - sep) + c0;
+    return range_bits(lo - at, hi - at) | (sep ? 0u : range_bits(-1, sink - at));
+  }
+};
 
 // This warp's 32 lanes x 8 TMEM columns from v[0..8) (see tmem_st16).
 __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
