@@ -54,24 +54,21 @@ __global__ void __launch_bounds__(256) window_delta_kernel(const uint4* __restri
 
 // ------------------------------- dQ ----------------------------------------
 // As the forward: a persistent CTA, two tiles of 128 packed query rows, key
-// tiles of 64 (S, dP and dQ of both row tiles fill TMEM at 128 channels).
-//   warps 0-7, 8-15  dS of row tile 0 and 1: two threads a row, 32 keys each.  What a
-//                    thread does between two waits is a chain of short latencies,
-//                    so a multiprocessor needs many of them (with one thread a row
-//                    the same code took 1.4 times as long).
-//   warps 16, 17     tensor-core issue for row tile 0 and 1
-//   warp 18          producer
+// tiles of 64 (S, dP and dQ of both row tiles fill TMEM at 128 channels).  One
+// thread a row: with two, the waits of a tile count twice (16384 tokens, 32 / 8 heads
+// of 128 channels: 904 us against 1037; 131072 tokens, 16 heads of 64: 928, 872).
 
-constexpr int kBwThreads = 608;
+constexpr int kBwThreads = 352;
 constexpr int kDqKeys = 64;
 
 template <int D>
 struct DqSmem {
   static constexpr int QT = TileShape<D>::bytes(128), KT = TileShape<D>::bytes(kDqKeys);
   static constexpr int NQ = D == 128 ? 1 : 2;  // Q and dO buffers of each row tile
-  static constexpr int NS = D == 128 ? 6 : 8;  // K / V ring
+  static constexpr int NS = D == 128 ? 5 : 8;  // K / V ring
   static constexpr int OFF_KV = 4 * NQ * QT;   // [row tile][buffer][Q, dO]
-  static constexpr int OFF_ITEM = OFF_KV + NS * KT;
+  static constexpr int OFF_ROWS = OFF_KV + NS * KT;
+  static constexpr int OFF_ITEM = OFF_ROWS + 8 * kRowBuf;
   static constexpr int OFF_BAR = OFF_ITEM + kItems * (int)sizeof(RowItem);
   // q_full[2][NQ], q_empty[2][NQ], kv_full[NS], kv_empty[NS], s_full[2], s_free[2], ds_full[2], dq_done[2],
   // item_full[], item_empty[], mma_done[2]
@@ -116,12 +113,12 @@ __global__ void __launch_bounds__(kBwThreads, 1)
     for (int i = 0; i < L::NS; ++i) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], 2);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&s_free[i], 8);
-      mbar_init(&ds_full[i], 8);
+      mbar_init(&s_free[i], 4);
+      mbar_init(&ds_full[i], 4);
       mbar_init(&dq_done[i], 1);
       mbar_init(&mma_done[i], 1);
     }
-    for (int i = 0; i < kItems; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 18);
+    for (int i = 0; i < kItems; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 10);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -137,7 +134,7 @@ __global__ void __launch_bounds__(kBwThreads, 1)
   // [384 + 32 u, +32) up to D = 64, else over S
   constexpr bool kOwnDs = D <= 64;
 
-  if (warp == 18) {
+  if (warp == 10) {
     // ------------------------------ producer ------------------------------
     if (elect_one()) {
       tma_prefetch_desc(&tm_q);
@@ -194,9 +191,9 @@ __global__ void __launch_bounds__(kBwThreads, 1)
       for (int j = max(0, J - L::NS); j < J; ++j) mbar_wait_drain(&kv_full[j % L::NS], (j / L::NS) & 1);
     }
     __syncwarp();
-  } else if (warp >= 16) {
+  } else if (warp >= 8) {
     // --------------------------- tensor-core issue ---------------------------
-    const int u = warp - 16;
+    const int u = warp - 8;
     const uint32_t tm_s = tmem + u * 128, tm_dp = tm_s + 64, tm_dq = tmem + 256 + u * D;
     const uint32_t tm_ds = kOwnDs ? tmem + 384 + 32 * u : tm_s;
     const uint32_t idesc_s = make_idesc(AB, 0, 0, 128, kDqKeys), idesc_q = make_idesc(AB, 0, 1, 128, D);
@@ -254,7 +251,7 @@ __global__ void __launch_bounds__(kBwThreads, 1)
         tc_fence_after();
         if (elect_one()) {
           const uint32_t k_base = smem_u32(sKV + st * L::KT);
-          mma_sum<D, kDqKeys, kOwnDs ? 0 : 16>(tm_dq, tm_ds, k_base, idesc_q, t > a);
+          mma_sum<D, kDqKeys>(tm_dq, tm_ds, k_base, idesc_q, t > a);
           umma_commit(&dq_done[u]);
           umma_commit(&kv_empty[st]);
         }
@@ -274,15 +271,13 @@ __global__ void __launch_bounds__(kBwThreads, 1)
     __syncwarp();
   } else {
     // ------------------------------ dS -------------------------------------
-    // p = exp2(s - lse), ds = p (dp - delta)
-    const int u = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
+    // A thread owns a row: p = exp2(s - lse), ds = p (dp - delta).
+    const int u = warp >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const int t_row = row / G, g = row - t_row * G;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const uint32_t tm_s = tmem + u * 128 + 32 * half + lanes, tm_dp = tm_s + 64;
-    const uint32_t tm_dq = tmem + 256 + u * D + half * (D / 2) + lanes;
-    // over S: the halves' places do not touch what the other one may still read
-    const uint32_t tm_ds = (kOwnDs ? tmem + 384 + 32 * u + 16 * half : tmem + u * 128 + 32 * half) + lanes;
+    const uint32_t tm_s = tmem + u * 128 + lanes, tm_dp = tm_s + 64, tm_dq = tmem + 256 + u * D + lanes;
+    const uint32_t tm_ds = (kOwnDs ? tmem + 384 + 32 * u : tmem + u * 128) + lanes;
     const float sl2 = p.scale * 1.4426950408889634f;
     int n_it = 0, ns = 0;
     while (true) {
@@ -293,59 +288,60 @@ __global__ void __launch_bounds__(kBwThreads, 1)
       if (it.stop) break;
       const int a = it.a[u], b = it.b[u];
       const bool live = t_row < it.n[u] && t_row < TT;
-      const RowView<kDqKeys> view(p, it, it.pos + u * TT + t_row, live, 32 * half, 32);
+      const RowView<kDqKeys> view(p, it, it.pos + u * TT + t_row, live, 0, kDqKeys);
       const long long orow = (long long)(it.tok + u * TT + t_row) * p.hq + it.hk * G + g;
       float lse2 = live ? p.lse[orow] * 1.4426950408889634f : 0.f;
       if (lse2 == -INFINITY) lse2 = 0.f;  // a row that sees nothing: every column is masked
       const float delta = live ? p.delta[orow] : 0.f;
       const float2 sc = make_float2(sl2, sl2), nl = make_float2(-lse2, -lse2), nd = make_float2(-delta, -delta);
       bool ok = true;
+      float s[32], d[32];
       for (int t = a; t < b; ++t) {
-        // this thread's 32 columns: which of them the row sees
-        uint32_t bits = 0u;
-        bool some = true, all = true;
-        if (!view.full(t)) {
-          bits = view.bits(t, 32 * half);
-          some = __any_sync(0xffffffffu, bits != 0u);
-          all = __all_sync(0xffffffffu, !live || bits == 0xffffffffu);
-        }
+        uint32_t bits[2] = {0xffffffffu, 0xffffffffu};
+        const bool all = view.full(t);
+        if (!all) bits[0] = view.bits(t, 0), bits[1] = view.bits(t, 32);
         if (!(ok = wait_phase(&s_full[u], ns & 1, abort_flag, p.err))) break;
         ++ns;
         tc_fence_after();
-        uint32_t w[16];
-        if (some) {
-          float s[32], d[32];
-          tmem_ld32(tm_s, s);
-          tmem_ld32(tm_dp, d);
-          tmem_wait_values<32>(s);
-          tmem_wait_values<32>(d);
-          if (kOwnDs) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s_free[u]);
-          }
+        uint32_t w[2][16];
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float2 e = fma2(make_float2(s[i], s[i + 1]), sc, nl);
-            e.x = ex2(e.x);
-            e.y = ex2(e.y);
-            e = mul2(e, add2(make_float2(d[i], d[i + 1]), nd));
-            if (!all) {
-              e.x = (bits >> i & 1u) ? e.x : 0.f;
-              e.y = (bits >> i & 2u) ? e.y : 0.f;
+        for (int c = 0; c < 2; ++c) {
+          if (all || __any_sync(0xffffffffu, bits[c] != 0u)) {
+            tmem_ld32(tm_s + 32 * c, s);
+            tmem_ld32(tm_dp + 32 * c, d);
+            tmem_wait_values<32>(s);
+            tmem_wait_values<32>(d);
+            const bool full = all || __all_sync(0xffffffffu, !live || bits[c] == 0xffffffffu);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              float2 e = fma2(make_float2(s[i], s[i + 1]), sc, nl);
+              e.x = ex2(e.x);
+              e.y = ex2(e.y);
+              e = mul2(e, add2(make_float2(d[i], d[i + 1]), nd));
+              s[i] = e.x;
+              s[i + 1] = e.y;
             }
-            w[i / 2] = pack2<BF16>(e.x, e.y);
-          }
-        } else {
-          if (kOwnDs && lane == 0) mbar_arrive(&s_free[u]);
+            if (!full) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) w[i] = 0u;
+              for (int i = 0; i < 32; ++i) s[i] = (bits[c] >> i & 1u) ? s[i] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) w[c][i / 2] = pack2<BF16>(s[i], s[i + 1]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[c][i] = 0u;
+          }
         }
-        if (kOwnDs && t > a) {  // dS's columns are free once the product of the tile before is over
-          if (!(ok = wait_phase(&dq_done[u], (ns - 2) & 1, abort_flag, p.err))) break;
+        if (kOwnDs) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[u]);
+          // dS's columns are free once the product of the tile before is over
+          if (t > a && !(ok = wait_phase(&dq_done[u], (ns - 2) & 1, abort_flag, p.err))) break;
           tc_fence_after();
         }
-        tmem_st16(tm_ds, w);
+        tmem_st16(tm_ds, w[0]);
+        tmem_st16(tm_ds + 16, w[1]);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -356,22 +352,18 @@ __global__ void __launch_bounds__(kBwThreads, 1)
         if (!wait_phase(&dq_done[u], (ns - 1) & 1, abort_flag, p.err)) break;
         tc_fence_after();
       }
-      uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.dq) + orow * D + half * (D / 2));
 #pragma unroll
-      for (int c = 0; c < D / 2; c += 16) {
-        float s[16];
+      for (int c = 0; c < D; c += 32) {
+        uint32_t w[16];
         if (b > a) {
-          tmem_ld16(tm_dq + c, s);
-          tmem_wait_values<16>(s);
+          tmem_ld32(tm_dq + c, s);
+          tmem_wait_values<32>(s);
         }
 #pragma unroll
-        for (int i = 0; i < 16; i += 8) {
-#pragma unroll
-          for (int j = i; j < i + 8; ++j) s[j] = b > a ? s[j] * p.scale : 0.f;
-          if (live)
-            out[(c + i) / 8] = make_uint4(pack2<BF16>(s[i], s[i + 1]), pack2<BF16>(s[i + 2], s[i + 3]),
-                                          pack2<BF16>(s[i + 4], s[i + 5]), pack2<BF16>(s[i + 6], s[i + 7]));
-        }
+        for (int i = 0; i < 32; i += 2)
+          w[i / 2] = b > a ? pack2<BF16>(s[i] * p.scale, s[i + 1] * p.scale) : 0u;
+        store_rows32(smem_u32(smem + L::OFF_ROWS + warp * kRowBuf), w, live ? orow : -1, static_cast<uint16_t*>(p.dq), D,
+                     c);
       }
       tc_fence_before();  // dQ is read before this warp's next dS lets the next item overwrite it
       __syncwarp();
@@ -410,9 +402,10 @@ template <int D>
 struct KvSmem {
   static constexpr int KT = TileShape<D>::bytes(128), QT = TileShape<D>::bytes(kKvRows);
   static constexpr int NK = D == 128 ? 1 : 2;  // K and V buffers
-  static constexpr int NS = 4;                 // ring of (Q, dO, lse, delta)
+  static constexpr int NS = D == 128 ? 3 : 4;  // ring of (Q, dO, lse, delta)
   static constexpr int OFF_Q = 2 * NK * KT;
-  static constexpr int OFF_STAT = OFF_Q + 2 * NS * QT;
+  static constexpr int OFF_ROWS = OFF_Q + 2 * NS * QT;
+  static constexpr int OFF_STAT = OFF_ROWS + (D >= 64 ? 16 * kRowBuf : 0);
   static constexpr int OFF_ITEM = OFF_STAT + NS * 2 * kKvRows * 4;
   static constexpr int OFF_BAR = OFF_ITEM + kItems * (int)sizeof(KvItem);
   // k_full[NK], k_empty[NK], q_full[NS], stat_full[NS], q_empty[NS], s_full[2], p_full[2], acc_done[2], acc_full,
@@ -596,7 +589,12 @@ __global__ void __launch_bounds__(kKvThreads, 1)
     __syncwarp();
   } else if (warp == 18) {
     // -------------------- lse and delta of the query rows --------------------
-    int n_it = 0, J = 0;
+    int tr[2], off[2], n_it = 0, J = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      tr[i] = (lane + 32 * i) / G;
+      off[i] = tr[i] * p.hq + lane + 32 * i - tr[i] * G;
+    }
     bool ok = true;
     while (ok) {
       const int r = n_it % kItems;
@@ -604,28 +602,33 @@ __global__ void __launch_bounds__(kKvThreads, 1)
       const KvItem& it = items[r];
       ++n_it;
       if (it.stop) break;
-      for (int t = 0; t * TT < it.ntok; ++t, ++J) {
-        float l[2], d[2];
+      const int ntok = it.ntok;
+      const long long base = (long long)it.tok * p.hq + it.hk * G;
+      float l[2], d[2];
+      auto fetch = [&](int t) {  // the next tile's are on their way while this one waits for its slot
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const int row = lane + 32 * i, tr = row / G, tok = t * TT + tr;
           l[i] = d[i] = 0.f;
-          if (tr < TT && tok < it.ntok) {
-            const long long idx = (long long)(it.tok + tok) * p.hq + it.hk * G + row - tr * G;
-            l[i] = p.lse[idx] * -1.4426950408889634f;
-            d[i] = -p.delta[idx];
-            if (l[i] == INFINITY) l[i] = 0.f;  // sees nothing: every key is masked
+          if (tr[i] < TT && t * TT + tr[i] < ntok) {
+            const long long at = base + (long long)t * TT * p.hq + off[i];
+            l[i] = p.lse[at];
+            d[i] = p.delta[at];
           }
         }
+      };
+      fetch(0);
+      for (int t = 0; t * TT < ntok; ++t, ++J) {
         const int st = J % L::NS;
         if (!(ok = wait_phase(&q_empty[st], ((J / L::NS) & 1) ^ 1, abort_flag, p.err))) break;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          stat[(2 * st) * kKvRows + lane + 32 * i] = l[i];
-          stat[(2 * st + 1) * kKvRows + lane + 32 * i] = d[i];
+          // a query that sees nothing (lse = -inf): every key is masked
+          stat[(2 * st) * kKvRows + lane + 32 * i] = l[i] == -INFINITY ? 0.f : l[i] * -1.4426950408889634f;
+          stat[(2 * st + 1) * kKvRows + lane + 32 * i] = -d[i];
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&stat_full[st]);
+        fetch(t + 1);
       }
       if (!ok) break;
       __syncwarp();
@@ -830,27 +833,33 @@ __global__ void __launch_bounds__(kKvThreads, 1)
       const bool to_part = it.part && j < p.sinks;
       const bool to_out = live && !it.sinks_only && !to_part;
       const float mul = wg ? p.scale : 1.f;
-      constexpr int DH = D / 2;
-      uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(wg ? p.dk : p.dv) +
-                                            ((long long)(it.key + row) * p.hkv + it.hk) * D + half * DH);
+      constexpr int DH = D / 2, CH = DH < 32 ? DH : 32;
+      uint16_t* out = static_cast<uint16_t*>(wg ? p.dk : p.dv);
+      const long long orow = (long long)(it.key + row) * p.hkv + it.hk;
       float4* part = to_part ? reinterpret_cast<float4*>(it.part + (long long)(j * 2 + wg) * D + half * DH) : nullptr;
 #pragma unroll
-      for (int c = 0; c < DH; c += 16) {
-        float s[16];
+      for (int c = 0; c < DH; c += CH) {
+        float s[CH];
+        uint32_t w[CH / 2];
         if (n > 0) {
-          tmem_ld16(tmem + 256 + wg * D + half * DH + c + lanes, s);
-          tmem_wait_values<16>(s);
+          tmem_load_cols<CH>(tmem + 256 + wg * D + half * DH + c + lanes, s);
+          tmem_wait_values<CH>(s);
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = n > 0 ? s[i] * mul : 0.f;
-        if (to_out) {
+        for (int i = 0; i < CH; ++i) s[i] = n > 0 ? s[i] * mul : 0.f;
 #pragma unroll
-          for (int i = 0; i < 16; i += 8)
-            out[(c + i) / 8] = make_uint4(pack2<BF16>(s[i], s[i + 1]), pack2<BF16>(s[i + 2], s[i + 3]),
-                                          pack2<BF16>(s[i + 4], s[i + 5]), pack2<BF16>(s[i + 6], s[i + 7]));
-        } else if (to_part && live) {
+        for (int i = 0; i < CH; i += 2) w[i / 2] = pack2<BF16>(s[i], s[i + 1]);
+        if constexpr (CH == 32) {
+          store_rows32(smem_u32(smem + L::OFF_ROWS + warp * kRowBuf), w, to_out ? orow : -1, out, D, half * DH + c);
+        } else if (to_out) {
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) part[(c + i) / 4] = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
+          for (int i = 0; i < CH; i += 8)
+            *reinterpret_cast<uint4*>(out + orow * D + half * DH + c + i) =
+                make_uint4(w[i / 2], w[i / 2 + 1], w[i / 2 + 2], w[i / 2 + 3]);
+        }
+        if (to_part && live) {
+#pragma unroll
+          for (int i = 0; i < CH; i += 4) part[(c + i) / 4] = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
         }
       }
       tc_fence_before();

@@ -36,9 +36,10 @@ struct FwSmem {
   static constexpr int NQ = D == 128 ? 1 : 2;  // Q buffers of each row tile
   static constexpr int RINGS = D == 128 ? 1 : 2;    // rings of work items and of K / V tiles
   static constexpr int ROWS = 2 / RINGS;            // row tiles of an item
-  static constexpr int NS = D == 128 ? 9 : 10;      // K / V tiles of a ring
+  static constexpr int NS = 9;                      // K / V tiles of a ring
   static constexpr int OFF_KV = 2 * NQ * QT;
-  static constexpr int OFF_ITEM = OFF_KV + RINGS * NS * KT;
+  static constexpr int OFF_ROWS = OFF_KV + RINGS * NS * KT;
+  static constexpr int OFF_ITEM = OFF_ROWS + 8 * kRowBuf;
   static constexpr int OFF_BAR = OFF_ITEM + RINGS * kItems * (int)sizeof(RowItem);
   // q_full[2][NQ], q_empty[2][NQ], kv_full[RINGS][NS], kv_empty[RINGS][NS], s_full[2][2], p_full[2][2],
   // pv_done[2][2], item_full[RINGS][], item_empty[RINGS][], mma_done[2]
@@ -368,22 +369,18 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       const float l = l2[0].x + l2[0].y + l2[1].x + l2[1].y;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const long long orow = (long long)(it.tok + ui * TT + t_row) * p.hq + it.hk * G + g;
-      uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + orow * D);
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         float* o = s[0];
+        uint32_t w[16];
         if (b > a) {
           tmem_ld32(tm_o + c, o);
           tmem_wait_values<32>(o);
         }
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-#pragma unroll
-          for (int j = i; j < i + 8; ++j) o[j] = l == 0.f ? 0.f : o[j] * inv;
-          if (live)
-            out[(c + i) / 8] = make_uint4(pack2<BF16>(o[i], o[i + 1]), pack2<BF16>(o[i + 2], o[i + 3]),
-                                          pack2<BF16>(o[i + 4], o[i + 5]), pack2<BF16>(o[i + 6], o[i + 7]));
-        }
+        for (int i = 0; i < 32; i += 2) w[i / 2] = l == 0.f ? 0u : pack2<BF16>(o[i] * inv, o[i + 1] * inv);
+        store_rows32(smem_u32(smem + L::OFF_ROWS + warp * kRowBuf), w, live ? orow : -1, static_cast<uint16_t*>(p.out),
+                     D, c);
       }
       if (live) p.lse[orow] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
       tc_fence_before();  // O is read before this warp's next P lets the next item overwrite it

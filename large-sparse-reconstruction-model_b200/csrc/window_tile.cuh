@@ -182,6 +182,32 @@ __device__ __forceinline__ uint32_t range_bits(int lo, int hi) {
   return (0xffffffffu >> (32 - (hi - lo))) << lo;
 }
 
+// Writes 32 channels of a warp's 32 rows (packed in w[16], a row a lane) to
+// out + row * ld + c, `row` negative: none.  Straight from the lanes each store
+// would touch 32 lines, which took longer than an item's last products; through
+// `buf` (2 KB of the warp's own) four lanes write a row's 64 bytes.
+constexpr int kRowBuf = 32 * 64;
+__device__ __forceinline__ void store_rows32(uint32_t buf, const uint32_t* w, long long row, uint16_t* out, int ld,
+                                             int c) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    st_shared_v4(buf + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4), w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2), ch = lane & 3;
+    uint32_t v[4];
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                 : "r"(buf + r * 64 + ((ch ^ ((r >> 1) & 3)) << 4))
+                 : "memory");
+    const long long at = __shfl_sync(0xffffffffu, row, r);
+    if (at >= 0) *reinterpret_cast<uint4*>(out + at * ld + c + ch * 8) = make_uint4(v[0], v[1], v[2], v[3]);
+  }
+  __syncwarp();
+}
+
 // Two-lane fp32 arithmetic (one issue slot for two results).
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 r;
