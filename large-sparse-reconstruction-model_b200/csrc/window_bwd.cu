@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(kBwThreads, 1)
     for (int w = blockIdx.x; ok; w += gridDim.x) {
       RowItem it;
       it.stop = w >= n_items;
-      if (!it.stop && !row_item<kDqKeys, 2>(p, w, TT, it)) continue;
+      if (!it.stop && !row_item<kDqKeys>(p, w, TT, it)) continue;
       const int r = n_it % kItems;
       if (!wait_phase(&item_empty[r], ((n_it / kItems) & 1) ^ 1, abort_flag, p.err)) break;
       if (lane == 0) {

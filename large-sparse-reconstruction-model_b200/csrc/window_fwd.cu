@@ -4,46 +4,52 @@
 //   o_i = sum_j exp(s_ij - lse_i) v_j      (no key: o = 0, lse = -inf)
 //
 // One pass over a query's keys with a running maximum and sum.  A persistent
-// CTA per multiprocessor has two tiles of 128 packed query rows under way:
+// CTA per multiprocessor walks work items (two tiles of 128 packed query rows
+// of one kv head and the keys that either sees):
 //   warps 0-3, 4-7  softmax of row tile 0 and 1, a row a thread: S from TMEM,
 //                   mask, running maximum, P = exp2(S - m) to TMEM as 16-bit
 //                   operand, at the end O / l to global memory
 //   warps 8, 9      tensor-core issue for row tile 0 and 1: S = Q K^T, O += P V
 //                   (P from TMEM)
-//   warps 10, 11    producers: work items, TMA of Q, K and V
-// S has two buffers of 64 columns a row tile and P lies over its S, so that the
-// products of the tiles before and after run under a tile's softmax (at 128 keys
-// a buffer TMEM holds one, and the two row tiles fell into step: both in their
-// softmax, then both waiting).  At 128 channels an item is two neighbouring row
-// tiles, and each K and V tile (64 keys) of its ring serves both, which halves
-// the L2 reads that would bound it.  Up to 64 channels each row tile is an item
-// of its own with its own ring and producer: sharing made the one ahead wait
-// for the other at every item's end.  Rounding: S, m, l and O are fp32; P is
-// rounded to the operand type (the sum l takes it unrounded), O once at the
+//   warp 10         producer: work items, TMA of Q, K and V
+// K and V tiles (64 keys) go through one ring and serve both row tiles, which
+// halves the L2 reads per product (a ring for each row tile: 131072 tokens, 16
+// heads of 64 channels, window 512, 766 us against 730).  S has two buffers of 64
+// columns a row tile and P lies over its S, so that the products of the tiles
+// before and after run under a tile's softmax.  Rounding: S, m, l and O are fp32;
+// P is rounded to the operand type (the sum l takes it unrounded), O once at the
 // end.
+//
+// What bounds it: 16384 tokens in two sequences, 32 / 8 heads of 128 channels,
+// causal window 2048: 545 us, 880 TFLOP/s (0.53 of the library's GEMM rate); the
+// tensor pipe is active 41 % of the time, the exponentials' pipe 40 %, and no
+// other unit more.  The softmax warps' chain of a tile (wait, TMEM read, maximum,
+// exponentials, TMEM write, arrive) takes 1.5 times the exponentials alone; the
+// two row tiles hide half of it.  Without the exponentials the time stays within
+// 3 % there, and falls by 15 % at 64 channels.  Tried without gain: tiles of 128
+// keys with a row's scores in registers (575 us), P in a place of its own (639),
+// two threads a row (999), the row tiles taking turns at the exponentials (633).
 #include "window_host.h"
 #include "window_tile.cuh"
 
 namespace lsrm {
 namespace {
 
-constexpr int kFwThreads = 384;
+constexpr int kFwThreads = 352;
 constexpr int kFwKeys = 64;
 
 template <int D>
 struct FwSmem {
   static constexpr int QT = TileShape<D>::bytes(128), KT = TileShape<D>::bytes(kFwKeys);
   static constexpr int NQ = D == 128 ? 1 : 2;  // Q buffers of each row tile
-  static constexpr int RINGS = D == 128 ? 1 : 2;    // rings of work items and of K / V tiles
-  static constexpr int ROWS = 2 / RINGS;            // row tiles of an item
-  static constexpr int NS = 9;                      // K / V tiles of a ring
+  static constexpr int NS = D == 128 ? 9 : 12;  // K / V ring
   static constexpr int OFF_KV = 2 * NQ * QT;
-  static constexpr int OFF_ROWS = OFF_KV + RINGS * NS * KT;
+  static constexpr int OFF_ROWS = OFF_KV + NS * KT;
   static constexpr int OFF_ITEM = OFF_ROWS + 8 * kRowBuf;
-  static constexpr int OFF_BAR = OFF_ITEM + RINGS * kItems * (int)sizeof(RowItem);
-  // q_full[2][NQ], q_empty[2][NQ], kv_full[RINGS][NS], kv_empty[RINGS][NS], s_full[2][2], p_full[2][2],
-  // pv_done[2][2], item_full[RINGS][], item_empty[RINGS][], mma_done[2]
-  static constexpr int NBAR = 4 * NQ + 2 * RINGS * NS + 12 + 2 * RINGS * kItems + 2;
+  static constexpr int OFF_BAR = OFF_ITEM + kItems * (int)sizeof(RowItem);
+  // q_full[2][NQ], q_empty[2][NQ], kv_full[NS], kv_empty[NS], s_full[2][2], p_full[2][2],
+  // pv_done[2][2], item_full[], item_empty[], mma_done[2]
+  static constexpr int NBAR = 4 * NQ + 2 * NS + 12 + 2 * kItems + 2;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int BYTES = OFF_MISC + 16 + 1024;
   static constexpr int ALLOC = BYTES > kOneCtaPerSmSmem ? BYTES : kOneCtaPerSmSmem;
@@ -64,14 +70,14 @@ __global__ void __launch_bounds__(kFwThreads, 1)
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* q_empty = q_full + 2 * L::NQ;
   uint64_t* kv_full = q_empty + 2 * L::NQ;
-  uint64_t* kv_empty = kv_full + L::RINGS * L::NS;
-  uint64_t* s_full = kv_empty + L::RINGS * L::NS;
+  uint64_t* kv_empty = kv_full + L::NS;
+  uint64_t* s_full = kv_empty + L::NS;
   // [row tile][buffer]: two tiles are under way, so each has its own phases
   uint64_t* p_full = s_full + 4;
   uint64_t* pv_done = p_full + 4;
   uint64_t* item_full = pv_done + 4;
-  uint64_t* item_empty = item_full + L::RINGS * kItems;
-  uint64_t* mma_done = item_empty + L::RINGS * kItems;
+  uint64_t* item_empty = item_full + kItems;
+  uint64_t* mma_done = item_empty + kItems;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
 
@@ -80,7 +86,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * L::NQ; ++i) mbar_init(&q_full[i], 1), mbar_init(&q_empty[i], 1);
-    for (int i = 0; i < L::RINGS * L::NS; ++i) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], L::ROWS);
+    for (int i = 0; i < L::NS; ++i) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], 2);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[2 * i], 1);
       mbar_init(&s_full[2 * i + 1], 1);
@@ -90,7 +96,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       mbar_init(&pv_done[2 * i + 1], 1);
       mbar_init(&mma_done[i], 1);
     }
-    for (int i = 0; i < L::RINGS * kItems; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 5 * L::ROWS);
+    for (int i = 0; i < kItems; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 10);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -104,17 +110,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
   const uint32_t tmem = *tmem_slot;
   // TMEM columns: S of row tile u, buffer i [128 u + 64 i, +64) with P over its first half; O [256 + u D, +D)
 
-  // this warp's row tile (of the CTA, and of its item) and ring
-  const int u = warp >= 10 ? warp - 10 : warp >= 8 ? warp - 8 : warp >> 2;
-  const int ring = L::RINGS == 1 ? 0 : u, ui = L::RINGS == 1 ? u : 0;
-  items += ring * kItems;
-  item_full += ring * kItems;
-  item_empty += ring * kItems;
-  sKV += ring * L::NS * L::KT;
-  kv_full += ring * L::NS;
-  kv_empty += ring * L::NS;
-
-  if (warp >= 10) {
+  if (warp == 10) {
     // ------------------------------ producer ------------------------------
     // The whole warp walks the items; one elected lane issues (under elect.sync
     // the compiler knows that one lane is active and issues TMA and tensor-core
@@ -126,13 +122,13 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       tma_prefetch_desc(&tm_v);
     }
     const uint32_t q_bytes = (uint32_t)(G * TT * D * 2);
-    int n_it = 0, J = 0, nq[L::ROWS] = {};
-    bool ok = u < L::RINGS;
-    for (int w = blockIdx.x * L::RINGS + ring; ok; w += gridDim.x * L::RINGS) {
+    int n_it = 0, J = 0, nq[2] = {0, 0};
+    bool ok = true;
+    for (int w = blockIdx.x; ok; w += gridDim.x) {
       RowItem it;
       it.stop = w >= n_items;
       if (!it.stop) {
-        if (!row_item<kFwKeys, L::ROWS>(p, w, TT, it)) continue;
+        if (!row_item<kFwKeys>(p, w, TT, it)) continue;
       }
       const int r = n_it % kItems;
       if (!wait_phase(&item_empty[r], ((n_it / kItems) & 1) ^ 1, abort_flag, p.err)) break;
@@ -144,9 +140,9 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       ++n_it;
       if (it.stop) break;
 #pragma unroll
-      for (int i = 0; i < L::ROWS; ++i) {
+      for (int i = 0; i < 2; ++i) {
         if (!ok || it.b[i] <= it.a[i]) continue;
-        const int st = (ring + i) * L::NQ + nq[i] % L::NQ;
+        const int st = i * L::NQ + nq[i] % L::NQ;
         if (!(ok = wait_phase(&q_empty[st], ((nq[i] / L::NQ) & 1) ^ 1, abort_flag, p.err))) continue;
         if (elect_one()) {
           mbar_arrive_expect_tx(&q_full[st], q_bytes);
@@ -171,14 +167,15 @@ __global__ void __launch_bounds__(kFwThreads, 1)
     }
     // after an abort: copies in flight land before the CTA exits
     if (lane == 0 && *abort_flag) {
-      for (int i = 0; i < L::ROWS; ++i)
+      for (int i = 0; i < 2; ++i)
         for (int k = max(0, nq[i] - L::NQ); k < nq[i]; ++k)
-          mbar_wait_drain(&q_full[(ring + i) * L::NQ + k % L::NQ], (k / L::NQ) & 1);
+          mbar_wait_drain(&q_full[i * L::NQ + k % L::NQ], (k / L::NQ) & 1);
       for (int j = max(0, J - L::NS); j < J; ++j) mbar_wait_drain(&kv_full[j % L::NS], (j / L::NS) & 1);
     }
     __syncwarp();
   } else if (warp >= 8) {
     // --------------------------- tensor-core issue ---------------------------
+    const int u = warp - 8;
     const uint32_t tm_s = tmem + u * 128, tm_o = tmem + 256 + u * D;
     const uint32_t idesc_o = make_idesc(AB, 0, 1, 128, D);
     int n_it = 0, J = 0, nq = 0;         // items, ring slots, Q tiles so far
@@ -191,7 +188,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       if (it.stop) break;
       const int st_q = u * L::NQ + nq % L::NQ;
       const uint32_t q_base = smem_u32(sQ + st_q * L::QT);
-      const int a = it.a[ui], b = it.b[ui];
+      const int a = it.a[u], b = it.b[u];
       // sinks of their own tile: only as many columns as they need
       auto cols_of = [&](int t) { return t < it.sep ? min(kFwKeys, (p.sinks - t * kFwKeys + 31) / 32 * 32) : kFwKeys; };
       auto wait_slot = [&](int j) { return wait_phase(&kv_full[j % L::NS], (j / L::NS) & 1, abort_flag, p.err); };
@@ -265,7 +262,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
     // one that all see is not masked, which leaves one masked chunk of a window's
     // slanted edge.
     constexpr float kLazy = 8.f;
-    const int quarter = warp & 3;
+    const int u = warp >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const int t_row = row / G, g = row - t_row * G;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
@@ -278,9 +275,9 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       const RowItem& it = items[r];
       ++n_it;
       if (it.stop) break;
-      const int a = it.a[ui], b = it.b[ui];
-      const bool live = t_row < it.n[ui] && t_row < TT;
-      const RowView<kFwKeys> view(p, it, it.pos + ui * TT + t_row, live, 0, kFwKeys);
+      const int a = it.a[u], b = it.b[u];
+      const bool live = t_row < it.n[u] && t_row < TT;
+      const RowView<kFwKeys> view(p, it, it.pos + u * TT + t_row, live, 0, kFwKeys);
       float m = -INFINITY;
       float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       bool ok = true;
@@ -368,7 +365,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       }
       const float l = l2[0].x + l2[0].y + l2[1].x + l2[1].y;
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      const long long orow = (long long)(it.tok + ui * TT + t_row) * p.hq + it.hk * G + g;
+      const long long orow = (long long)(it.tok + u * TT + t_row) * p.hq + it.hk * G + g;
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         float* o = s[0];
@@ -407,8 +404,8 @@ int launch_fwd(const WindowParams& p, cudaStream_t s) {
   const void* v = p.total_k ? p.v : p.q;
   if ((rc = make_tmap_3d(&mk, k, D, p.hkv, p.total_k, p.total_k ? p.k_stride : p.q_stride, 1, kFwKeys, S::kCols))) return rc;
   if ((rc = make_tmap_3d(&mv, v, D, p.hkv, p.total_k, p.total_k ? p.v_stride : p.q_stride, 1, kFwKeys, S::kCols))) return rc;
-  const int n_items = tile_slots(p.total_q, p.num_seqs, L::ROWS * tt) * p.hkv;
-  const int grid = std::min((n_items + L::RINGS - 1) / L::RINGS, num_sms());
+  const int n_items = tile_slots(p.total_q, p.num_seqs, 2 * tt) * p.hkv;
+  const int grid = std::min(n_items, num_sms());
   LSRM_CUDA_TRY(cudaFuncSetAttribute(window_fwd_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC));
   window_fwd_kernel<D, BF16><<<grid, kFwThreads, L::ALLOC, s>>>(mq, mk, mv, p, n_items);
   LSRM_LAUNCH_CHECK();

@@ -278,7 +278,7 @@ __device__ __forceinline__ void tmem_wait_values(float* v) {
 }
 
 // ---------------------------------------------------------------------------
-// Work items of the kernels that keep query rows (forward, dQ): one or two
+// Work items of the kernels that keep query rows (forward, dQ): two
 // tiles of TT tokens x G heads, one kv head, and the key tiles (KT keys) that
 // either sees.  The producer plans them; the other warps read them from a ring.
 // ---------------------------------------------------------------------------
@@ -305,18 +305,18 @@ struct RowItem {
   }
 };
 
-// Plans work item `w` of ROWS row tiles; false when it holds no query.
-template <int KT, int ROWS>
+// Plans work item `w`; false when it holds no query.
+template <int KT>
 __device__ __forceinline__ bool row_item(const WindowParams& p, int w, int tt, RowItem& it) {
   const int slot = w / p.hkv;
   it.hk = w - slot * p.hkv;
-  const int b = seq_of_slot(p.cu_q, p.num_seqs, ROWS * tt, slot);
+  const int b = seq_of_slot(p.cu_q, p.num_seqs, 2 * tt, slot);
   const Seq s = seq_of(p, b);
-  const int i0 = (slot - (p.cu_q[b] / (ROWS * tt) + b)) * ROWS * tt;
+  const int i0 = (slot - (p.cu_q[b] / (2 * tt) + b)) * 2 * tt;
   if (i0 < 0 || i0 >= s.lq) return false;
   it.tok = s.q0 + i0;
   it.n[0] = min(tt, s.lq - i0);
-  it.n[1] = ROWS > 1 ? max(0, min(tt, s.lq - i0 - tt)) : 0;
+  it.n[1] = max(0, min(tt, s.lq - i0 - tt));
   it.lk = b < p.num_seqs ? s.lk : 0;
   it.pos = i0 + s.lk - s.lq;
   it.key0 = s.k0;
