@@ -453,21 +453,23 @@ __global__ void __launch_bounds__(512) residual_norm_bwd_kernel(const NormParams
   }
 }
 
-// dw[c] = sum over the blocks' partial rows, in a fixed order: 8 segments of
-// the rows per column, then the segments in order.
+// dw[c] = sum over the blocks' partial rows, in a fixed order: 32 interleaved
+// runs of the rows per column, then the runs in order.
+constexpr int kDwRuns = 32;
 template <typename T>
-__global__ void __launch_bounds__(256) norm_dw_kernel(const float* __restrict__ part, int blocks, int cols, T* dw) {
-  __shared__ float s[8][32];
+__global__ void __launch_bounds__(32 * kDwRuns) norm_dw_kernel(const float* __restrict__ part, int blocks, int cols,
+                                                               T* dw) {
+  __shared__ float s[kDwRuns][33];
   const int c = blockIdx.x * 32 + threadIdx.x;
   float a = 0.f;
   if (c < cols) {
-#pragma unroll 8
-    for (int b = threadIdx.y; b < blocks; b += 8) a += part[(long long)b * cols + c];
+#pragma unroll 4
+    for (int b = threadIdx.y; b < blocks; b += kDwRuns) a += part[(long long)b * cols + c];
   }
   s[threadIdx.y][threadIdx.x] = a;
   __syncthreads();
   if (threadIdx.y == 0 && c < cols) {
-    for (int i = 1; i < 8; ++i) a += s[i][threadIdx.x];
+    for (int i = 1; i < kDwRuns; ++i) a += s[i][threadIdx.x];
     dw[c] = (T)a;
   }
 }
@@ -795,7 +797,7 @@ extern "C" int lsrm_residual_rms_norm_bwd(int64_t rows, int32_t cols, int32_t dt
   }
   if (!dweight) return LSRM_OK;
   ProfScope ps("residual_rms_norm_dw", s);
-  const dim3 grid((cols + 31) / 32), block(32, 8);
+  const dim3 grid((cols + 31) / 32), block(32, kDwRuns);
   if (weight_dtype == LSRM_DTYPE_F32)
     norm_dw_kernel<<<grid, block, 0, s>>>(p.dw_part, blocks, cols, static_cast<float*>(dweight));
   else if (dtype == LSRM_DTYPE_BF16)

@@ -10,3 +10,4 @@ from .api import (compressed_attention, dequantize_8bit, dropout, get_block_scor
                   sparse_window_attention, spatial_selection_attention, window_sink_attention, window_sink_decode)
 from .module import (SparseResBlock, SpatialSparseAttentionIn, SpatialSparseAttentionMid,
                      SpatialSparseAttentionOut)
+from .window_block import WindowBlock, WindowCache, WindowStack

@@ -239,11 +239,14 @@ class WindowSinkAttnFn(torch.autograd.Function):
         ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
         ctx.args = (window, sinks, causal, scale)
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
         return out, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _dlse):
+        if dout is None:
+            return (None,) * 9
         q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
         dq, dk, dv = ops.window_attn_bwd(q, k, v, out, lse, dout, cu_q, cu_k, *ctx.args)
         return dq, dk, dv, None, None, None, None, None, None

@@ -473,29 +473,33 @@ def _cuda(name: str, *ts):
 
 
 def _run(dev: torch.device, name: str, *args):
-    """Call the entry point ``name`` on the current stream of ``dev``."""
-    fn = getattr(_lib.lib(), name)
-    if dev.index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream().cuda_stream), name)
+    """Call the entry point ``name`` on the current stream of ``dev`` (its raw
+    handle: building a Stream object takes longer than the smallest kernels)."""
+    fn, i = getattr(_lib.lib(), name), dev.index
+    if i == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
     else:
         with torch.cuda.device(dev):
-            check(fn(*args, torch.cuda.current_stream().cuda_stream), name)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc:
+        check(rc, name)
 
 
 def _flat(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """Contiguous and 16-byte aligned (a copy for any other layout)."""
     if t is None:
         return None
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _token_rows(t: torch.Tensor):
-    """[..., heads, head_dim] with contiguous heads in aligned rows, as is or
-    copied, and the row stride (the stride of the dimension before the heads)."""
-    h, d = t.shape[-2:]
-    n, lead = t.shape[-3], t.stride(-3)
-    ok = (t.stride(-1) == 1 or d == 1) and (h == 1 or t.stride(-2) == d) and t.data_ptr() % 16 == 0
+    """[n, heads, head_dim] with contiguous heads in aligned rows, as is or
+    copied, and the row stride."""
+    n, h, d = t.shape
+    lead, per_head, unit = t.stride()
+    ok = unit == 1 and (h == 1 or per_head == d) and t.data_ptr() % 16 == 0
     if ok and n <= 1:
         return t, h * d
     if ok and lead >= h * d and lead % 8 == 0:
@@ -568,15 +572,19 @@ def window_decode(q, k_new, v_new, k_cache, v_cache, lengths, window: int, sinks
           f"{name}: shapes {tuple(q.shape)}, {tuple(k_new.shape)} and {tuple(k_cache.shape)} do not go together")
     _need(q.dtype == k_new.dtype == v_new.dtype == k_cache.dtype == v_cache.dtype, f"{name}: tensors must have one dtype")
     _need(lengths.dtype == torch.int32 and tuple(lengths.shape) == (b,), f"{name}: lengths must be int32 [batch]")
+    strides = []
     for c in (k_cache, v_cache):  # written in place: no copy may stand in
-        _need(c.stride(3) == 1 and (hkv == 1 or c.stride(2) == d) and c.stride(1) % 8 == 0 and c.stride(0) % 8 == 0
-              and c.stride(1) >= hkv * d and (b == 1 or c.stride(0) >= hkv * d) and c.data_ptr() % 16 == 0,
+        sb, sl, sh, sd = c.stride()
+        if b == 1:  # the stride of a single sequence says nothing
+            sb = sl
+        _need(sd == 1 and (hkv == 1 or sh == d) and sl % 8 == 0 and sb % 8 == 0 and sl >= hkv * d and sb >= hkv * d
+              and c.data_ptr() % 16 == 0,
               f"{name}: the caches need contiguous heads and strides of 8 elements, aligned to 16 bytes")
+        strides += [sb, sl]
     (q, qs), (k_new, ks), (v_new, vs) = _token_rows(q), _token_rows(k_new), _token_rows(v_new)
     lengths = lengths.contiguous()
     sh = _lib.WindowDecodeShape(b, q.shape[1], hkv, d, _dtype_code(q), k_cache.shape[1], min(int(window), 2**31 - 1),
-                                int(sinks), qs, ks, vs, k_cache.stride(0), k_cache.stride(1), v_cache.stride(0),
-                                v_cache.stride(1), float(softmax_scale) if softmax_scale else 0.0)
+                                int(sinks), qs, ks, vs, *strides, float(softmax_scale) if softmax_scale else 0.0)
     out = torch.empty(b, q.shape[1], d, dtype=q.dtype, device=dev)
     _run(dev, "lsrm_window_decode", ctypes.byref(sh), _addr(q), _addr(k_new), _addr(v_new), _addr(k_cache),
          _addr(v_cache), _addr(lengths), _addr(out))
