@@ -494,17 +494,19 @@ typedef struct lsrm_window_shape {
   float softmax_scale;  /* <= 0 selects 1/sqrt(D) */
 } lsrm_window_shape;
 
-/* out [total_q, Hq, D], lse [total_q, Hq] fp32 (natural log). */
+/* out [total_q, Hq, D], lse [total_q, Hq] fp32 (natural log).  out_rest (like
+ * out, or NULL) receives what out's rounding left over; the backward takes it
+ * so that rowsum(o * do) does not inherit that rounding. */
 int lsrm_window_attn_fwd(const lsrm_window_shape* shape, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
-                         const void* q, const void* k, const void* v, void* out, float* lse, int* err_flags,
-                         void* stream);
-/* dout, dq [total_q, Hq, D], dk, dv [total_k, Hkv, D], contiguous; sums are
- * taken in a fixed order. */
+                         const void* q, const void* k, const void* v, void* out, void* out_rest, float* lse,
+                         int* err_flags, void* stream);
+/* dout, dq [total_q, Hq, D], dk, dv [total_k, Hkv, D], contiguous; out_rest may
+ * be NULL; sums are taken in a fixed order. */
 size_t lsrm_window_attn_workspace_bytes(const lsrm_window_shape* shape);
 int lsrm_window_attn_bwd(const lsrm_window_shape* shape, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
-                         const void* q, const void* k, const void* v, const void* out, const float* lse,
-                         const void* dout, void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
-                         int* err_flags, void* stream);
+                         const void* q, const void* k, const void* v, const void* out, const void* out_rest,
+                         const float* lse, const void* dout, void* dq, void* dk, void* dv, void* workspace,
+                         size_t workspace_bytes, int* err_flags, void* stream);
 
 /* The causal form for one new token a sequence, over a ring cache [batch,
  * capacity, Hkv, D] (strides in elements, multiples of 8).  Sequence b holds

@@ -31,10 +31,13 @@ struct WindowBwdParams : WindowParams {
   float* part;         // [chunk_slots][hkv][sinks][2][D]
 };
 
-// delta = rowsum(o * do), D / 8 lanes a row.
+// delta = rowsum(o * do), D / 8 lanes a row.  o is the forward's output and what
+// its rounding left over (`rest`, may be null): from the rounded output alone
+// delta's error is half of ds's own rounding and shows in dq and dk.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) window_delta_kernel(const uint4* __restrict__ o, const uint4* __restrict__ d,
-                                                           float* __restrict__ delta, long long rows) {
+__global__ void __launch_bounds__(256) window_delta_kernel(const uint4* __restrict__ o, const uint4* __restrict__ rest,
+                                                           const uint4* __restrict__ d, float* __restrict__ delta,
+                                                           long long rows) {
   constexpr int GL = D / 8;
   const long long stride = (long long)gridDim.x * blockDim.x;
   const long long n = rows * GL, top = (n + 31) / 32 * 32;  // whole warps take part in the shuffles
@@ -45,6 +48,12 @@ __global__ void __launch_bounds__(256) window_delta_kernel(const uint4* __restri
       const T *x = reinterpret_cast<const T*>(&a), *y = reinterpret_cast<const T*>(&b);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s = fmaf((float)x[j], (float)y[j], s);
+      if (rest) {
+        const uint4 c = rest[i];
+        const T* z = reinterpret_cast<const T*>(&c);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = fmaf((float)z[j], (float)y[j], s);
+      }
     }
 #pragma unroll
     for (int k = GL / 2; k > 0; k >>= 1) s += __shfl_xor_sync(0xffffffffu, s, k);
@@ -938,8 +947,9 @@ int launch_bwd(const WindowBwdParams& p, cudaStream_t s) {
     ProfScope ps("window_attn_delta", s);
     const long long rows = (long long)p.total_q * p.hq;
     const int grid = (int)std::min<long long>((rows * (D / 8) + 255) / 256, (long long)num_sms() * 8);
-    window_delta_kernel<T, D><<<grid, 256, 0, s>>>(static_cast<const uint4*>(p.out), static_cast<const uint4*>(p.dout),
-                                                   p.delta, rows);
+    window_delta_kernel<T, D><<<grid, 256, 0, s>>>(static_cast<const uint4*>(p.out),
+                                                   static_cast<const uint4*>(p.out_rest),
+                                                   static_cast<const uint4*>(p.dout), p.delta, rows);
     LSRM_LAUNCH_CHECK();
   }
   // no query or no key at all: the maps are never read
@@ -1002,14 +1012,15 @@ extern "C" size_t lsrm_window_attn_workspace_bytes(const lsrm_window_shape* shap
 
 extern "C" int lsrm_window_attn_bwd(const lsrm_window_shape* shape, const int32_t* cu_seqlens_q,
                                     const int32_t* cu_seqlens_k, const void* q, const void* k, const void* v,
-                                    const void* out, const float* lse, const void* dout, void* dq, void* dk, void* dv,
-                                    void* workspace, size_t workspace_bytes, int* err_flags, void* stream) {
+                                    const void* out, const void* out_rest, const float* lse, const void* dout,
+                                    void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                                    int* err_flags, void* stream) {
   int rc = check_window(shape, cu_seqlens_q, cu_seqlens_k, q, k, v);
   if (rc) return rc;
   LSRM_CHECK_ARG((shape->total_q == 0 || (out && lse && dout && dq)) && (shape->total_k == 0 || (dk && dv)),
                  "out, lse, dout and the gradients must not be NULL");
-  LSRM_CHECK_ARG((((uintptr_t)out | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) == 0,
-                 "out, dout and the gradients must be 16-byte aligned");
+  LSRM_CHECK_ARG((((uintptr_t)out | (uintptr_t)out_rest | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk |
+                   (uintptr_t)dv) & 15) == 0, "out, out_rest, dout and the gradients must be 16-byte aligned");
   LSRM_CHECK_ARG(shape->num_seqs <= 65535, "at most 65535 sequences");
   if (!workspace || workspace_bytes < lsrm_window_attn_workspace_bytes(shape)) {
     set_error("workspace too small: %zu bytes, %zu needed", workspace_bytes, lsrm_window_attn_workspace_bytes(shape));
@@ -1020,7 +1031,7 @@ extern "C" int lsrm_window_attn_bwd(const lsrm_window_shape* shape, const int32_
   WindowBwdParams p;
   static_cast<WindowParams&>(p) = window_params(shape, cu_seqlens_q, cu_seqlens_k, q, k, v, const_cast<void*>(out),
                                                 const_cast<float*>(lse), err_flags);
-  p.dout = dout, p.dq = dq, p.dk = dk, p.dv = dv;
+  p.out_rest = const_cast<void*>(out_rest), p.dout = dout, p.dq = dq, p.dk = dk, p.dv = dv;
   const BwdLayout l = bwd_layout(p, shape->head_dim);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.delta = reinterpret_cast<float*>(ws + l.delta);

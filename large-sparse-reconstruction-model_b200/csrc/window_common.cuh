@@ -8,9 +8,23 @@
 
 #include <cstdint>
 
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
 #include "lsrm_sparse.h"
 
 namespace lsrm {
+
+// The two 16-bit values of a packed word.
+template <bool BF16>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  if constexpr (BF16) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+  } else {
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+  }
+}
+
 
 struct WindowParams {
   int num_seqs, total_q, total_k;
@@ -21,7 +35,7 @@ struct WindowParams {
   const int32_t *cu_q, *cu_k;
   long long q_stride, k_stride, v_stride;  // elements between tokens
   const void *q, *k, *v;
-  void* out;
+  void *out, *out_rest;  // out_rest: what out's rounding left over, may be null
   float* lse;            // [total_q, hq], natural log
   int* err;
 };

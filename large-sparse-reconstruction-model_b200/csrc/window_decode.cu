@@ -21,6 +21,7 @@
 
 #include "common.cuh"
 #include "host_util.h"
+#include "window_common.cuh"
 
 namespace lsrm {
 namespace {
@@ -81,15 +82,6 @@ __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, const uint
                  "{%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
-}
-
-template <bool BF16>
-__device__ __forceinline__ float2 unpack2(uint32_t v) {
-  if constexpr (BF16) {
-    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
-  } else {
-    return __half22float2(*reinterpret_cast<const __half2*>(&v));
-  }
 }
 
 // cp.async of 16 bytes, or of zeros where `live` is false.

@@ -376,8 +376,16 @@ __global__ void __launch_bounds__(kFwThreads, 1)
         }
 #pragma unroll
         for (int i = 0; i < 32; i += 2) w[i / 2] = l == 0.f ? 0u : pack2<BF16>(o[i] * inv, o[i + 1] * inv);
-        store_rows32(smem_u32(smem + L::OFF_ROWS + warp * kRowBuf), w, live ? orow : -1, static_cast<uint16_t*>(p.out),
-                     D, c);
+        const uint32_t buf = smem_u32(smem + L::OFF_ROWS + warp * kRowBuf);
+        store_rows32(buf, w, live ? orow : -1, static_cast<uint16_t*>(p.out), D, c);
+        if (p.out_rest) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float2 r = unpack2<BF16>(w[i / 2]);
+            w[i / 2] = l == 0.f ? 0u : pack2<BF16>(fmaf(o[i], inv, -r.x), fmaf(o[i + 1], inv, -r.y));
+          }
+          store_rows32(buf, w, live ? orow : -1, static_cast<uint16_t*>(p.out_rest), D, c);
+        }
       }
       if (live) p.lse[orow] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
       tc_fence_before();  // O is read before this warp's next P lets the next item overwrite it
@@ -419,13 +427,14 @@ using namespace lsrm;
 
 extern "C" int lsrm_window_attn_fwd(const lsrm_window_shape* shape, const int32_t* cu_seqlens_q,
                                     const int32_t* cu_seqlens_k, const void* q, const void* k, const void* v,
-                                    void* out, float* lse, int* err_flags, void* stream) {
+                                    void* out, void* out_rest, float* lse, int* err_flags, void* stream) {
   int rc = check_window(shape, cu_seqlens_q, cu_seqlens_k, q, k, v);
   if (rc) return rc;
   if (shape->total_q == 0) return LSRM_OK;
   LSRM_CHECK_ARG(out && lse, "out and lse must not be NULL");
-  LSRM_CHECK_ARG(((uintptr_t)out & 15) == 0, "out must be 16-byte aligned");
-  const WindowParams p = window_params(shape, cu_seqlens_q, cu_seqlens_k, q, k, v, out, lse, err_flags);
+  LSRM_CHECK_ARG((((uintptr_t)out | (uintptr_t)out_rest) & 15) == 0, "out and out_rest must be 16-byte aligned");
+  WindowParams p = window_params(shape, cu_seqlens_q, cu_seqlens_k, q, k, v, out, lse, err_flags);
+  p.out_rest = out_rest;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   ProfScope ps("window_attn_fwd", s);
 #define CALL(BF, D) return launch_fwd<D, BF>(p, s);

@@ -189,12 +189,13 @@ _SIGS = {
     ),
     "lsrm_qkv_norm_bwd": (c_int, [c_int64, c_int32, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p]),
     "lsrm_window_attn_fwd": (
-        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]
+        c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                c_void_p]
     ),
     "lsrm_window_attn_workspace_bytes": (c_size_t, [c_void_p]),
     "lsrm_window_attn_bwd": (
         c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]
+                c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]
     ),
     "lsrm_window_decode": (
         c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]

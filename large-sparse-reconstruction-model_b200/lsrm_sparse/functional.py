@@ -235,8 +235,8 @@ class WindowSinkAttnFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, cu_q, cu_k, window, sinks, causal, scale):
-        out, lse = ops.window_attn_fwd(q, k, v, cu_q, cu_k, window, sinks, causal, scale)
-        ctx.save_for_backward(q, k, v, out, lse, cu_q, cu_k)
+        out, lse, rest = ops.window_attn_fwd(q, k, v, cu_q, cu_k, window, sinks, causal, scale, need_rest=True)
+        ctx.save_for_backward(q, k, v, out, rest, lse, cu_q, cu_k)
         ctx.args = (window, sinks, causal, scale)
         ctx.mark_non_differentiable(lse)
         ctx.set_materialize_grads(False)
@@ -247,8 +247,8 @@ class WindowSinkAttnFn(torch.autograd.Function):
     def backward(ctx, dout, _dlse):
         if dout is None:
             return (None,) * 9
-        q, k, v, out, lse, cu_q, cu_k = ctx.saved_tensors
-        dq, dk, dv = ops.window_attn_bwd(q, k, v, out, lse, dout, cu_q, cu_k, *ctx.args)
+        q, k, v, out, rest, lse, cu_q, cu_k = ctx.saved_tensors
+        dq, dk, dv = ops.window_attn_bwd(q, k, v, out, rest, lse, dout, cu_q, cu_k, *ctx.args)
         return dq, dk, dv, None, None, None, None, None, None
 
 

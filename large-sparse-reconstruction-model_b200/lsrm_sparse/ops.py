@@ -532,19 +532,23 @@ def check_window_attn(q, k, v, cu_seqlens_q, cu_seqlens_k, window, sinks):
     _need(int(sinks) >= 0, f"{name}: sinks ({sinks}) must not be negative")
 
 
-def window_attn_fwd(q, k, v, cu_q, cu_k, window: int, sinks: int, causal: bool, softmax_scale=None):
-    """Returns (out [Nq, Hq, D], lse [Nq, Hq] fp32, natural log)."""
+def window_attn_fwd(q, k, v, cu_q, cu_k, window: int, sinks: int, causal: bool, softmax_scale=None,
+                    need_rest: bool = False):
+    """Returns (out [Nq, Hq, D], lse [Nq, Hq] fp32, natural log), and with
+    ``need_rest`` what out's rounding left over, for the backward."""
     sh, q, k, v = _window_shape(q, k, v, cu_q, window, sinks, causal, softmax_scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    rest = torch.empty_like(out) if need_rest else None
     lse = torch.empty(q.shape[0], q.shape[1], dtype=torch.float32, device=q.device)
     cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
     _run(q.device, "lsrm_window_attn_fwd", ctypes.byref(sh), _addr(cu_q), _addr(cu_k), _addr(q), _addr(k), _addr(v),
-         _addr(out), _addr(lse), _addr(_err_word(q.device)))
-    return out, lse
+         _addr(out), _addr(rest), _addr(lse), _addr(_err_word(q.device)))
+    return (out, lse, rest) if need_rest else (out, lse)
 
 
-def window_attn_bwd(q, k, v, out, lse, dout, cu_q, cu_k, window: int, sinks: int, causal: bool, softmax_scale=None):
-    """Returns (dq, dk, dv)."""
+def window_attn_bwd(q, k, v, out, rest, lse, dout, cu_q, cu_k, window: int, sinks: int, causal: bool,
+                    softmax_scale=None):
+    """Returns (dq, dk, dv); ``rest`` is the forward's, or None."""
     sh, q, k, v = _window_shape(q, k, v, cu_q, window, sinks, causal, softmax_scale)
     dout = _flat(dout)
     dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -553,7 +557,7 @@ def window_attn_bwd(q, k, v, out, lse, dout, cu_q, cu_k, window: int, sinks: int
     cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
     ws = _workspace(_lib.lib().lsrm_window_attn_workspace_bytes(ctypes.byref(sh)), q.device)
     _run(q.device, "lsrm_window_attn_bwd", ctypes.byref(sh), _addr(cu_q), _addr(cu_k), _addr(q), _addr(k), _addr(v),
-         _addr(out), _addr(lse), _addr(dout), _addr(dq), _addr(dk), _addr(dv), _addr(ws), ws.numel(),
+         _addr(out), _addr(rest), _addr(lse), _addr(dout), _addr(dq), _addr(dk), _addr(dv), _addr(ws), ws.numel(),
          _addr(_err_word(q.device)))
     return dq, dk, dv
 

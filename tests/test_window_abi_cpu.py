@@ -31,27 +31,27 @@ def test_window_attn_arguments(lib, change, text):  # noqa: F811
     h = lib.lib()
     sh = _shape(lib, **change)
     p = 1 << 20  # never dereferenced: the checks come first
-    assert h.lsrm_window_attn_fwd(ctypes.byref(sh), p, p, p, p, p, p, p, None, None) == INVALID
+    assert h.lsrm_window_attn_fwd(ctypes.byref(sh), p, p, p, p, p, p, p, p, None, None) == INVALID
     assert text in h.lsrm_last_error().decode()
-    assert h.lsrm_window_attn_bwd(ctypes.byref(sh), p, p, p, p, p, p, p, p, p, p, p, p, 1 << 30, None, None) == INVALID
+    assert h.lsrm_window_attn_bwd(ctypes.byref(sh), p, p, p, p, p, p, p, p, p, p, p, p, p, 1 << 30, None, None) == INVALID
 
 
 def test_window_attn_pointers_and_workspace(lib):  # noqa: F811
     h = lib.lib()
     sh, p = _shape(lib), 1 << 20
-    fwd = [ctypes.byref(sh), p, p, p, p, p, p, p, None, None]
-    for i in (1, 2, 3, 4, 5, 6, 7):
+    fwd = [ctypes.byref(sh), p, p, p, p, p, p, None, p, None, None]
+    for i in (1, 2, 3, 4, 5, 6, 8):
         assert h.lsrm_window_attn_fwd(*[None if j == i else a for j, a in enumerate(fwd)]) == INVALID
     assert h.lsrm_window_attn_fwd(*[p + 8 if j == 3 else a for j, a in enumerate(fwd)]) == INVALID
     need = h.lsrm_window_attn_workspace_bytes(ctypes.byref(sh))
     # delta of every row, the sinks' own sums, and one slot of partial sums more than the tokens fill
     row = 2 * 2 * 2 * 64 * 4
     assert need >= 64 * 4 * 4 + row + 2 * row
-    assert h.lsrm_window_attn_bwd(ctypes.byref(sh), p, p, p, p, p, p, p, p, p, p, p, p, need - 1, None,
+    assert h.lsrm_window_attn_bwd(ctypes.byref(sh), p, p, p, p, p, p, p, p, p, p, p, p, p, need - 1, None,
                                   None) == WORKSPACE
     assert h.lsrm_window_attn_fwd(None, *fwd[1:]) == INVALID
     empty = _shape(lib, total_q=0, total_k=0)
-    assert h.lsrm_window_attn_fwd(ctypes.byref(empty), p, p, None, None, None, None, None, None, None) == 0
+    assert h.lsrm_window_attn_fwd(ctypes.byref(empty), p, p, None, None, None, None, None, None, None, None) == 0
 
 
 @pytest.mark.parametrize("change,text", [
