@@ -25,7 +25,6 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
   }
 }
 
-
 struct WindowParams {
   int num_seqs, total_q, total_k;
   int hq, hkv, g;        // query heads, kv heads, query heads per kv head
@@ -58,28 +57,6 @@ __device__ __forceinline__ Seq seq_of(const WindowParams& p, int b) {
   return Seq{q0, q1 - q0, k0, k1 - k0};
 }
 
-// Keys that a query at `pos` sees: [lo, hi) and [0, sink) (sink <= lo, so the
-// two never overlap).
-struct Seen {
-  int sink, lo, hi;
-};
-
-__device__ __forceinline__ Seen keys_of(const WindowParams& p, int pos, int lk, bool live) {
-  Seen s;
-  s.lo = max(0, pos - p.left);
-  s.hi = min(lk, pos + p.right + 1);
-  s.sink = min(min(p.sinks, p.causal ? pos + 1 : lk), lk);
-  if (!live || s.hi < 0) s.hi = 0;
-  if (!live || s.sink < 0) s.sink = 0;
-  if (s.hi <= s.lo) s.lo = s.hi = max(s.sink, 0);
-  if (s.sink >= s.lo) {  // the window reaches into the sinks: one range
-    s.hi = max(s.hi, s.sink);
-    s.lo = 0;
-    s.sink = 0;
-  }
-  return s;
-}
-
 // Tiles of `rows` tokens of ragged sequences: sequence b's tiles start at slot
 // cu[b] / rows + b, which leaves each sequence at least as many slots as it
 // has tiles; total / rows + num_seqs + 1 slots cover all, the tail's included.
@@ -92,16 +69,6 @@ __device__ __forceinline__ int seq_of_slot(const int32_t* cu, int num_seqs, int 
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
     if (cu[mid] / rows + mid <= slot) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
-}
-
-__device__ __forceinline__ int seq_of_token(const int32_t* cu, int num_seqs, int token) {
-  int lo = 0, hi = num_seqs;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (cu[mid] <= token) lo = mid;
     else hi = mid - 1;
   }
   return lo;
