@@ -417,9 +417,9 @@ struct KvSmem {
   static constexpr int OFF_STAT = OFF_ROWS + (D >= 64 ? 16 * kRowBuf : 0);
   static constexpr int OFF_ITEM = OFF_STAT + NS * 2 * kKvRows * 4;
   static constexpr int OFF_BAR = OFF_ITEM + kItems * (int)sizeof(KvItem);
-  // k_full[NK], k_empty[NK], q_full[NS], stat_full[NS], q_empty[NS], s_full[2], p_full[2], acc_done[2], acc_full,
+  // k_full[NK], k_empty[NK], q_full[NS], q_empty[NS], s_full[2], p_full[2], acc_done[2], acc_full,
   // acc_free, item_full[], item_empty[], mma_done[2]
-  static constexpr int NBAR = 2 * NK + 3 * NS + 6 + 2 + 2 * kItems + 2;
+  static constexpr int NBAR = 2 * NK + 2 * NS + 6 + 2 + 2 * kItems + 2;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int BYTES = OFF_MISC + 16 + 1024;
   static constexpr int ALLOC = BYTES > kOneCtaPerSmSmem ? BYTES : kOneCtaPerSmSmem;
@@ -505,8 +505,7 @@ __global__ void __launch_bounds__(kKvThreads, 1)
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* k_empty = k_full + L::NK;
   uint64_t* q_full = k_empty + L::NK;
-  uint64_t* stat_full = q_full + L::NS;
-  uint64_t* q_empty = stat_full + L::NS;
+  uint64_t* q_empty = q_full + L::NS;
   uint64_t* s_full = q_empty + L::NS;
   uint64_t* p_full = s_full + 2;
   uint64_t* acc_done = p_full + 2;
@@ -523,7 +522,7 @@ __global__ void __launch_bounds__(kKvThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::NK; ++i) mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1);
-    for (int i = 0; i < L::NS; ++i) mbar_init(&q_full[i], 1), mbar_init(&stat_full[i], 1), mbar_init(&q_empty[i], 1);
+    for (int i = 0; i < L::NS; ++i) mbar_init(&q_full[i], 2), mbar_init(&q_empty[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 8), mbar_init(&acc_done[i], 1);
     mbar_init(acc_full, 1);
     mbar_init(acc_free, 16);
@@ -636,7 +635,7 @@ __global__ void __launch_bounds__(kKvThreads, 1)
           stat[(2 * st + 1) * kKvRows + lane + 32 * i] = -d[i];
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&stat_full[st]);
+        if (lane == 0) mbar_arrive(&q_full[st]);
         fetch(t + 1);
       }
       if (!ok) break;
@@ -749,13 +748,63 @@ __global__ void __launch_bounds__(kKvThreads, 1)
     const uint32_t tm_ds = kOwnP ? tm_p + 32 : tm_p + 64;
     const float sl2 = p.scale * 1.4426950408889634f;
     const float2 sc = make_float2(sl2, sl2);
+    const float mul = wg ? p.scale : 1.f;
+    uint16_t* out = static_cast<uint16_t*>(wg ? p.dk : p.dv);
+    constexpr int DH = D / 2, CH = DH < 32 ? DH : 32;
+    // An item's sums leave after the group's first tile of the next one: what they wait for runs under that tile.
+    bool due = false;
+    long long due_row = -1;   // row of dK / dV, or none
+    float* due_part = nullptr;  // place of a sink's sums, or none
     int n_it = 0, J = 0, n_acc = 0;
+    // warps 0-7 write dV, warps 8-15 dK, a half of the channels each
+    auto write_sums = [&](bool any) -> bool {
+      if (any) {
+        if (!wait_phase(acc_full, n_acc & 1, abort_flag, p.err)) return false;
+        ++n_acc;
+        tc_fence_after();
+      }
+#pragma unroll
+      for (int c = 0; c < DH; c += CH) {
+        float s[CH];
+        uint32_t w[CH / 2];
+        if (any) {
+          tmem_load_cols<CH>(tmem + 256 + wg * D + half * DH + c + lanes, s);
+          tmem_wait_values<CH>(s);
+          if (c + CH == DH) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_free);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < CH; ++i) s[i] = any ? s[i] * mul : 0.f;
+#pragma unroll
+        for (int i = 0; i < CH; i += 2) w[i / 2] = pack2<BF16>(s[i], s[i + 1]);
+        if constexpr (CH == 32) {
+          store_rows32(smem_u32(smem + L::OFF_ROWS + warp * kRowBuf), w, due_row, out, D, half * DH + c);
+        } else if (due_row >= 0) {
+#pragma unroll
+          for (int i = 0; i < CH; i += 8)
+            *reinterpret_cast<uint4*>(out + due_row * D + half * DH + c + i) =
+                make_uint4(w[i / 2], w[i / 2 + 1], w[i / 2 + 2], w[i / 2 + 3]);
+        }
+        if (due_part) {
+#pragma unroll
+          for (int i = 0; i < CH; i += 4)
+            *reinterpret_cast<float4*>(due_part + c + i) = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
+        }
+      }
+      return true;
+    };
     while (true) {
       const int r = n_it % kItems;
       if (!wait_phase(&item_full[r], (n_it / kItems) & 1, abort_flag, p.err)) break;
       const KvItem& it = items[r];
       ++n_it;
-      if (it.stop) break;
+      if (it.stop) {
+        if (due) write_sums(true);
+        break;
+      }
       const int n = (it.ntok + TT - 1) / TT;
       // queries that see this thread's key, as a token range of the item
       const int j = it.j0 + row;
@@ -770,13 +819,17 @@ __global__ void __launch_bounds__(kKvThreads, 1)
       hi = min(hi, it.ntok);
       const bool live = row < it.nk;
       if (!live) hi = lo;
+      const bool to_part = live && it.part && j < p.sinks;
+      const long long row_out = live && !it.sinks_only && !to_part ? (long long)(it.key + row) * p.hkv + it.hk : -1;
+      float* const part = to_part ? it.part + (long long)(j * 2 + wg) * D + half * DH : nullptr;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[r]);
       bool ok = true;
       for (int t = (J & 1) ^ wg; t < n; t += 2) {
         const int jt = J + t, st = jt % L::NS;
         const uint32_t bits = range_bits((lo - t * TT) * G - 32 * half, (min(hi, (t + 1) * TT) - t * TT) * G - 32 * half);
         const bool some = __any_sync(0xffffffffu, bits != 0u);
         const bool full = __all_sync(0xffffffffu, !live || bits == 0xffffffffu);
-        if (!(ok = wait_phase(&stat_full[st], (jt / L::NS) & 1, abort_flag, p.err))) break;
         if (!(ok = wait_phase(&s_full[wg], (jt >> 1) & 1, abort_flag, p.err))) break;
         tc_fence_after();
         const float* nl = stat + (2 * st) * kKvRows + 32 * half;
@@ -830,53 +883,21 @@ __global__ void __launch_bounds__(kKvThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[wg]);
+        if (due) {
+          due = false;
+          if (!(ok = write_sums(true))) break;
+        }
       }
       if (!ok) break;
       J += n;
-      if (n > 0) {
-        if (!wait_phase(acc_full, n_acc & 1, abort_flag, p.err)) break;
-        ++n_acc;
-        tc_fence_after();
+      if (due) {  // the group had no tile of this item
+        due = false;
+        if (!write_sums(true)) break;
       }
-      // warps 0-7 write dV, warps 8-15 dK, a half of the channels each
-      const bool to_part = it.part && j < p.sinks;
-      const bool to_out = live && !it.sinks_only && !to_part;
-      const float mul = wg ? p.scale : 1.f;
-      constexpr int DH = D / 2, CH = DH < 32 ? DH : 32;
-      uint16_t* out = static_cast<uint16_t*>(wg ? p.dk : p.dv);
-      const long long orow = (long long)(it.key + row) * p.hkv + it.hk;
-      float4* part = to_part ? reinterpret_cast<float4*>(it.part + (long long)(j * 2 + wg) * D + half * DH) : nullptr;
-#pragma unroll
-      for (int c = 0; c < DH; c += CH) {
-        float s[CH];
-        uint32_t w[CH / 2];
-        if (n > 0) {
-          tmem_load_cols<CH>(tmem + 256 + wg * D + half * DH + c + lanes, s);
-          tmem_wait_values<CH>(s);
-        }
-#pragma unroll
-        for (int i = 0; i < CH; ++i) s[i] = n > 0 ? s[i] * mul : 0.f;
-#pragma unroll
-        for (int i = 0; i < CH; i += 2) w[i / 2] = pack2<BF16>(s[i], s[i + 1]);
-        if constexpr (CH == 32) {
-          store_rows32(smem_u32(smem + L::OFF_ROWS + warp * kRowBuf), w, to_out ? orow : -1, out, D, half * DH + c);
-        } else if (to_out) {
-#pragma unroll
-          for (int i = 0; i < CH; i += 8)
-            *reinterpret_cast<uint4*>(out + orow * D + half * DH + c + i) =
-                make_uint4(w[i / 2], w[i / 2 + 1], w[i / 2 + 2], w[i / 2 + 3]);
-        }
-        if (to_part && live) {
-#pragma unroll
-          for (int i = 0; i < CH; i += 4) part[(c + i) / 4] = make_float4(s[i], s[i + 1], s[i + 2], s[i + 3]);
-        }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (n > 0) mbar_arrive(acc_free);
-        mbar_arrive(&item_empty[r]);
-      }
+      due_row = row_out;
+      due_part = part;
+      if (n > 0) due = true;
+      else write_sums(false);
     }
   }
   tc_fence_before();
