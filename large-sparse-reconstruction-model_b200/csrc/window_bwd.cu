@@ -388,12 +388,23 @@ __global__ void __launch_bounds__(kBwThreads, 1)
 // ----------------------------- dK and dV ------------------------------------
 // A persistent CTA keeps 128 keys of a kv head and walks the queries that see
 // them, 64 packed rows at a time:
-//   S^T = K Q^T, dP^T = V dO^T (128 keys x 64 rows, two TMEM stages)
+//   S^T = K Q^T, dP^T = V dO^T (128 keys x 64 rows; three TMEM stages up to 64 channels, two at 128)
 //   warps 0-7 (even query tiles), 8-15 (odd ones): two threads a key, 32 rows each;
-//   P^T and dS^T as 16-bit operands in TMEM;  dV += P^T dO, dK += dS^T Q
+//   P^T and dS^T as 16-bit operands in TMEM, over S^T and dP^T;  dV += P^T dO, dK += dS^T Q
 //   warp 16 issues the first two products, warp 19 the sums (one warp for all
 //   four spends longer on issuing than they take), warp 17 loads, warp 18 gathers
 //   the rows' lse and delta.
+//
+// What bounds it: a tile's chain (products, exponentials, sums), of which two or
+// three are in flight.  131072 tokens, 16 heads of 64 channels, symmetric window
+// 512: 1018 us; with two stages, whose P^T and dS^T have places of their own,
+// 1083 us.  16384 tokens, 32 / 8 heads of 128 channels, causal window 2048: 1005 us,
+// the tensor pipe's own time about 650.  The scores come from TMEM eight columns
+// at a time: with sixteen 1050 us there, with all 32 up front 1183 (the registers
+// then leave the exponentials no slack).  Four threads a key, all 16 warps on one
+// tile, gives 1008 us there and loses elsewhere (ragged sequences, 32 / 2 heads of
+// 32 channels: 320 us against 273).  An item's sums leave under the next one's first
+// tiles: 1244 us against 1125 before the other steps.
 
 constexpr int kKvRows = 64;  // packed query rows of a tile
 constexpr int kKvThreads = 640;
@@ -411,15 +422,16 @@ template <int D>
 struct KvSmem {
   static constexpr int KT = TileShape<D>::bytes(128), QT = TileShape<D>::bytes(kKvRows);
   static constexpr int NK = D == 128 ? 1 : 2;  // K and V buffers
-  static constexpr int NS = D == 128 ? 3 : 4;  // ring of (Q, dO, lse, delta)
+  static constexpr int NS = D == 128 ? 3 : 5;  // ring of (Q, dO, lse, delta)
+  static constexpr int NT = D == 128 ? 2 : 3;  // TMEM stages of S^T and dP^T
   static constexpr int OFF_Q = 2 * NK * KT;
   static constexpr int OFF_ROWS = OFF_Q + 2 * NS * QT;
   static constexpr int OFF_STAT = OFF_ROWS + (D >= 64 ? 16 * kRowBuf : 0);
   static constexpr int OFF_ITEM = OFF_STAT + NS * 2 * kKvRows * 4;
   static constexpr int OFF_BAR = OFF_ITEM + kItems * (int)sizeof(KvItem);
-  // k_full[NK], k_empty[NK], q_full[NS], q_empty[NS], s_full[2], p_full[2], acc_done[2], acc_full,
+  // k_full[NK], k_empty[NK], q_full[NS], q_empty[NS], s_full[NT], p_full[NT], acc_done[NT], acc_full,
   // acc_free, item_full[], item_empty[], mma_done[2]
-  static constexpr int NBAR = 2 * NK + 2 * NS + 6 + 2 + 2 * kItems + 2;
+  static constexpr int NBAR = 2 * NK + 2 * NS + 3 * NT + 2 + 2 * kItems + 2;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int BYTES = OFF_MISC + 16 + 1024;
   static constexpr int ALLOC = BYTES > kOneCtaPerSmSmem ? BYTES : kOneCtaPerSmSmem;
@@ -507,9 +519,9 @@ __global__ void __launch_bounds__(kKvThreads, 1)
   uint64_t* q_full = k_empty + L::NK;
   uint64_t* q_empty = q_full + L::NS;
   uint64_t* s_full = q_empty + L::NS;
-  uint64_t* p_full = s_full + 2;
-  uint64_t* acc_done = p_full + 2;
-  uint64_t* acc_full = acc_done + 2;
+  uint64_t* p_full = s_full + L::NT;
+  uint64_t* acc_done = p_full + L::NT;
+  uint64_t* acc_full = acc_done + L::NT;
   uint64_t* acc_free = acc_full + 1;
   uint64_t* item_full = acc_free + 1;
   uint64_t* item_empty = item_full + kItems;
@@ -523,7 +535,7 @@ __global__ void __launch_bounds__(kKvThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::NK; ++i) mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1);
     for (int i = 0; i < L::NS; ++i) mbar_init(&q_full[i], 2), mbar_init(&q_empty[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 8), mbar_init(&acc_done[i], 1);
+    for (int i = 0; i < L::NT; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 8), mbar_init(&acc_done[i], 1);
     mbar_init(acc_full, 1);
     mbar_init(acc_free, 16);
     for (int i = 0; i < kItems; ++i) mbar_init(&item_full[i], 1), mbar_init(&item_empty[i], 19);
@@ -540,9 +552,9 @@ __global__ void __launch_bounds__(kKvThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // TMEM columns: stage st: S^T [128 st, +64), dP^T [128 st + 64, +64); dV [256, +D), dK [256 + D, +D); P^T and
-  // dS^T (32 each) of a stage in [384 + 64 st, +64) up to D = 64, else over its S^T and dP^T
-  constexpr bool kOwnP = D <= 64;
+  // TMEM columns: stage st: S^T [128 st, +64), dP^T [128 st + 64, +64), P^T and dS^T over them; then dV, dK
+  constexpr int NT = L::NT;
+  const uint32_t tacc = tmem + NT * 128;
 
   if (warp == 17) {
     // ------------------------------ producer ------------------------------
@@ -660,7 +672,7 @@ __global__ void __launch_bounds__(kKvThreads, 1)
         if (!wait_phase(&k_full[sk], (nk / L::NK) & 1, abort_flag, p.err)) break;
         ++nk;
         for (int t = 0; t < n; ++t, ++J) {
-          const int st = J % L::NS, stage = J & 1;
+          const int st = J % L::NS, stage = J % NT;
           if (!(ok = wait_phase(&q_full[st], (J / L::NS) & 1, abort_flag, p.err))) break;
           // rows that hold no query of the sequence must not reach the sums, not even times zero
           const int rows = min(TT, ntok - t * TT) * G;
@@ -668,10 +680,8 @@ __global__ void __launch_bounds__(kKvThreads, 1)
             zero_rows<D>(sQ + 2 * st * L::QT, kKvRows, rows);
             zero_rows<D>(sQ + (2 * st + 1) * L::QT, kKvRows, rows);
           }
-          // the stage's last S^T and dP^T have been read; where P^T and dS^T lie over them, the sums that read those
-          // are over
-          if (J >= 2 && !(ok = wait_phase(kOwnP ? &p_full[stage] : &acc_done[stage], ((J >> 1) & 1) ^ 1, abort_flag, p.err)))
-            break;
+          // the sums that read the stage's last P^T and dS^T are over
+          if (J >= NT && !(ok = wait_phase(&acc_done[stage], ((J / NT) & 1) ^ 1, abort_flag, p.err))) break;
           tc_fence_after();
           if (elect_one()) {
             const uint32_t q_base = smem_u32(sQ + 2 * st * L::QT), do_base = q_base + L::QT;
@@ -697,7 +707,7 @@ __global__ void __launch_bounds__(kKvThreads, 1)
     // ------------------------ tensor-core issue: dV and dK --------------------
     // (S^T's issue has seen the tile's Q and dO, and zeroed what is no query, before P^T can be announced)
     const uint32_t idesc = make_idesc(AB, 0, 1, 128, D);
-    const uint32_t tm_dv = tmem + 256, tm_dk = tmem + 256 + D;
+    const uint32_t tm_dv = tacc, tm_dk = tacc + D;
     int n_it = 0, J = 0, n_acc = 0;  // items, query tiles, items with sums so far
     while (true) {
       const int r = n_it % kItems;
@@ -708,19 +718,17 @@ __global__ void __launch_bounds__(kKvThreads, 1)
       const int n = (it.ntok + TT - 1) / TT;
       bool ok = true;
       for (int t = 0; t < n; ++t, ++J) {
-        const int st = J % L::NS, stage = J & 1;
+        const int st = J % L::NS, stage = J % NT;
         // the last item's sums have been read
         if (t == 0 && n_acc > 0 && !(ok = wait_phase(acc_free, (n_acc - 1) & 1, abort_flag, p.err))) break;
         if (!(ok = wait_phase(&q_full[st], (J / L::NS) & 1, abort_flag, p.err))) break;
-        if (!(ok = wait_phase(&p_full[stage], (J >> 1) & 1, abort_flag, p.err))) break;
+        if (!(ok = wait_phase(&p_full[stage], (J / NT) & 1, abort_flag, p.err))) break;
         tc_fence_after();
         if (elect_one()) {
           const uint32_t q_base = smem_u32(sQ + 2 * st * L::QT), do_base = q_base + L::QT;
-          const uint32_t tm_p = kOwnP ? tmem + 384 + 64 * stage : tmem + 128 * stage;
-          const uint32_t tm_ds = kOwnP ? tm_p + 32 : tm_p + 64;
-          constexpr int kGap = kOwnP ? 0 : 16;
-          mma_sum<D, kKvRows, kGap>(tm_dv, tm_p, do_base, idesc, t > 0);
-          mma_sum<D, kKvRows, kGap>(tm_dk, tm_ds, q_base, idesc, t > 0);
+          const uint32_t tm_p = tmem + 128 * stage;
+          mma_sum<D, kKvRows, 16>(tm_dv, tm_p, do_base, idesc, t > 0);
+          mma_sum<D, kKvRows, 16>(tm_dk, tm_p + 64, q_base, idesc, t > 0);
           umma_commit(&acc_done[stage]);
           umma_commit(&q_empty[st]);
           if (t == n - 1) umma_commit(acc_full);
@@ -742,10 +750,6 @@ __global__ void __launch_bounds__(kKvThreads, 1)
     const int wg = warp >> 3, half = (warp >> 2) & 1, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const uint32_t tm_s = tmem + wg * 128 + 32 * half + lanes, tm_dp = tm_s + 64;
-    // over S^T and dP^T: the halves' places do not touch what the other one may still read
-    const uint32_t tm_p = (kOwnP ? tmem + 384 + 64 * wg + 16 * half : tmem + 128 * wg + 32 * half) + lanes;
-    const uint32_t tm_ds = kOwnP ? tm_p + 32 : tm_p + 64;
     const float sl2 = p.scale * 1.4426950408889634f;
     const float2 sc = make_float2(sl2, sl2);
     const float mul = wg ? p.scale : 1.f;
@@ -768,7 +772,7 @@ __global__ void __launch_bounds__(kKvThreads, 1)
         float s[CH];
         uint32_t w[CH / 2];
         if (any) {
-          tmem_load_cols<CH>(tmem + 256 + wg * D + half * DH + c + lanes, s);
+          tmem_load_cols<CH>(tacc + wg * D + half * DH + c + lanes, s);
           tmem_wait_values<CH>(s);
           if (c + CH == DH) {
             tc_fence_before();
@@ -826,37 +830,39 @@ __global__ void __launch_bounds__(kKvThreads, 1)
       if (lane == 0) mbar_arrive(&item_empty[r]);
       bool ok = true;
       for (int t = (J & 1) ^ wg; t < n; t += 2) {
-        const int jt = J + t, st = jt % L::NS;
+        const int jt = J + t, st = jt % L::NS, sg = jt % NT;
+        // P^T and dS^T go over S^T and dP^T: the halves' places do not touch what the other one may still read
+        const uint32_t tm_s = tmem + sg * 128 + 32 * half + lanes, tm_dp = tm_s + 64;
         const uint32_t bits = range_bits((lo - t * TT) * G - 32 * half, (min(hi, (t + 1) * TT) - t * TT) * G - 32 * half);
         const bool some = __any_sync(0xffffffffu, bits != 0u);
         const bool full = __all_sync(0xffffffffu, !live || bits == 0xffffffffu);
-        if (!(ok = wait_phase(&s_full[wg], (jt >> 1) & 1, abort_flag, p.err))) break;
+        if (!(ok = wait_phase(&s_full[sg], (jt / NT) & 1, abort_flag, p.err))) break;
         tc_fence_after();
         const float* nl = stat + (2 * st) * kKvRows + 32 * half;
         const float* nd = nl + kKvRows;
-        if (kOwnP && jt >= 2) {  // P^T's and dS^T's columns are free once the sums of the stage's last tile are over
-          if (!(ok = wait_phase(&acc_done[wg], ((jt >> 1) & 1) ^ 1, abort_flag, p.err))) break;
-          tc_fence_after();
-        }
         if (some) {
 #pragma unroll
-          for (int c = 0; c < 32; c += 16) {
-            float s[16], d[16];
-            uint32_t wp[8], wd[8];
-            tmem_ld16(tm_s + c, s);
-            tmem_ld16(tm_dp + c, d);
-            tmem_wait_values<16>(s);
-            tmem_wait_values<16>(d);
+          for (int c = 0; c < 32; c += 8) {
+            float s[8], d[8];
+            uint32_t wp[4], wd[4];
+            tmem_ld8(tm_s + c, s);
+            tmem_wait_values<8>(s);
+            tmem_ld8(tm_dp + c, d);
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
+            for (int i = 0; i < 8; i += 4) {
               const float4 l4 = *reinterpret_cast<const float4*>(nl + c + i);
-              const float4 d4 = *reinterpret_cast<const float4*>(nd + c + i);
               float2 e0 = fma2(make_float2(s[i], s[i + 1]), sc, make_float2(l4.x, l4.y));
               float2 e1 = fma2(make_float2(s[i + 2], s[i + 3]), sc, make_float2(l4.z, l4.w));
-              e0.x = ex2(e0.x);
-              e0.y = ex2(e0.y);
-              e1.x = ex2(e1.x);
-              e1.y = ex2(e1.y);
+              s[i] = ex2(e0.x);
+              s[i + 1] = ex2(e0.y);
+              s[i + 2] = ex2(e1.x);
+              s[i + 3] = ex2(e1.y);
+            }
+            tmem_wait_values<8>(d);
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+              const float4 d4 = *reinterpret_cast<const float4*>(nd + c + i);
+              float2 e0 = make_float2(s[i], s[i + 1]), e1 = make_float2(s[i + 2], s[i + 3]);
               float2 f0 = mul2(e0, add2(make_float2(d[i], d[i + 1]), make_float2(d4.x, d4.y)));
               float2 f1 = mul2(e1, add2(make_float2(d[i + 2], d[i + 3]), make_float2(d4.z, d4.w)));
               if (!full) {
@@ -871,18 +877,18 @@ __global__ void __launch_bounds__(kKvThreads, 1)
               wd[i / 2] = pack2<BF16>(f0.x, f0.y);
               wd[i / 2 + 1] = pack2<BF16>(f1.x, f1.y);
             }
-            tmem_st8(tm_p + c / 2, wp);  // over S^T and dP^T, the columns are ones that have been read
-            tmem_st8(tm_ds + c / 2, wd);
+            tmem_st4(tm_s + c / 2, wp);  // over S^T and dP^T, the columns are ones that have been read
+            tmem_st4(tm_dp + c / 2, wd);
           }
         } else {
           const uint32_t z[16] = {};
-          tmem_st16(tm_p, z);
-          tmem_st16(tm_ds, z);
+          tmem_st16(tm_s, z);
+          tmem_st16(tm_dp, z);
         }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[wg]);
+        if (lane == 0) mbar_arrive(&p_full[sg]);
         if (due) {
           due = false;
           if (!(ok = write_sums(true))) break;

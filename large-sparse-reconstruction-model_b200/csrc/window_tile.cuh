@@ -118,37 +118,6 @@ __device__ __forceinline__ void mma_sum(uint32_t d, uint32_t a_tmem, uint32_t b_
       mma_ts<(int)desc_hi<D>()>(d, a_tmem + ks * 8 + (ks / 2) * GAP, b + step_mn<D>(ks), idesc, acc || ks > 0);
 }
 
-// The same with A in shared memory: [128][ROWS] 16-bit values in sub-tiles of 64
-// (128-byte rows, 128-byte swizzle), as store_row writes them.
-template <int D, int ROWS>
-__device__ __forceinline__ void mma_sum_smem(uint32_t d, uint32_t a_base, uint32_t b_base, uint32_t idesc, bool acc,
-                                             int steps = ROWS / 16) {
-  static_assert(D == 128 && ROWS % 64 == 0, "both operands have 128-byte rows");
-  const uint32_t a = desc_k<ROWS>(a_base), b = desc_mn<D, ROWS>(b_base);
-#pragma unroll
-  for (int ks = 0; ks < ROWS / 16; ++ks)
-    if (ks < steps)
-      mma_ss<(int)desc_hi<D>()>(d, a + step_k<ROWS, 128>(ks), b + step_mn<D>(ks), idesc, acc || ks > 0);
-}
-// Columns [32 c, 32 c + 32) of row `row` of such an operand, packed in w[16].
-__device__ __forceinline__ void store_row(uint32_t base, int row, int c, const uint32_t* w) {
-  const uint32_t sub = base + (c >> 1) * 128 * 128;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    st_shared_v4(sub + swz_offset<128>(row, (c & 1) * 4 + i), w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-}
-
-// Hands registers from the warpgroups that need few to those that hold rows of
-// scores: the shares of a block's warpgroups add up to what it was launched with.
-template <int N>
-__device__ __forceinline__ void registers_up() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void registers_down() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
-}
-
 // TMA of one operand tile: rows of `heads` heads x tokens from (head, token).
 template <int D>
 __device__ __forceinline__ void load_tile(uint8_t* dst, int rows, const CUtensorMap* map, int head, int token,
@@ -383,10 +352,10 @@ struct RowView {
   }
 };
 
-// This warp's 32 lanes x 8 TMEM columns from v[0..8) (see tmem_st16).
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
-               "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+// This warp's 32 lanes x 4 TMEM columns from v[0..4) (see tmem_st16).
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3])
                : "memory");
 }
 
