@@ -65,7 +65,14 @@ __global__ void __launch_bounds__(256) window_delta_kernel(const uint4* __restri
 // As the forward: a persistent CTA, two tiles of 128 packed query rows, key
 // tiles of 64 (S, dP and dQ of both row tiles fill TMEM at 128 channels).  One
 // thread a row: with two, the waits of a tile count twice (16384 tokens, 32 / 8 heads
-// of 128 channels: 904 us against 1037; 131072 tokens, 16 heads of 64: 928, 872).
+// of 128 channels: 904 us against 1037 in the first form).
+//
+// What bounds it: a row tile's chain of a key tile, of which the two row tiles
+// hide each other's.  S and dP have barriers of their own: the next S is formed
+// under the exponentials, and dS lies over dP, whose next product follows dQ's
+// under the next exponentials: 685 us there, 1.0 PFLOP/s, against 913 with both
+// waiting for dS; 131072 tokens, 16 heads of 64 channels, symmetric window 512:
+// 880 us against 922.
 
 constexpr int kBwThreads = 352;
 constexpr int kDqKeys = 64;
@@ -79,9 +86,9 @@ struct DqSmem {
   static constexpr int OFF_ROWS = OFF_KV + NS * KT;
   static constexpr int OFF_ITEM = OFF_ROWS + 8 * kRowBuf;
   static constexpr int OFF_BAR = OFF_ITEM + kItems * (int)sizeof(RowItem);
-  // q_full[2][NQ], q_empty[2][NQ], kv_full[NS], kv_empty[NS], s_full[2], s_free[2], ds_full[2], dq_done[2],
-  // item_full[], item_empty[], mma_done[2]
-  static constexpr int NBAR = 4 * NQ + 2 * NS + 8 + 2 * kItems + 2;
+  // q_full[2][NQ], q_empty[2][NQ], kv_full[NS], kv_empty[NS], s_full[2], s_free[2], dp_full[2], ds_full[2],
+  // dq_done[2], item_full[], item_empty[], mma_done[2]
+  static constexpr int NBAR = 4 * NQ + 2 * NS + 10 + 2 * kItems + 2;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int BYTES = OFF_MISC + 16 + 1024;
   static constexpr int ALLOC = BYTES > kOneCtaPerSmSmem ? BYTES : kOneCtaPerSmSmem;
@@ -106,7 +113,8 @@ __global__ void __launch_bounds__(kBwThreads, 1)
   uint64_t* kv_empty = kv_full + L::NS;
   uint64_t* s_full = kv_empty + L::NS;
   uint64_t* s_free = s_full + 2;
-  uint64_t* ds_full = s_free + 2;
+  uint64_t* dp_full = s_free + 2;
+  uint64_t* ds_full = dp_full + 2;
   uint64_t* dq_done = ds_full + 2;
   uint64_t* item_full = dq_done + 2;
   uint64_t* item_empty = item_full + kItems;
@@ -123,6 +131,7 @@ __global__ void __launch_bounds__(kBwThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&s_free[i], 4);
+      mbar_init(&dp_full[i], 1);
       mbar_init(&ds_full[i], 4);
       mbar_init(&dq_done[i], 1);
       mbar_init(&mma_done[i], 1);
@@ -139,9 +148,7 @@ __global__ void __launch_bounds__(kBwThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // TMEM columns per row tile u: S [128 u, +64), dP [128 u + 64, +64), dQ [256 + u D, + D), and dS (32) in
-  // [384 + 32 u, +32) up to D = 64, else over S
-  constexpr bool kOwnDs = D <= 64;
+  // TMEM columns per row tile u: S [128 u, +64), dP [128 u + 64, +64) with dS over it, dQ [256 + u D, +D)
 
   if (warp == 10) {
     // ------------------------------ producer ------------------------------
@@ -204,7 +211,6 @@ __global__ void __launch_bounds__(kBwThreads, 1)
     // --------------------------- tensor-core issue ---------------------------
     const int u = warp - 8;
     const uint32_t tm_s = tmem + u * 128, tm_dp = tm_s + 64, tm_dq = tmem + 256 + u * D;
-    const uint32_t tm_ds = kOwnDs ? tmem + 384 + 32 * u : tm_s;
     const uint32_t idesc_s = make_idesc(AB, 0, 0, 128, kDqKeys), idesc_q = make_idesc(AB, 0, 1, 128, D);
     int n_it = 0, J = 0, nq = 0, ns = 0, np = 0;  // items, ring slots, Q tiles, S and dQ products so far
     while (true) {
@@ -226,19 +232,27 @@ __global__ void __launch_bounds__(kBwThreads, 1)
         __syncwarp();
         return true;
       };
-      auto issue_s = [&](int t) {
-        const int sk = (J + 2 * t) % L::NS, sv = (J + 2 * t + 1) % L::NS;
-        if (!wait_slot(J + 2 * t) || !wait_slot(J + 2 * t + 1)) return false;
-        // the last S and dP have been read; where dS lies over S, the product that reads it is over
-        if (kOwnDs && ns > 0 && !wait_phase(&s_free[u], (ns - 1) & 1, abort_flag, p.err)) return false;
-        if (!kOwnDs && np > 0 && !wait_phase(&dq_done[u], (np - 1) & 1, abort_flag, p.err)) return false;
+      auto issue_s = [&](int t) {  // once the last S has been read
+        const int sk = (J + 2 * t) % L::NS;
+        if (!wait_slot(J + 2 * t)) return false;
+        if (ns > 0 && !wait_phase(&s_free[u], (ns - 1) & 1, abort_flag, p.err)) return false;
         ++ns;
         tc_fence_after();
         if (elect_one()) {
-          const uint32_t k_base = smem_u32(sKV + sk * L::KT), v_base = smem_u32(sKV + sv * L::KT);
-          mma_rows<D, 128, kDqKeys>(tm_s, q_base, k_base, idesc_s);
-          mma_rows<D, 128, kDqKeys>(tm_dp, do_base, v_base, idesc_s);
+          mma_rows<D, 128, kDqKeys>(tm_s, q_base, smem_u32(sKV + sk * L::KT), idesc_s);
           umma_commit(&s_full[u]);
+        }
+        __syncwarp();
+        return true;
+      };
+      auto issue_dp = [&](int t) {  // once the product that reads the last dS is over
+        const int sv = (J + 2 * t + 1) % L::NS;
+        if (!wait_slot(J + 2 * t + 1)) return false;
+        if (np > 0 && !wait_phase(&dq_done[u], (np - 1) & 1, abort_flag, p.err)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+          mma_rows<D, 128, kDqKeys>(tm_dp, do_base, smem_u32(sKV + sv * L::KT), idesc_s);
+          umma_commit(&dp_full[u]);
           umma_commit(&kv_empty[sv]);
           if (t == b - 1) umma_commit(&q_empty[st_q]);
         }
@@ -248,11 +262,11 @@ __global__ void __launch_bounds__(kBwThreads, 1)
       bool ok = true;
       for (int t = 0; t < a && ok; ++t) ok = pass(t);
       if (ok && b > a) {
-        ok = wait_phase(&q_full[st_q], (nq / L::NQ) & 1, abort_flag, p.err) && issue_s(a);
+        ok = wait_phase(&q_full[st_q], (nq / L::NQ) & 1, abort_flag, p.err) && issue_s(a) && issue_dp(a);
         ++nq;
       }
       for (int t = a; t < b && ok; ++t) {
-        if (kOwnDs && t + 1 < b && !(ok = issue_s(t + 1))) break;
+        if (t + 1 < b && !(ok = issue_s(t + 1))) break;
         const int st = (J + 2 * t) % L::NS, valid = it.valid<kDqKeys>(t);
         if (valid < kDqKeys) zero_rows<D>(sKV + st * L::KT, kDqKeys, valid);
         if (!(ok = wait_phase(&ds_full[u], np & 1, abort_flag, p.err))) break;
@@ -260,12 +274,12 @@ __global__ void __launch_bounds__(kBwThreads, 1)
         tc_fence_after();
         if (elect_one()) {
           const uint32_t k_base = smem_u32(sKV + st * L::KT);
-          mma_sum<D, kDqKeys>(tm_dq, tm_ds, k_base, idesc_q, t > a);
+          mma_sum<D, kDqKeys>(tm_dq, tm_dp, k_base, idesc_q, t > a);
           umma_commit(&dq_done[u]);
           umma_commit(&kv_empty[st]);
         }
         __syncwarp();
-        if (!kOwnDs && t + 1 < b) ok = issue_s(t + 1);
+        if (t + 1 < b) ok = issue_dp(t + 1);
       }
       for (int t = b > a ? b : a; t < it.tiles && ok; ++t) ok = pass(t);
       if (!ok) break;
@@ -286,97 +300,122 @@ __global__ void __launch_bounds__(kBwThreads, 1)
     const int t_row = row / G, g = row - t_row * G;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t tm_s = tmem + u * 128 + lanes, tm_dp = tm_s + 64, tm_dq = tmem + 256 + u * D + lanes;
-    const uint32_t tm_ds = (kOwnDs ? tmem + 384 + 32 * u : tmem + u * 128) + lanes;
     const float sl2 = p.scale * 1.4426950408889634f;
+    const float2 sc = make_float2(sl2, sl2);
+    // An item's rows leave while the next one's lse, delta and first products are on their way.
+    bool due = false, due_any = false;
+    long long due_row = -1;
     int n_it = 0, ns = 0;
+    auto write_rows = [&]() -> bool {
+      if (due_any) {
+        if (!wait_phase(&dq_done[u], (ns - 1) & 1, abort_flag, p.err)) return false;
+        tc_fence_after();
+      }
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        float s[32];
+        uint32_t w[16];
+        if (due_any) {
+          tmem_ld32(tm_dq + c, s);
+          tmem_wait_values<32>(s);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 2)
+          w[i / 2] = due_any ? pack2<BF16>(s[i] * p.scale, s[i + 1] * p.scale) : 0u;
+        store_rows32(smem_u32(smem + L::OFF_ROWS + warp * kRowBuf), w, due_row, static_cast<uint16_t*>(p.dq), D, c);
+      }
+      tc_fence_before();  // dQ is read before this warp's next dS lets the next item overwrite it
+      return true;
+    };
     while (true) {
       const int r = n_it % kItems;
       if (!wait_phase(&item_full[r], (n_it / kItems) & 1, abort_flag, p.err)) break;
       const RowItem& it = items[r];
       ++n_it;
-      if (it.stop) break;
+      if (it.stop) {
+        if (due) write_rows();
+        break;
+      }
       const int a = it.a[u], b = it.b[u];
       const bool live = t_row < it.n[u] && t_row < TT;
-      const RowView<kDqKeys> view(p, it, it.pos + u * TT + t_row, live, 0, kDqKeys);
       const long long orow = (long long)(it.tok + u * TT + t_row) * p.hq + it.hk * G + g;
       float lse2 = live ? p.lse[orow] * 1.4426950408889634f : 0.f;
-      if (lse2 == -INFINITY) lse2 = 0.f;  // a row that sees nothing: every column is masked
       const float delta = live ? p.delta[orow] : 0.f;
-      const float2 sc = make_float2(sl2, sl2), nl = make_float2(-lse2, -lse2), nd = make_float2(-delta, -delta);
+      const RowView<kDqKeys> view(p, it, it.pos + u * TT + t_row, live, 0, kDqKeys);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[r]);
+      if (due && !write_rows()) break;
+      due = true;
+      due_any = b > a;
+      due_row = live ? orow : -1;
+      if (lse2 == -INFINITY) lse2 = 0.f;  // a row that sees nothing: every column is masked
+      const float2 nl = make_float2(-lse2, -lse2), nd = make_float2(-delta, -delta);
       bool ok = true;
-      float s[32], d[32];
       for (int t = a; t < b; ++t) {
         uint32_t bits[2] = {0xffffffffu, 0xffffffffu};
         const bool all = view.full(t);
         if (!all) bits[0] = view.bits(t, 0), bits[1] = view.bits(t, 32);
+        const bool some[2] = {all || __any_sync(0xffffffffu, bits[0] != 0u), all || __any_sync(0xffffffffu, bits[1] != 0u)};
         if (!(ok = wait_phase(&s_full[u], ns & 1, abort_flag, p.err))) break;
+        tc_fence_after();
+        float s[2][32];
+        if (some[0]) tmem_ld32(tm_s, s[0]);
+        if (some[1]) tmem_ld32(tm_s + 32, s[1]);
+        tmem_wait_values<32>(s[0]);
+        tmem_wait_values<32>(s[1]);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[u]);  // the next tile's S is formed under this one's exponentials
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          if (some[c]) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float2 e = fma2(make_float2(s[c][i], s[c][i + 1]), sc, nl);
+              s[c][i] = ex2(e.x);
+              s[c][i + 1] = ex2(e.y);
+            }
+          }
+        }
+        if (!(ok = wait_phase(&dp_full[u], ns & 1, abort_flag, p.err))) break;
         ++ns;
         tc_fence_after();
         uint32_t w[2][16];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          if (all || __any_sync(0xffffffffu, bits[c] != 0u)) {
-            tmem_ld32(tm_s + 32 * c, s);
-            tmem_ld32(tm_dp + 32 * c, d);
-            tmem_wait_values<32>(s);
-            tmem_wait_values<32>(d);
+          if (some[c]) {
             const bool full = all || __all_sync(0xffffffffu, !live || bits[c] == 0xffffffffu);
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float2 e = fma2(make_float2(s[i], s[i + 1]), sc, nl);
-              e.x = ex2(e.x);
-              e.y = ex2(e.y);
-              e = mul2(e, add2(make_float2(d[i], d[i + 1]), nd));
-              s[i] = e.x;
-              s[i + 1] = e.y;
+            for (int h = 0; h < 32; h += 16) {
+              float d[16];
+              tmem_ld16(tm_dp + 32 * c + h, d);
+              tmem_wait_values<16>(d);
+#pragma unroll
+              for (int i = 0; i < 16; i += 2) {
+                const float2 e = mul2(make_float2(s[c][h + i], s[c][h + i + 1]), add2(make_float2(d[i], d[i + 1]), nd));
+                s[c][h + i] = e.x;
+                s[c][h + i + 1] = e.y;
+              }
             }
             if (!full) {
 #pragma unroll
-              for (int i = 0; i < 32; ++i) s[i] = (bits[c] >> i & 1u) ? s[i] : 0.f;
+              for (int i = 0; i < 32; ++i) s[c][i] = (bits[c] >> i & 1u) ? s[c][i] : 0.f;
             }
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) w[c][i / 2] = pack2<BF16>(s[i], s[i + 1]);
+            for (int i = 0; i < 32; i += 2) w[c][i / 2] = pack2<BF16>(s[c][i], s[c][i + 1]);
           } else {
 #pragma unroll
             for (int i = 0; i < 16; ++i) w[c][i] = 0u;
           }
         }
-        if (kOwnDs) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_free[u]);
-          // dS's columns are free once the product of the tile before is over
-          if (t > a && !(ok = wait_phase(&dq_done[u], (ns - 2) & 1, abort_flag, p.err))) break;
-          tc_fence_after();
-        }
-        tmem_st16(tm_ds, w[0]);
-        tmem_st16(tm_ds + 16, w[1]);
+        tmem_st16(tm_dp, w[0]);  // over dP
+        tmem_st16(tm_dp + 16, w[1]);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&ds_full[u]);
       }
       if (!ok) break;
-      if (b > a) {
-        if (!wait_phase(&dq_done[u], (ns - 1) & 1, abort_flag, p.err)) break;
-        tc_fence_after();
-      }
-#pragma unroll
-      for (int c = 0; c < D; c += 32) {
-        uint32_t w[16];
-        if (b > a) {
-          tmem_ld32(tm_dq + c, s);
-          tmem_wait_values<32>(s);
-        }
-#pragma unroll
-        for (int i = 0; i < 32; i += 2)
-          w[i / 2] = b > a ? pack2<BF16>(s[i] * p.scale, s[i + 1] * p.scale) : 0u;
-        store_rows32(smem_u32(smem + L::OFF_ROWS + warp * kRowBuf), w, live ? orow : -1, static_cast<uint16_t*>(p.dq), D,
-                     c);
-      }
-      tc_fence_before();  // dQ is read before this warp's next dS lets the next item overwrite it
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&item_empty[r]);
     }
   }
   tc_fence_before();
