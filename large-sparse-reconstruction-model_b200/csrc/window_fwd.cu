@@ -21,7 +21,8 @@
 // end.
 //
 // What bounds it: 16384 tokens in two sequences, 32 / 8 heads of 128 channels,
-// causal window 2048: 545 us, 880 TFLOP/s (0.53 of the library's GEMM rate); the
+// causal window 2048: 530 us, 900 TFLOP/s (0.54 of the library's GEMM rate; 565 us
+// with what O's rounding leaves over, which training keeps); the
 // tensor pipe is active 41 % of the time, the exponentials' pipe 40 %, and no
 // other unit more.  The softmax warps' chain of a tile (wait, TMEM read, maximum,
 // exponentials, TMEM write, arrive) takes 1.5 times the exponentials alone; the
@@ -269,15 +270,61 @@ __global__ void __launch_bounds__(kFwThreads, 1)
     const uint32_t tm_s0 = tmem + u * 128 + lanes, tm_o = tmem + 256 + u * D + lanes;
     const float sl2 = p.scale * 1.4426950408889634f;
     int n_it = 0, ns = 0;  // items, tiles so far
+    // An item's rows leave while the next one's first products run (1 to 5 % of the time, against at its own end).
+    struct {
+      bool due;
+      float m, l;
+      long long row;
+    } last = {};
+    auto write_rows = [&](bool any) -> bool {
+      last.due = false;
+      if (any) {
+        if (!wait_phase(&pv_done[2 * u + ((ns - 1) & 1)], ((ns - 1) >> 1) & 1, abort_flag, p.err)) return false;
+        tc_fence_after();
+      }
+      const bool none = !any || last.l == 0.f;
+      const float inv = none ? 0.f : 1.f / last.l;
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        float o[32];
+        uint32_t w[16];
+        if (any) {
+          tmem_ld32(tm_o + c, o);
+          tmem_wait_values<32>(o);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) w[i / 2] = none ? 0u : pack2<BF16>(o[i] * inv, o[i + 1] * inv);
+        const uint32_t buf = smem_u32(smem + L::OFF_ROWS + warp * kRowBuf);
+        store_rows32(buf, w, last.row, static_cast<uint16_t*>(p.out), D, c);
+        if (p.out_rest) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float2 r = unpack2<BF16>(w[i / 2]);
+            w[i / 2] = none ? 0u : pack2<BF16>(fmaf(o[i], inv, -r.x), fmaf(o[i + 1], inv, -r.y));
+          }
+          store_rows32(buf, w, last.row, static_cast<uint16_t*>(p.out_rest), D, c);
+        }
+      }
+      tc_fence_before();  // O is read before this warp's next P lets the next item overwrite it
+      if (last.row >= 0) p.lse[last.row] = none ? -INFINITY : (last.m + log2f(last.l)) * 0.6931471805599453f;
+      return true;
+    };
     while (true) {
       const int r = n_it % kItems;
       if (!wait_phase(&item_full[r], (n_it / kItems) & 1, abort_flag, p.err)) break;
       const RowItem& it = items[r];
       ++n_it;
-      if (it.stop) break;
+      if (it.stop) {
+        if (last.due) write_rows(true);
+        break;
+      }
       const int a = it.a[u], b = it.b[u];
       const bool live = t_row < it.n[u] && t_row < TT;
+      const long long orow = live ? (long long)(it.tok + u * TT + t_row) * p.hq + it.hk * G + g : -1;
       const RowView<kFwKeys> view(p, it, it.pos + u * TT + t_row, live, 0, kFwKeys);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[r]);
+      if (last.due && !write_rows(true)) break;
       float m = -INFINITY;
       float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
       bool ok = true;
@@ -359,38 +406,14 @@ __global__ void __launch_bounds__(kFwThreads, 1)
         if (lane == 0) mbar_arrive(&p_full[2 * u + ((ns - 1) & 1)]);
       }
       if (!ok) break;
+      last.row = orow;
       if (b > a) {
-        if (!wait_phase(&pv_done[2 * u + ((ns - 1) & 1)], ((ns - 1) >> 1) & 1, abort_flag, p.err)) break;
-        tc_fence_after();
+        last.due = true;
+        last.m = m;
+        last.l = l2[0].x + l2[0].y + l2[1].x + l2[1].y;
+      } else {
+        write_rows(false);
       }
-      const float l = l2[0].x + l2[0].y + l2[1].x + l2[1].y;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      const long long orow = (long long)(it.tok + u * TT + t_row) * p.hq + it.hk * G + g;
-#pragma unroll
-      for (int c = 0; c < D; c += 32) {
-        float* o = s[0];
-        uint32_t w[16];
-        if (b > a) {
-          tmem_ld32(tm_o + c, o);
-          tmem_wait_values<32>(o);
-        }
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) w[i / 2] = l == 0.f ? 0u : pack2<BF16>(o[i] * inv, o[i + 1] * inv);
-        const uint32_t buf = smem_u32(smem + L::OFF_ROWS + warp * kRowBuf);
-        store_rows32(buf, w, live ? orow : -1, static_cast<uint16_t*>(p.out), D, c);
-        if (p.out_rest) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float2 r = unpack2<BF16>(w[i / 2]);
-            w[i / 2] = l == 0.f ? 0u : pack2<BF16>(fmaf(o[i], inv, -r.x), fmaf(o[i + 1], inv, -r.y));
-          }
-          store_rows32(buf, w, live ? orow : -1, static_cast<uint16_t*>(p.out_rest), D, c);
-        }
-      }
-      if (live) p.lse[orow] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-      tc_fence_before();  // O is read before this warp's next P lets the next item overwrite it
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&item_empty[r]);
     }
   }
   tc_fence_before();
