@@ -21,15 +21,17 @@
 // end.
 //
 // What bounds it: 16384 tokens in two sequences, 32 / 8 heads of 128 channels,
-// causal window 2048: 530 us, 900 TFLOP/s (0.54 of the library's GEMM rate; 565 us
-// with what O's rounding leaves over, which training keeps); the
-// tensor pipe is active 41 % of the time, the exponentials' pipe 40 %, and no
-// other unit more.  The softmax warps' chain of a tile (wait, TMEM read, maximum,
-// exponentials, TMEM write, arrive) takes 1.5 times the exponentials alone; the
-// two row tiles hide half of it.  Without the exponentials the time stays within
-// 3 % there, and falls by 15 % at 64 channels.  Tried without gain: tiles of 128
-// keys with a row's scores in registers (575 us), P in a place of its own (639),
-// two threads a row (999), the row tiles taking turns at the exponentials (633).
+// causal window 2048: 530 us, 900 TFLOP/s (0.54 of the library's GEMM rate; 560 us
+// with what O's rounding leaves over, which training keeps); the tensor pipe is
+// active 41 % of the time, the exponentials' pipe 40 %, and no other unit more.
+// 131072 tokens, 16 heads of 64 channels, symmetric window 512: 720 us (763).  The
+// softmax warps' chain of a tile (wait, TMEM read, maximum, exponentials, TMEM
+// write, arrive) takes 1.5 times the exponentials alone; the two row tiles hide
+// half of it.  Without the exponentials the time stays within 3 % at 128
+// channels, and falls by 15 % at 64.  Tried without gain: tiles of 128 keys with a
+// row's scores in registers (575 us at 128 channels), P in a place of its own
+// (639), two threads a row (999), the row tiles taking turns at the exponentials
+// (633), two CTAs a multiprocessor that read S twice (847 us at 64 channels).
 #include "window_host.h"
 #include "window_tile.cuh"
 
