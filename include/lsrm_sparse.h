@@ -480,7 +480,9 @@ int lsrm_qkv_norm_bwd(int64_t M, int32_t N, int32_t head_dim, const lsrm_qkv_gra
  *   otherwise: |pos - j| <= window / 2 or j < sinks.
  * A query that sees no key gets o = 0 and lse = -inf, and its gradients are
  * zero; so do tokens after the last sequence, whose contents are not used.
- * Offsets that leave the tensors set LSRM_ERR_BAD_INDEX in err_flags. */
+ * Offsets that leave the tensors set LSRM_ERR_BAD_INDEX in err_flags.  A value
+ * that is no finite number stays within its sequence; inside it, it may reach
+ * queries that do not see it (0 times it, in a shared tile of keys). */
 typedef struct lsrm_window_shape {
   int32_t num_seqs, total_q, total_k;
   int32_t num_q_heads;  /* Hq, a multiple of Hkv, at most 64 times as many */

@@ -131,7 +131,9 @@ def window_sink_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, window: i
       band, with sinks)
 
     A query that sees nothing gives 0.  Differentiable in q, k and v.  With
-    ``return_lse`` also the natural-log LSE [Hq, Nq] fp32."""
+    ``return_lse`` also the natural-log LSE [Hq, Nq] fp32.  A value that is no
+    finite number stays within its sequence, where it may reach queries that do
+    not see it (0 times it, in a shared tile of keys)."""
     cu_k = cu_seqlens_q if cu_seqlens_k is None else cu_seqlens_k
     out, lse = F.window_sink_attention(q, k, v, cu_seqlens_q, cu_k, window, sinks, causal, softmax_scale)
     _raise_on_device_errors()
