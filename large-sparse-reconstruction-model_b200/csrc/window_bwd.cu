@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(256) window_delta_kernel(const uint4* __restri
 // under the exponentials, and dS lies over dP, whose next product follows dQ's
 // under the next exponentials: 685 us there, 1.0 PFLOP/s, against 913 with both
 // waiting for dS; 131072 tokens, 16 heads of 64 channels, symmetric window 512:
-// 880 us against 922.
+// 866 us (884 then) against 922.
 
 constexpr int kBwThreads = 352;
 constexpr int kDqKeys = 64;
@@ -437,14 +437,16 @@ __global__ void __launch_bounds__(kBwThreads, 1)
 //
 // What bounds it: a tile's chain (products, exponentials, sums), of which two or
 // three are in flight.  131072 tokens, 16 heads of 64 channels, symmetric window
-// 512: 1018 us; with two stages, whose P^T and dS^T have places of their own,
-// 1083 us.  16384 tokens, 32 / 8 heads of 128 channels, causal window 2048: 1005 us,
+// 512: 1002 us; with two stages, whose P^T and dS^T have places of their own, 1083
+// against 1018.  16384 tokens, 32 / 8 heads of 128 channels, causal window 2048: 991 us,
 // the tensor pipe's own time about 650.  The scores come from TMEM eight columns
-// at a time: with sixteen 1050 us there, with all 32 up front 1183 (the registers
-// then leave the exponentials no slack).  Four threads a key, all 16 warps on one
+// at a time: with sixteen 1050 us there against 1005, with all 32 up front 1183 (the
+// registers then leave the exponentials no slack).  Four threads a key, all 16 warps on one
 // tile, gives 1008 us there and loses elsewhere (ragged sequences, 32 / 2 heads of
-// 32 channels: 320 us against 273).  An item's sums leave under the next one's first
-// tiles: 1244 us against 1125 before the other steps.
+// 32 channels: 320 us against 273); S^T and dP^T on barriers of their own, as in dQ,
+// keep a tile's exponentials in registers that are not there (1108 us against 1016;
+// with one thread a key 1037 against 994).  An item's sums leave under the next one's
+// first tiles: 1125 us against 1244 before the other steps (131072 tokens).
 
 constexpr int kKvRows = 64;  // packed query rows of a tile
 constexpr int kKvThreads = 640;

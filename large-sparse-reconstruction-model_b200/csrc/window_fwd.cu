@@ -24,7 +24,7 @@
 // causal window 2048: 530 us, 900 TFLOP/s (0.54 of the library's GEMM rate; 560 us
 // with what O's rounding leaves over, which training keeps); the tensor pipe is
 // active 41 % of the time, the exponentials' pipe 40 %, and no other unit more.
-// 131072 tokens, 16 heads of 64 channels, symmetric window 512: 720 us (763).  The
+// 131072 tokens, 16 heads of 64 channels, symmetric window 512: 710 us (752).  The
 // softmax warps' chain of a tile (wait, TMEM read, maximum, exponentials, TMEM
 // write, arrive) takes 1.5 times the exponentials alone; the two row tiles hide
 // half of it.  Without the exponentials the time stays within 3 % at 128
