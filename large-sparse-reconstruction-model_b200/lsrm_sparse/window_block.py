@@ -57,12 +57,20 @@ class WindowCache:
         self.window, self.sinks = window, sinks
 
     def fill(self, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor):
-        """Keep what later tokens can see of packed prompts k / v [N, heads, head_dim]."""
+        """Keep what later tokens can see of packed prompts k / v [N, heads, head_dim].
+        Tokens before the first and after the last sequence are padding, as in
+        ``window_sink_attention``."""
+        n = cu_seqlens.numel() - 1
+        if n == 0:
+            return
         cu = cu_seqlens.long()
         tok = torch.arange(k.shape[0], device=k.device)
         seq = torch.searchsorted(cu, tok, right=True) - 1
+        inside = (seq >= 0) & (seq < n)
+        seq = seq.clamp(0, n - 1)
         pos, left = tok - cu[seq], cu[seq + 1] - tok
-        kept = (pos < self.sinks) | (left <= self.window)
+        inside &= (pos >= 0) & (left > 0)  # offsets that are out of order write nothing out of range
+        kept = inside & ((pos < self.sinks) | (left <= self.window))
         tok, seq, pos = tok[kept], seq[kept], pos[kept]
         slot = torch.where(pos < self.sinks, pos, self.sinks + (pos - self.sinks) % self.window)
         self.k[seq, slot], self.v[seq, slot] = k[tok], v[tok]

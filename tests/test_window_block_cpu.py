@@ -1,0 +1,45 @@
+"""The windowed stack's host side, on CPU tensors: which keys and values a
+prompt leaves in the ring cache."""
+
+import pytest
+import torch
+
+from lsrm_sparse.window_block import WindowCache
+
+
+def _filled(cu, n, window, sinks):
+    """(cache after fill, cache expected): token t's key is t + 1, untouched slots hold 0."""
+    batch = len(cu) - 1
+    cache = WindowCache(batch, window, sinks, 1, 1, torch.float32, "cpu")
+    cache.k.zero_()
+    cache.v.zero_()
+    k = torch.arange(1.0, n + 1)[:, None, None]
+    cache.fill(k, -k, torch.tensor(cu, dtype=torch.int32))
+    want = torch.zeros(batch, sinks + window, 1, 1)
+    for b in range(batch):
+        length = cu[b + 1] - cu[b]
+        for pos in range(length):
+            if pos < sinks or length - pos <= window:
+                want[b, pos if pos < sinks else sinks + (pos - sinks) % window] = cu[b] + pos + 1
+    return cache, want
+
+
+@pytest.mark.parametrize("cu,n", [
+    ([0, 5, 5, 30], 30),
+    ([0, 5, 12], 20),     # tokens after the last sequence
+    ([4, 9, 21], 21),     # and before the first
+    ([3, 3], 8),          # an empty sequence between padding
+    ([0], 6),             # no sequence at all
+    ([0], 0),
+])
+@pytest.mark.parametrize("window,sinks", [(4, 2), (1, 0), (40, 3)])
+def test_cache_keeps_what_later_tokens_see(cu, n, window, sinks):
+    cache, want = _filled(cu, n, window, sinks)
+    assert torch.equal(cache.k, want) and torch.equal(cache.v, -want)
+
+
+def test_offsets_out_of_order_stay_inside_the_cache():
+    """Such offsets are an error of the caller's that the attention reports; the cache's indices stay in range."""
+    for cu in ([0, 9, 4, 12], [8, 2, 30], [-3, 40]):
+        cache = WindowCache(len(cu) - 1, 4, 2, 1, 1, torch.float32, "cpu")
+        cache.fill(torch.ones(12, 1, 1), torch.ones(12, 1, 1), torch.tensor(cu, dtype=torch.int32))
