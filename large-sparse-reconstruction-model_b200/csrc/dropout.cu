@@ -3,10 +3,11 @@
 // call on the gradient.  A thread takes eight elements (two counter blocks).
 //
 // Bound by the 32 x 32 bit products rather than by HBM: 36 of them per eight
-// elements, four cycles a warp on their pipe.  537 million bf16 elements: 475
-// us (4.5 TB/s); without the generator's last seven rounds 340 us, without the
-// memory 437 us, a plain copy 330 us.  Loading an iteration ahead does not
-// help (487 us): the warps that are resident hide the loads.
+// elements, four cycles a warp on their pipe.  537 million elements: bf16 486 us
+// (4.4 TB/s), fp16 471; a plain copy 329.  Of 475 us before the products went to
+// 32 bits: 340 without the generator's last seven rounds, 437 without the
+// memory.  Loading an iteration ahead does not help: the warps that are
+// resident hide the loads.
 #include <algorithm>
 
 #include "host_util.h"
@@ -16,25 +17,19 @@
 namespace lsrm {
 namespace {
 
-// Two packed 16-bit values times 1 / (1 - p), as hi + lo of it in their type:
-// x * lo is below x * hi by the type's precision, so its rounding is far below
-// the result's, and two instructions replace the unpacking, two products and
-// the packing.
-__device__ __forceinline__ uint32_t scale2(uint32_t x, __nv_bfloat162 hi, __nv_bfloat162 lo) {
-  const __nv_bfloat162 v = *reinterpret_cast<const __nv_bfloat162*>(&x), r = __hfma2(v, hi, __hmul2(v, lo));
+// Two packed 16-bit values times 1 / (1 - p): the 32-bit product rounded once,
+// right for infinities and at both ends of the type's range.  (The scale as
+// the sum of two 16-bit values would save two conversions and 2 % of the time,
+// and turns infinities into NaN.)
+__device__ __forceinline__ uint32_t scale2(uint32_t x, float s, __nv_bfloat16) {
+  const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
+  const __nv_bfloat162 r = __floats2bfloat162_rn(f.x * s, f.y * s);
   return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ uint32_t scale2(uint32_t x, __half2 hi, __half2 lo) {
-  const __half2 v = *reinterpret_cast<const __half2*>(&x), r = __hfma2(v, hi, __hmul2(v, lo));
+__device__ __forceinline__ uint32_t scale2(uint32_t x, float s, __half) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x));
+  const __half2 r = __floats2half2_rn(f.x * s, f.y * s);
   return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ void split_scale(float s, __nv_bfloat162& hi, __nv_bfloat162& lo) {
-  hi = __float2bfloat162_rn(s);
-  lo = __float2bfloat162_rn(s - __low2float(hi));
-}
-__device__ __forceinline__ void split_scale(float s, __half2& hi, __half2& lo) {
-  hi = __float2half2_rn(s);
-  lo = __float2half2_rn(s - __low2float(hi));
 }
 
 template <typename T>
@@ -47,14 +42,11 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, T
   for (; c < full; c += stride) {
     Raw8<T> r = load8_raw(x, c);  // in flight over the generator's rounds
     if constexpr (sizeof(T) == 2) {
-      using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
-      T2 hi, lo;
-      split_scale(d.scale, hi, lo);
       uint32_t w[8], *v = reinterpret_cast<uint32_t*>(r.u);
       dropout_words(d, ph, c, w);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        uint32_t s = scale2(v[i], hi, lo);
+        uint32_t s = scale2(v[i], d.scale, T());
         if (w[2 * i] < d.threshold) s &= 0xffff0000u;
         if (w[2 * i + 1] < d.threshold) s &= 0xffffu;
         v[i] = s;
