@@ -561,7 +561,8 @@ int lsrm_residual_rms_norm_bwd(int64_t rows, int32_t cols, int32_t dtype, int32_
 /* The forward with y in 8 bits (e4m3 or int8) and fp32 scales [rows,
  * ceil(cols / group)] per `group` columns (32, 64, 128; 0: one per row):
  * scale = max|y| / 448 (e4m3) or / 127 (int8), 1 for zeros; values =
- * y / scale rounded to nearest even. */
+ * y / scale rounded to nearest even.  A group whose y holds a NaN or an
+ * infinity has a NaN scale. */
 int lsrm_residual_rms_norm_8bit(int64_t rows, int32_t cols, int32_t dtype, int32_t stream_dtype, int32_t weight_dtype,
                                 float eps, int32_t out_dtype, int32_t group, const void* x, const void* residual,
                                 const void* weight, void* values, float* scales, void* h, void* stream);

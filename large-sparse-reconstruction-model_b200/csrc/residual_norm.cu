@@ -62,6 +62,13 @@ struct NormParams {
   float* dw_part;        // [blocks, cols] or null
 };
 
+// The larger of two magnitudes; NaN when either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // Sum / max over the TPR threads of a team.  Teams wider than a warp are whole
 // blocks; `buf` has two slots that alternate between calls, so one barrier a
 // call is enough.
@@ -70,7 +77,7 @@ __device__ __forceinline__ float team_reduce(float v, int tpr, float (*buf)[16],
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const float u = __shfl_xor_sync(0xffffffffu, v, o);
-    v = MAX ? fmaxf(v, u) : v + u;
+    v = MAX ? max_nan(v, u) : v + u;
   }
   if (tpr == 32) return v;
   const int warps = tpr >> 5;
@@ -79,7 +86,7 @@ __device__ __forceinline__ float team_reduce(float v, int tpr, float (*buf)[16],
   if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = v;
   __syncthreads();
   v = b[0];
-  for (int i = 1; i < warps; ++i) v = MAX ? fmaxf(v, b[i]) : v + b[i];
+  for (int i = 1; i < warps; ++i) v = MAX ? max_nan(v, b[i]) : v + b[i];
   return v;
 }
 
@@ -125,9 +132,12 @@ __device__ __forceinline__ void read_w8(const NormParams& p, int col0, float* f)
 enum NormOut { kOutPlain = 0, kOutE4m3 = 1, kOutInt8 = 2 };
 
 // A group's scale: its largest magnitude over the format's, 1 for a group of
-// zeros, and never so small that its reciprocal overflows.
+// zeros, and never so small that its reciprocal overflows.  A group that holds
+// a NaN or an infinity gets a NaN scale: int8 has no value for them, so the
+// scale says that the group's values stand for no numbers.
 __device__ __forceinline__ float scale_of(float amax, float q_inv) {
-  return amax > 0.f ? fmaxf(amax * q_inv, 1.1754944e-38f) : 1.f;
+  if (amax == 0.f) return 1.f;
+  return amax <= 3.4028235e38f ? fmaxf(amax * q_inv, 1.1754944e-38f) : __int_as_float(0x7fffffff);
 }
 
 // Eight values of at most q_max / inv to 8 bits, to nearest even: e4m3 by the
@@ -253,7 +263,7 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const NormParams p) 
         if (k < n8) write_chunk<EVEN>(y, c0 + k, EVEN ? Part{0, 8} : part_of(c0 + k, e0, p.cols), v[i]);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[i][j]));
+        for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(v[i][j]));
       }
     }
     if (OUT == kOutPlain) continue;
@@ -285,8 +295,8 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const NormParams p) 
         if (!whole) {
           a = 0.f;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) a = fmaxf(a, fabsf(v[i][j]));
-          for (int o = p.group >> 4; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+          for (int j = 0; j < 8; ++j) a = max_nan(a, fabsf(v[i][j]));
+          for (int o = p.group >> 4; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
         }
         const float scale = scale_of(a, p.q_inv);
         if (k < n8) {

@@ -178,8 +178,8 @@ def residual_rms_norm_8bit(x, residual=None, weight=None, *, eps: float = 1e-6, 
                            group: int = 0):
     """``residual_rms_norm`` (without dropout) with y in 8 bits: returns
     (values, scales, h).  ``dtype`` is float8_e4m3fn or int8; one fp32 scale per
-    row, or per ``group`` (32, 64, 128) columns; y ~ values * scale.  Not
-    differentiable."""
+    row, or per ``group`` (32, 64, 128) columns; y ~ values * scale.  The scale of
+    a row or group whose y holds a NaN or an infinity is NaN.  Not differentiable."""
     if group not in (0, 32, 64, 128):
         raise ValueError(f"residual_rms_norm_8bit: group ({group}) must be 0, 32, 64 or 128")
     with torch.no_grad():
