@@ -166,9 +166,10 @@ class WindowStack(nn.Module):
     @torch.no_grad()
     def step(self, x, caches, lengths):
         """The next token of each sequence, x [batch, dim], with ``lengths`` tokens
-        before it; returns its output and the new lengths."""
+        before it; returns its output and the new lengths.  A negative length marks
+        an idle row: its caches and its length stay as they are."""
         branch, stream = x, None
         for b, c in zip(self.blocks, caches):
             branch, stream = b.step(branch, stream, c, lengths)
         y = api.residual_rms_norm(branch, stream, self.norm, eps=self.eps)[0]
-        return y, lengths + 1
+        return y, lengths + (lengths >= 0).to(lengths.dtype)

@@ -35,3 +35,32 @@ def test_padded_prompts_then_tokens():
             c = torch.tensor([0, m + t + 1], dtype=torch.int32, device="cuda")
             ref = _reference(stack, full[i, :m + t + 1], c)[-1]
             assert (y[i].double() - ref).norm() <= 10 * 2.0**-8 * ref.norm(), (i, t)
+
+
+def test_idle_rows_stay_idle():
+    """A row of negative length keeps it and its caches over several steps; the others go on as if it were not there."""
+    stack = _stack().eval()
+    full = torch.randn(3, 12, 256, device="cuda").bfloat16()
+    caches = stack.make_caches(3, torch.bfloat16, "cuda")
+    for c in caches:
+        c.k.fill_(float("nan"))
+        c.v.fill_(float("nan"))
+    lengths = torch.tensor([0, -1, 0], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 6], dtype=torch.int32, device="cuda")
+    outs = []
+    for t in range(6):
+        y, lengths = stack.step(full[:, t], caches, lengths)
+        outs.append(y)
+    assert lengths.tolist() == [6, -1, 6] and lengths.dtype == torch.int32
+    for c in caches:
+        assert torch.isnan(c.k[1]).all() and torch.isnan(c.v[1]).all()
+    for i in (0, 2):
+        ref = _reference(stack, full[i, :6], cu)
+        got = torch.stack(outs, 1)[i].double()
+        assert (got - ref).norm() <= 10 * 2.0**-8 * ref.norm(), i
+    # taken up later, the row starts from its own position
+    lengths[1] = 0
+    y, lengths = stack.step(full[:, 6], caches, lengths)
+    ref = _reference(stack, full[1, 6:7], torch.tensor([0, 1], dtype=torch.int32, device="cuda"))
+    assert lengths.tolist() == [7, 1, 7]
+    assert (y[1:2].double() - ref).norm() <= 10 * 2.0**-8 * ref.norm()
