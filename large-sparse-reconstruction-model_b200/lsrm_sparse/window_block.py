@@ -103,10 +103,16 @@ class WindowBlock(nn.Module):
         hq, hkv, d = self.num_q_heads, self.num_kv_heads, self.head_dim
         return (t.unflatten(1, (-1, d)) for t in qkv.split([hq * d, hkv * d, hkv * d], 1))
 
+    def _check_causal(self):
+        if not self.causal:
+            raise ValueError("the single-token form is causal: a stack with causal=False has no prefill and no step")
+
     def forward(self, branch, stream, cu_seqlens, seed: int = 0, site: int = 0, first: bool = False,
                 cache: Optional[WindowCache] = None):
         """branch and stream [N, dim] (stream None at the stack's start); returns
         the next (branch, stream).  ``site`` counts the stack's dropout sites."""
+        if cache is not None:
+            self._check_causal()
         p = self.dropout if self.training else 0.0
         qkv, stream = self._norm_linear(branch, stream, self.norm_attn, self.qkv, 0.0 if first else p, seed,
                                         site * _SITE)
@@ -119,7 +125,8 @@ class WindowBlock(nn.Module):
         return self.fc2(api.dropout(self.act(hidden), p, seed, (site + 2) * _SITE)), stream
 
     def step(self, branch, stream, cache: WindowCache, lengths):
-        """One token of each sequence ([batch, dim]) over the cache."""
+        """One token of each sequence ([batch, dim]) over the cache (causal blocks)."""
+        self._check_causal()
         qkv, stream = self._norm_linear(branch, stream, self.norm_attn, self.qkv, 0.0, 0, 0)
         q, k, v = self._split(qkv)
         o = api.window_sink_decode(q, k, v, cache.k, cache.v, lengths, window=self.window, sinks=self.sinks)

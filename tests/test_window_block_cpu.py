@@ -4,7 +4,7 @@ prompt leaves in the ring cache."""
 import pytest
 import torch
 
-from lsrm_sparse.window_block import WindowCache
+from lsrm_sparse.window_block import WindowCache, WindowStack
 
 
 def _filled(cu, n, window, sinks):
@@ -43,3 +43,13 @@ def test_offsets_out_of_order_stay_inside_the_cache():
     for cu in ([0, 9, 4, 12], [8, 2, 30], [-3, 40]):
         cache = WindowCache(len(cu) - 1, 4, 2, 1, 1, torch.float32, "cpu")
         cache.fill(torch.ones(12, 1, 1), torch.ones(12, 1, 1), torch.tensor(cu, dtype=torch.int32))
+
+
+def test_symmetric_stacks_have_no_single_token_form():
+    stack = WindowStack(1, 64, 2, 1, window=4, causal=False)
+    x, cu = torch.zeros(3, 64), torch.tensor([0, 3], dtype=torch.int32)
+    caches = stack.make_caches(1, torch.float32, "cpu")
+    for call in (lambda: stack.prefill(x, cu), lambda: stack(x, cu, caches=caches),
+                 lambda: stack.step(x[:1], caches, torch.zeros(1, dtype=torch.int32))):
+        with pytest.raises(ValueError, match="causal"):
+            call()
