@@ -479,7 +479,8 @@ int lsrm_qkv_norm_bwd(int64_t M, int32_t N, int32_t head_dim, const lsrm_qkv_gra
  *   causal:    j <= pos and (pos - j < window or j < sinks)
  *   otherwise: |pos - j| <= window / 2 or j < sinks.
  * A query that sees no key gets o = 0 and lse = -inf, and its gradients are
- * zero; so do tokens after the last sequence, whose contents are not used.
+ * zero; so do tokens before the first and after the last sequence, whose
+ * contents are not used.
  * Offsets that leave the tensors set LSRM_ERR_BAD_INDEX in err_flags.  A value
  * that is no finite number stays within its sequence; inside it, it may reach
  * queries that do not see it (0 times it, in a shared tile of keys). */

@@ -511,10 +511,10 @@ __device__ __forceinline__ bool kv_item(const WindowBwdParams& p, int w, int D, 
     const int slot = w / p.hkv;
     it.hk = w - slot * p.hkv;
     const int b = seq_of_slot(p.cu_q, p.num_seqs, p.chunk, slot);
-    if (b >= p.num_seqs) return false;
+    if (b < 0 || b >= p.num_seqs) return false;
     const Seq s = seq_of(p, b);
     int first, last;
-    sink_queries(p, s, p.chunk, slot - (p.cu_q[b] / p.chunk + b), first, last);
+    sink_queries(p, s, p.chunk, slot - first_slot(p.cu_q, b, p.chunk), first, last);
     if (last <= first) return false;
     it.key = s.k0;
     it.nk = min(p.sinks, s.lk);
@@ -530,16 +530,17 @@ __device__ __forceinline__ bool kv_item(const WindowBwdParams& p, int w, int D, 
   it.hk = w - slot * p.hkv;
   const int b = seq_of_slot(p.cu_k, p.num_seqs, 128, slot);
   const Seq s = seq_of(p, b);
-  it.j0 = (slot - (p.cu_k[b] / 128 + b)) * 128;
+  const bool real = b >= 0 && b < p.num_seqs;
+  it.j0 = (slot - first_slot(p.cu_k, b, 128)) * 128;
   if (it.j0 < 0 || it.j0 >= s.lk) return false;
   it.key = s.k0 + it.j0;
   it.nk = min(128, s.lk - it.j0);
   int first = 0, last = 0;
-  if (b < p.num_seqs) window_queries(p, s, it.j0, it.nk, first, last);
+  if (real) window_queries(p, s, it.j0, it.nk, first, last);
   it.tok = s.q0 + first;
   it.ntok = last - first;
   it.pos = first + s.lk - s.lq;
-  if (it.j0 == 0 && p.sinks > 0 && b < p.num_seqs) it.part = p.part0 + (long long)(b * p.hkv + it.hk) * row;
+  if (it.j0 == 0 && p.sinks > 0 && real) it.part = p.part0 + (long long)(b * p.hkv + it.hk) * row;
   return true;
 }
 
@@ -964,7 +965,7 @@ __global__ void __launch_bounds__(4 * 2 * D) sink_sum_kernel(const WindowBwdPara
   const Seq s = seq_of(p, b);
   if (j >= min(p.sinks, s.lk)) return;
   const long long row = (long long)p.sinks * 2 * D;
-  const int slot0 = p.cu_q[b] / p.chunk + b;
+  const int slot0 = first_slot(p.cu_q, b, p.chunk);
   float a = 0.f;
   for (int c = threadIdx.y; c * p.chunk < s.lq; c += 4) {
     int first, last;

@@ -39,15 +39,16 @@ struct WindowParams {
   int* err;
 };
 
-// One sequence's tokens.  Index num_seqs stands for the tokens after the last
-// sequence, which see and are seen by nothing (their outputs are zero).
+// One sequence's tokens.  Index -1 stands for the tokens before the first
+// sequence and num_seqs for those after the last one, which see and are seen by
+// nothing (their outputs are zero).
 struct Seq {
   int q0, lq, k0, lk;
 };
 
 __device__ __forceinline__ Seq seq_of(const WindowParams& p, int b) {
-  const bool tail = b >= p.num_seqs;
-  int q0 = p.cu_q[b], k0 = p.cu_k[b];
+  const bool head = b < 0, tail = b >= p.num_seqs;
+  int q0 = head ? 0 : p.cu_q[b], k0 = head ? 0 : p.cu_k[b];
   int q1 = tail ? p.total_q : p.cu_q[b + 1], k1 = tail ? p.total_k : p.cu_k[b + 1];
   // offsets outside the tensors or out of order: report and touch nothing
   if (q0 < 0 || q1 < q0 || q1 > p.total_q || k0 < 0 || k1 < k0 || k1 > p.total_k) {
@@ -58,17 +59,20 @@ __device__ __forceinline__ Seq seq_of(const WindowParams& p, int b) {
 }
 
 // Tiles of `rows` tokens of ragged sequences: sequence b's tiles start at slot
-// cu[b] / rows + b, which leaves each sequence at least as many slots as it
-// has tiles; total / rows + num_seqs + 1 slots cover all, the tail's included.
+// cu[b] / rows + b + 1 (those of the tokens before the first one at slot 0),
+// which leaves each as many slots as it has tiles; total / rows + num_seqs + 2
+// slots cover all, the tokens after the last sequence included.
 __host__ __device__ __forceinline__ int tile_slots(int total, int num_seqs, int rows) {
-  return total / rows + num_seqs + 1;
+  return total / rows + num_seqs + 2;
 }
 
+__device__ __forceinline__ int first_slot(const int32_t* cu, int b, int rows) { return b < 0 ? 0 : cu[b] / rows + b + 1; }
+
 __device__ __forceinline__ int seq_of_slot(const int32_t* cu, int num_seqs, int rows, int slot) {
-  int lo = 0, hi = num_seqs;  // the last sequence whose first slot is <= slot
+  int lo = -1, hi = num_seqs;  // the last index whose first slot is <= slot
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (cu[mid] / rows + mid <= slot) lo = mid;
+    if (first_slot(cu, mid, rows) <= slot) lo = mid;
     else hi = mid - 1;
   }
   return lo;

@@ -287,12 +287,12 @@ __device__ __forceinline__ bool row_item(const WindowParams& p, int w, int tt, R
   it.hk = w - slot * p.hkv;
   const int b = seq_of_slot(p.cu_q, p.num_seqs, 2 * tt, slot);
   const Seq s = seq_of(p, b);
-  const int i0 = (slot - (p.cu_q[b] / (2 * tt) + b)) * 2 * tt;
+  const int i0 = (slot - first_slot(p.cu_q, b, 2 * tt)) * 2 * tt;
   if (i0 < 0 || i0 >= s.lq) return false;
   it.tok = s.q0 + i0;
   it.n[0] = min(tt, s.lq - i0);
   it.n[1] = max(0, min(tt, s.lq - i0 - tt));
-  it.lk = b < p.num_seqs ? s.lk : 0;
+  it.lk = b >= 0 && b < p.num_seqs ? s.lk : 0;
   it.pos = i0 + s.lk - s.lq;
   it.key0 = s.k0;
   int lo[2], hi[2], sink[2], first = 0x7fffffff, end = 0, top = 0;

@@ -130,7 +130,7 @@ def window_sink_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, window: i
     * symmetric: |pos - j| <= window // 2 or j < sinks (``sliding_window_attention``'s
       band, with sinks)
 
-    A query that sees nothing gives 0.  Differentiable in q, k and v.  With
+    A query that sees nothing gives 0, and so do tokens outside the sequences.  Differentiable in q, k and v.  With
     ``return_lse`` also the natural-log LSE [Hq, Nq] fp32.  A value that is no
     finite number stays within its sequence, where it may reach queries that do
     not see it (0 times it, in a shared tile of keys)."""

@@ -1,0 +1,56 @@
+"""Windowed attention with sinks where the sequences do not fill the tensors, at
+strides that are no multiple of a head, with no queries or no keys."""
+
+import math
+
+import pytest
+import torch
+
+from tests import window_oracle as oracle
+from tests.test_gpu_window_attn import _check, _cu, _inputs, _run
+
+pytestmark = pytest.mark.gpu
+
+NAMES = ("out", "dq", "dk", "dv")
+
+
+def _poison():
+    """Memory that the allocator hands out next holds NaN."""
+    for n in (1 << 12, 1 << 16, 1 << 20, 1 << 23):
+        del_me = [torch.full((n,), math.nan, device="cuda") for _ in range(8)]
+        del del_me
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d,hq,hkv", [(32, 16, 1), (64, 4, 2), (128, 2, 2)])
+@pytest.mark.parametrize("lead_q,lead_k,trail", [(1, 1, 0), (64, 64, 3), (130, 130, 70), (300, 17, 0), (17, 300, 1), (0, 5, 0)])
+def test_tokens_before_the_first_sequence(causal, d, hq, hkv, lead_q, lead_k, trail):
+    """They get zero outputs and gradients, and what they hold (NaN, infinities) reaches nothing."""
+    lens = [150, 0, 67]
+    n = sum(lens)
+    cu = _cu(lens)
+    q, _, _, do = _inputs(lead_q + n + trail, 1, hq, hkv, d, torch.bfloat16, seed=lead_q)
+    _, k, v, _ = _inputs(1, lead_k + n + trail, hq, hkv, d, torch.bfloat16, seed=lead_k + 1)
+    for t, lead in ((q, lead_q), (do, lead_q), (k, lead_k), (v, lead_k)):
+        t[:lead] = math.nan
+        t[1:lead:3] = math.inf
+        t[lead + n:] = math.nan
+    _poison()
+    got = _run(q, k, v, do, cu + lead_q, cu + lead_k, window=40, sinks=3, causal=causal)
+    sq, sk = slice(lead_q, lead_q + n), slice(lead_k, lead_k + n)
+    ref = oracle.attention(q[sq], k[sk], v[sk], cu, cu, 40, 3, causal, dout=do[sq], bounds=True)
+    _check({x: got[x][sq if x in ("out", "dq") else sk] for x in NAMES}, ref, NAMES)
+    for x in NAMES:
+        s = sq if x in ("out", "dq") else sk
+        assert (got[x][:s.start] == 0).all() and (got[x][s.stop:] == 0).all(), x
+    assert (got["lse"][:lead_q] == -math.inf).all()
+
+
+def test_no_sequence_at_all():
+    """Offsets of no sequence: every token is outside."""
+    for at in (0, 30, 77):
+        cu = torch.tensor([at], dtype=torch.int32, device="cuda")
+        q, k, v, do = _inputs(77, 77, 2, 1, 64, torch.bfloat16)
+        _poison()
+        got = _run(q, k, v, do, cu, cu, window=8, sinks=2, causal=True)
+        assert all((got[x] == 0).all() for x in NAMES)
