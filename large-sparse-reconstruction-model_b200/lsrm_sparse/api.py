@@ -130,7 +130,9 @@ def window_sink_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, window: i
     * symmetric: |pos - j| <= window // 2 or j < sinks (``sliding_window_attention``'s
       band, with sinks)
 
-    A query that sees nothing gives 0, and so do tokens outside the sequences.  Differentiable in q, k and v.  With
+    A query that sees nothing gives 0, and so do tokens outside the sequences.
+    ``sinks`` is at most 128, Hq at most 64 times Hkv; ``softmax_scale`` None or 0
+    selects 1 / sqrt(D), a negative one is refused.  Differentiable in q, k and v.  With
     ``return_lse`` also the natural-log LSE [Hq, Nq] fp32.  A value that is no
     finite number stays within its sequence, where it may reach queries that do
     not see it (0 times it, in a shared tile of keys)."""
@@ -147,7 +149,8 @@ def window_sink_decode(q, k_new, v_new, k_cache, v_cache, lengths, *, window: in
     capacity >= sinks + window, lengths [B] int32 (tokens before the new one;
     negative: an idle row).  Writes the new key and value to their slot (position
     j lives in slot j below ``sinks``, else in sinks + (j - sinks) % (capacity -
-    sinks)) and returns the attention's output [B, Hq, D].  ``lengths`` is not
+    sinks)) and returns the attention's output [B, Hq, D].  ``sinks`` has no limit
+    here; ``softmax_scale`` as in ``window_sink_attention``.  ``lengths`` is not
     advanced.  Not differentiable."""
     with torch.no_grad():
         return ops.window_decode(q, k_new, v_new, k_cache, v_cache, lengths, window, sinks, softmax_scale)

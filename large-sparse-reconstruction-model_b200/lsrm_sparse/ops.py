@@ -460,6 +460,14 @@ def _need(cond: bool, msg: str):
         raise ValueError(msg)
 
 
+def _scale(name: str, scale) -> float:
+    """What the entry points take for ``softmax_scale``: None and 0 select 1/sqrt(head_dim)."""
+    if not scale:
+        return 0.0
+    _need(2.0**-126 <= scale < 2.0**127, f"{name}: softmax_scale ({scale}) must be positive and finite in 32 bits")
+    return float(scale)
+
+
 def _cuda(name: str, *ts):
     """All tensors (None passes) on one CUDA device, which is returned."""
     dev = None
@@ -513,7 +521,7 @@ def _window_shape(q, k, v, cu_q, window, sinks, causal, scale):
     v, vs = _token_rows(v)
     sh = _lib.WindowShape(cu_q.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2],
                           _dtype_code(q), min(int(window), 2**31 - 1), int(sinks), int(bool(causal)), qs, ks, vs,
-                          float(scale) if scale else 0.0)
+                          _scale("window_sink_attention", scale))
     return sh, q, k, v
 
 
@@ -588,7 +596,7 @@ def window_decode(q, k_new, v_new, k_cache, v_cache, lengths, window: int, sinks
     (q, qs), (k_new, ks), (v_new, vs) = _token_rows(q), _token_rows(k_new), _token_rows(v_new)
     lengths = lengths.contiguous()
     sh = _lib.WindowDecodeShape(b, q.shape[1], hkv, d, _dtype_code(q), k_cache.shape[1], min(int(window), 2**31 - 1),
-                                int(sinks), qs, ks, vs, *strides, float(softmax_scale) if softmax_scale else 0.0)
+                                int(sinks), qs, ks, vs, *strides, _scale(name, softmax_scale))
     out = torch.empty(b, q.shape[1], d, dtype=q.dtype, device=dev)
     _run(dev, "lsrm_window_decode", ctypes.byref(sh), _addr(q), _addr(k_new), _addr(v_new), _addr(k_cache),
          _addr(v_cache), _addr(lengths), _addr(out))

@@ -54,3 +54,18 @@ def test_no_sequence_at_all():
         _poison()
         got = _run(q, k, v, do, cu, cu, window=8, sinks=2, causal=True)
         assert all((got[x] == 0).all() for x in NAMES)
+
+
+def test_softmax_scale_refusals():
+    from lsrm_sparse import api
+
+    q, k, v, _ = _inputs(64, 64, 4, 2, 64, torch.bfloat16)
+    kc, vc = (torch.zeros(64, 10, 2, 64, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    ln = torch.zeros(64, dtype=torch.int32, device="cuda")
+    for scale in (-0.125, math.nan, math.inf):
+        with pytest.raises(ValueError, match="softmax_scale"):
+            api.window_sink_attention(q, k, v, _cu([64]), window=8, softmax_scale=scale)
+        with pytest.raises(ValueError, match="softmax_scale"):
+            api.window_sink_decode(q, k, v, kc, vc, ln, window=8, softmax_scale=scale)
+    a = api.window_sink_attention(q, k, v, _cu([64]), window=8)
+    assert torch.equal(a, api.window_sink_attention(q, k, v, _cu([64]), window=8, softmax_scale=0.0))
