@@ -13,8 +13,10 @@ to it: a block's first act is ``residual_rms_norm(branch, stream)``, which adds
 of the step's seed and the place in the stack, so activation recomputation and
 the backward see the forward's masks.  ``quantize_()`` turns the Linears that
 follow a norm into 8-bit ones (e4m3 weights and activations, a scale per row)
-for inference: the norm then writes their operand in 8 bits directly.  The
-Linears themselves are library GEMMs, as in the decoder.
+for inference: the norm then writes their operand in 8 bits directly.  Such a
+stack takes no dropout and no gradient: its parameters are frozen, and a
+backward pass through it raises.  The Linears themselves are library GEMMs, as
+in the decoder.
 """
 
 from __future__ import annotations
@@ -42,9 +44,23 @@ class Linear8(nn.Module):
         self.bias = linear.bias
 
     def forward(self, values, scales, dtype):
+        # bf16 whatever ``dtype``: the library's fp16 form with a scale per row gives wrong products, and next to
+        # e4m3's rounding (2^-4) bf16's (2^-9) is small
         y = torch._scaled_mm(values, self.weight.t(), scale_a=scales, scale_b=self.scale, out_dtype=torch.bfloat16)
         y = y.to(dtype)
         return y if self.bias is None else y + self.bias
+
+
+class _NoGradient(torch.autograd.Function):
+    """``t``, behind the ``sources`` that no gradient reaches."""
+
+    @staticmethod
+    def forward(ctx, t, *sources):
+        return t.view_as(t)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("8-bit Linears are for inference: no gradient passes through the norm in front of them")
 
 
 class WindowCache:
@@ -89,13 +105,17 @@ class WindowBlock(nn.Module):
 
     def quantize_(self):
         self.qkv, self.fc1 = Linear8(self.qkv), Linear8(self.fc1)
-        return self
+        return self.requires_grad_(False)
 
     def _norm_linear(self, branch, stream, weight, linear, p, seed, offset):
         """(linear(norm(stream + dropout(branch))), the new stream)."""
         if isinstance(linear, Linear8):
-            values, scales, stream = api.residual_rms_norm_8bit(branch, stream, weight, eps=self.eps)
-            return linear(values, scales, branch.dtype), stream
+            if p:
+                raise ValueError("8-bit Linears are for inference: the norm in front of them has no dropout (call eval())")
+            values, scales, h = api.residual_rms_norm_8bit(branch, stream, weight, eps=self.eps)
+            if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (branch, stream)):
+                h = _NoGradient.apply(h, branch, stream)
+            return linear(values, scales, branch.dtype), h
         y, stream = api.residual_rms_norm(branch, stream, weight, eps=self.eps, p=p, seed=seed, offset=offset)
         return linear(y), stream
 

@@ -64,3 +64,68 @@ def test_idle_rows_stay_idle():
     ref = _reference(stack, full[1, 6:7], torch.tensor([0, 1], dtype=torch.int32, device="cuda"))
     assert lengths.tolist() == [7, 1, 7]
     assert (y[1:2].double() - ref).norm() <= 10 * 2.0**-8 * ref.norm()
+
+
+def test_8bit_stack_takes_no_gradient():
+    """A backward pass raises where it would leave gradients out; without one the stack runs in any mode."""
+    stack = _stack().quantize_()
+    cu = torch.tensor([0, 64, 100], dtype=torch.int32, device="cuda")
+    x = torch.randn(100, 256, device="cuda").bfloat16()
+    with torch.no_grad():
+        ref = stack(x, cu)
+    y = stack(x, cu)  # training mode without dropout; only the final norm's weight takes a gradient
+    assert torch.equal(y.detach(), ref)
+    y.float().sum().backward()
+    assert stack.norm.grad is not None and stack.norm.grad.abs().sum() > 0
+    leaf = x.clone().requires_grad_()
+    y = stack(leaf, cu)
+    assert torch.equal(y.detach(), ref)
+    with pytest.raises(RuntimeError, match="inference"):
+        y.float().sum().backward()
+
+
+def test_8bit_stack_takes_no_dropout():
+    stack = _stack(dropout=0.2).quantize_()
+    cu = torch.tensor([0, 100], dtype=torch.int32, device="cuda")
+    x = torch.randn(100, 256, device="cuda").bfloat16()
+    with torch.no_grad(), pytest.raises(ValueError, match="dropout"):
+        stack(x, cu, seed=1)
+    with torch.no_grad():
+        stack.eval()(x, cu)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_linear8_is_the_product_of_its_operands(dtype):
+    """Linear8 against the 64-bit product of the numbers that its 8-bit operands stand for: one rounding to bf16 (and one
+    to fp16), sums of 512 products in 32 bits; and the weights within half a step of the Linear's."""
+    from lsrm_sparse import api
+    from lsrm_sparse.window_block import Linear8
+
+    g = torch.Generator(device="cuda").manual_seed(5)
+    lin = torch.nn.Linear(512, 192, device="cuda", dtype=dtype)
+    lin8 = Linear8(lin)
+    x = torch.randn(70, 512, device="cuda", generator=g).to(dtype)
+    values, scales, _ = api.residual_rms_norm_8bit(x, None, None)
+    with torch.no_grad():
+        y = lin8(values, scales, dtype)
+    a = values.double() * scales.double()
+    w = lin8.weight.double() * lin8.scale.double().t()
+    assert ((w - lin.weight.double()).abs() <= 2.0**-4 * lin.weight.double().abs() + 2.0**-10 * lin8.scale.double().t()).all()
+    bias = lin.bias.detach().double()
+    ref = a @ w.t()
+    # the product's rounding, then the sum's with the bias (both at most 2^-8, bf16)
+    bound = 2.0**-8 * (ref.abs() + (ref + bias).abs()) + 2.0**-12 * (a.abs() @ w.abs().t()) + 2.0**-25
+    assert y.dtype == dtype and ((y.double() - ref - bias).abs() <= bound).all()
+
+
+def test_8bit_stack_error_is_the_formats():
+    """e4m3 is off by at most 2^-4 of a value, 2^-4 / sqrt(3) in the mean square, and so is a long product of two such
+    operands by sqrt(2) of that; four of them on branches no larger than the stream add in quadrature, next to ten 16-bit roundings."""
+    stack = _stack().eval()
+    cu = torch.tensor([0, 64, 160], dtype=torch.int32, device="cuda")
+    x = torch.randn(160, 256, device="cuda").bfloat16()
+    ref = _reference(stack, x, cu)
+    with torch.no_grad():
+        y = stack.quantize_()(x, cu)
+    bound = 4**0.5 * 2**0.5 * 2.0**-4 / 3**0.5 + 10 * 2.0**-8
+    assert (y.double() - ref).norm() <= bound * ref.norm()
