@@ -104,7 +104,8 @@ class WindowBlock(nn.Module):
         self.fc1, self.act, self.fc2 = nn.Linear(dim, int(dim * mlp_ratio)), act_layer(), nn.Linear(int(dim * mlp_ratio), dim)
 
     def quantize_(self):
-        self.qkv, self.fc1 = Linear8(self.qkv), Linear8(self.fc1)
+        if not isinstance(self.qkv, Linear8):
+            self.qkv, self.fc1 = Linear8(self.qkv), Linear8(self.fc1)
         return self.requires_grad_(False)
 
     def _norm_linear(self, branch, stream, weight, linear, p, seed, offset):

@@ -53,3 +53,11 @@ def test_symmetric_stacks_have_no_single_token_form():
                  lambda: stack.step(x[:1], caches, torch.zeros(1, dtype=torch.int32))):
         with pytest.raises(ValueError, match="causal"):
             call()
+
+
+def test_quantize_twice():
+    stack = WindowStack(2, 64, 2, 1, window=4).quantize_()
+    before = [b.clone() for b in stack.buffers()]
+    stack.quantize_()
+    assert len(before) == 8 and all(torch.equal(a.float(), b.float()) for a, b in zip(before, stack.buffers()))
+    assert [n for n, p in stack.named_parameters() if p.requires_grad] == ["norm"]
