@@ -134,7 +134,7 @@ class WindowBlock(nn.Module):
         the next (branch, stream).  ``site`` counts the stack's dropout sites."""
         if cache is not None:
             self._check_causal()
-        p = self.dropout if self.training else 0.0
+        p = self.dropout if self.training and cache is None else 0.0
         qkv, stream = self._norm_linear(branch, stream, self.norm_attn, self.qkv, 0.0 if first else p, seed,
                                         site * _SITE)
         q, k, v = self._split(qkv)
@@ -176,11 +176,12 @@ class WindowStack(nn.Module):
 
     def forward(self, x, cu_seqlens, seed: int = 0, caches: Optional[List[WindowCache]] = None):
         """x [N, dim] of sequences at cu_seqlens (int32).  ``seed`` picks the
-        step's dropout masks; ``caches`` are filled for ``step``."""
+        step's dropout masks; ``caches`` are filled for ``step`` (which, like it,
+        takes no dropout in any mode)."""
         branch, stream = x, None
         for i, b in enumerate(self.blocks):
             branch, stream = b(branch, stream, cu_seqlens, seed, 3 * i, i == 0, caches[i] if caches else None)
-        p = self.blocks[0].dropout if self.training else 0.0
+        p = self.blocks[0].dropout if self.training and not caches else 0.0
         return api.residual_rms_norm(branch, stream, self.norm, eps=self.eps, p=p, seed=seed,
                                      offset=3 * len(self.blocks) * _SITE)[0]
 

@@ -129,3 +129,15 @@ def test_8bit_stack_error_is_the_formats():
         y = stack.quantize_()(x, cu)
     bound = 4**0.5 * 2**0.5 * 2.0**-4 / 3**0.5 + 10 * 2.0**-8
     assert (y.double() - ref).norm() <= bound * ref.norm()
+
+
+def test_prefill_takes_no_dropout():
+    """As step: whatever the mode, the prompt's outputs and caches are those of the stack without dropout."""
+    stack = _stack(dropout=0.3).train()
+    cu = torch.tensor([0, 40], dtype=torch.int32, device="cuda")
+    x = torch.randn(40, 256, device="cuda").bfloat16()
+    y, caches, _ = stack.prefill(x, cu)
+    ref, want, _ = stack.eval().prefill(x, cu)
+    assert torch.equal(y, ref)
+    for a, b in zip(caches, want):
+        assert torch.equal(a.k[:, :27], b.k[:, :27]) and torch.equal(a.v[:, :27], b.v[:, :27])
