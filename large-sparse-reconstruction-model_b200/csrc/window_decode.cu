@@ -131,9 +131,10 @@ __global__ void __launch_bounds__(kDcThreads) window_decode_kernel(const DecodeP
   uint16_t* out = static_cast<uint16_t*>(p.out) + ((long long)b * p.hq + h0) * D;
 
   // visible positions, numbered 0 .. cnt - 1: the sinks, then the window's; the last one is the new token
-  const int sink = n < 0 ? 0 : min(p.sinks, n + 1);
+  // (n itself may be the largest int: no n + 1)
+  const int sink = n < 0 ? 0 : n < p.sinks ? n + 1 : p.sinks;
   const int lo = max(p.sinks, n - p.window + 1);
-  const int cnt = n < 0 ? 0 : sink + max(0, n + 1 - lo);
+  const int cnt = n < 0 ? 0 : sink + (n < lo ? 0 : n - lo + 1);
   const int first_slot = lo > p.sinks ? (lo - p.sinks) % ring : 0;  // the window's first position in the ring
   auto slot_of = [&](int i) {
     if (i < sink) return i;

@@ -69,3 +69,23 @@ def test_softmax_scale_refusals():
             api.window_sink_decode(q, k, v, kc, vc, ln, window=8, softmax_scale=scale)
     a = api.window_sink_attention(q, k, v, _cu([64]), window=8)
     assert torch.equal(a, api.window_sink_attention(q, k, v, _cu([64]), window=8, softmax_scale=0.0))
+
+
+@pytest.mark.parametrize("window,sinks,slack", [(1, 0, 0), (16, 4, 3), (200, 1, 0)])
+def test_decode_at_the_largest_lengths(window, sinks, slack):
+    from lsrm_sparse import api
+    from tests.test_gpu_window_attn import _decode_ref
+
+    g = torch.Generator(device="cuda").manual_seed(2)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g).bfloat16()  # noqa: E731
+    cap = sinks + window + slack
+    q, kn, vn, kc, vc = r(3, 4, 64), r(3, 2, 64), r(3, 2, 64), r(3, cap, 2, 64), r(3, cap, 2, 64)
+    ln = torch.tensor([2**31 - 1, 2**31 - 2, 2**30], dtype=torch.int32, device="cuda")
+    kr, vr = kc.clone(), vc.clone()
+    # the oracle counts positions one by one: the same slots as at lengths a whole number of rings smaller
+    ring = cap - sinks
+    small = torch.tensor([sinks + window + (n - sinks - window) % ring for n in ln.tolist()], device="cuda")
+    out = api.window_sink_decode(q, kn, vn, kc, vc, ln, window=window, sinks=sinks)
+    ref, bound = _decode_ref(q, kn, vn, kr, vr, small, window, sinks)
+    assert torch.equal(kc, kr) and torch.equal(vc, vr)
+    assert ((out.double() - ref).abs() <= bound).all()
