@@ -961,7 +961,7 @@ __global__ void __launch_bounds__(kKvThreads, 1)
 template <typename T, int D>
 __global__ void __launch_bounds__(4 * 2 * D) sink_sum_kernel(const WindowBwdParams p) {
   __shared__ float sum[4][2 * D];
-  const int j = blockIdx.x, hk = blockIdx.y, b = blockIdx.z, e = threadIdx.x;
+  const int b = blockIdx.x, hk = blockIdx.y, j = blockIdx.z, e = threadIdx.x;
   const Seq s = seq_of(p, b);
   if (j >= min(p.sinks, s.lk)) return;
   const long long row = (long long)p.sinks * 2 * D;
@@ -1060,7 +1060,7 @@ int launch_bwd(const WindowBwdParams& p, cudaStream_t s) {
     }
     if (p.chunk) {
       ProfScope ps("window_attn_sinks", s);
-      sink_sum_kernel<T, D><<<dim3(p.sinks, p.hkv, p.num_seqs), dim3(2 * D, 4), 0, s>>>(p);
+      sink_sum_kernel<T, D><<<dim3(p.num_seqs, p.hkv, p.sinks), dim3(2 * D, 4), 0, s>>>(p);
       LSRM_LAUNCH_CHECK();
     }
   }
@@ -1092,7 +1092,6 @@ extern "C" int lsrm_window_attn_bwd(const lsrm_window_shape* shape, const int32_
                  "out, lse, dout and the gradients must not be NULL");
   LSRM_CHECK_ARG((((uintptr_t)out | (uintptr_t)out_rest | (uintptr_t)dout | (uintptr_t)dq | (uintptr_t)dk |
                    (uintptr_t)dv) & 15) == 0, "out, out_rest, dout and the gradients must be 16-byte aligned");
-  LSRM_CHECK_ARG(shape->num_seqs <= 65535, "at most 65535 sequences");
   if (!workspace || workspace_bytes < lsrm_window_attn_workspace_bytes(shape)) {
     set_error("workspace too small: %zu bytes, %zu needed", workspace_bytes, lsrm_window_attn_workspace_bytes(shape));
     return LSRM_ERR_WORKSPACE;

@@ -89,3 +89,18 @@ def test_decode_at_the_largest_lengths(window, sinks, slack):
     ref, bound = _decode_ref(q, kn, vn, kr, vr, small, window, sinks)
     assert torch.equal(kc, kr) and torch.equal(vc, vr)
     assert ((out.double() - ref).abs() <= bound).all()
+
+
+def test_more_sequences_than_a_grid_dimension():
+    """70001 sequences of one token, each its own sink: out = v, dv = do, and the scores' gradients cancel."""
+    n, hq, hkv, d = 70001, 2, 1, 32
+    cu = torch.arange(n + 1, device="cuda", dtype=torch.int32)
+    q, k, v, do = _inputs(n, n, hq, hkv, d, torch.bfloat16, seed=14)
+    _poison()
+    got = _run(q, k, v, do, cu, cu, window=4, sinks=1, causal=True)
+    assert torch.equal(got["out"], v.expand(n, hq, d))
+    # a sum of two 16-bit values, rounded once
+    assert torch.equal(got["dv"], do.float().sum(1, keepdim=True).bfloat16())
+    big = (do.double().abs() * v.double().abs()).sum(2).amax(1, keepdim=True)[..., None] * d**-0.5 * 2.0**-14
+    assert (got["dq"].double().abs() <= big * k.double().abs()).all()
+    assert (got["dk"].double().abs() <= hq * big * q.double().abs().amax(1, keepdim=True)).all()
