@@ -104,3 +104,64 @@ def test_more_sequences_than_a_grid_dimension():
     big = (do.double().abs() * v.double().abs()).sum(2).amax(1, keepdim=True)[..., None] * d**-0.5 * 2.0**-14
     assert (got["dq"].double().abs() <= big * k.double().abs()).all()
     assert (got["dk"].double().abs() <= hq * big * q.double().abs().amax(1, keepdim=True)).all()
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(32, 6, 2), (64, 4, 4), (128, 3, 1)])
+def test_token_strides_that_are_no_multiple_of_a_head(d, hq, hkv):
+    """Rows padded by eight elements, and by a head and eight: the bits of contiguous tensors."""
+    cu = _cu([100, 1, 232])
+    q, k, v, do = _inputs(333, 333, hq, hkv, d, torch.bfloat16, seed=15)
+
+    def padded(t, pad):
+        n, h, _ = t.shape
+        return torch.full((n, h * d + pad), math.nan, device="cuda", dtype=t.dtype)[:, :h * d].unflatten(1, (h, d)).copy_(t)
+
+    a = _run(q, k, v, do, cu, cu, window=60, sinks=2, causal=True)
+    b = _run(padded(q, 8), padded(k, d + 8), padded(v, 24), padded(do, 8), cu, cu, window=60, sinks=2, causal=True)
+    assert all(torch.equal(a[x], b[x]) for x in a)
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(32, 8, 1), (64, 4, 2), (128, 2, 2)])
+def test_no_queries_or_no_keys(d, hq, hkv):
+    """One side empty: the other side's outputs and gradients are zero."""
+    zero, some = _cu([0, 0]), _cu([70, 61])
+    for cu_q, cu_k in ((zero, some), (some, zero)):
+        nq, nk = int(cu_q[-1]), int(cu_k[-1])
+        q, k, v, do = _inputs(nq, nk, hq, hkv, d, torch.float16, seed=16)
+        _poison()
+        got = _run(q, k, v, do, cu_q, cu_k, window=8, sinks=2, causal=False)
+        assert all((got[x] == 0).all() for x in NAMES)
+        assert got["dk"].shape[0] == nk and got["out"].shape[0] == nq
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_delta_does_not_inherit_the_outputs_rounding(dtype):
+    """Keys and values around a large common one, nearly uniform rows of a hundred keys and more: the rounding of the
+    output then moves delta, and with it dq, by more than everything else does.  The 64-bit error of a delta from the
+    rounded output predicts the backward without what the rounding left over; with it the error is a small part of that:
+    p's roundings, which a row averages (1 / sqrt(100)), and ds's, which meet the values' spread (1/16) alone."""
+    from lsrm_sparse import ops
+
+    n, hq, hkv, d, window = 600, 4, 2, 64, 300
+    g = torch.Generator(device="cuda").manual_seed(17)
+    r = lambda h: torch.randn(n, h, d, device="cuda", generator=g)  # noqa: E731
+    q, k, v, do = ((0.3 * r(hq)).to(dtype), (1 + 0.3 * r(hkv)).to(dtype), (4 + 0.25 * r(hkv)).to(dtype), r(hq).to(dtype))
+    cu = _cu([n])
+    args = (cu, cu, window, 4, True)
+    ref = oracle.attention(q, k, v, cu, cu, window, 4, True, dout=do)
+    out, lse, rest = ops.window_attn_fwd(q, k, v, *args, need_rest=True)
+    # what an error of delta does to dq: - scale * error * sum_j p_j k_j
+    vis = oracle.visible(n, n, window, 4, True, "cuda")
+    moved = torch.empty_like(ref["dq"])
+    off = (do.double() * (ref["out"].to(dtype).double() - ref["out"])).sum(2)
+    for h in range(hq):
+        s = (q[:, h].double() @ k[:, h // 2].double().T * d**-0.5).masked_fill(~vis, -math.inf)
+        moved[:, h] = -d**-0.5 * off[:, h, None] * (torch.softmax(s, 1) @ k[:, h // 2].double())
+    rows = slice(100, None)  # a hundred keys at least
+    err = {}
+    for name, left in (("without", None), ("with", rest)):
+        dq, dk, dv = ops.window_attn_bwd(q, k, v, out, left, lse, do, *args)
+        err[name] = (dq.double() - ref["dq"])[rows].norm().item()
+    predicted = moved[rows].norm().item()
+    assert 0.7 * predicted <= err["without"] <= 1.4 * predicted
+    assert err["with"] <= 0.35 * predicted
