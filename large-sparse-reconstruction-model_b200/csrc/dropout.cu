@@ -2,12 +2,14 @@
 // Philox word (philox.cuh) is kept, else 0.  The backward pass is the same
 // call on the gradient.  A thread takes eight elements (two counter blocks).
 //
-// Bound by the 32 x 32 bit products rather than by HBM: 36 of them per eight
-// elements, four cycles a warp on their pipe.  537 million elements: bf16 486 us
-// (4.4 TB/s), fp16 471; a plain copy 329.  Of 475 us before the products went to
-// 32 bits: 340 without the generator's last seven rounds, 437 without the
-// memory.  Loading an iteration ahead does not help: the warps that are
-// resident hide the loads.
+// Bound by the generator's arithmetic, not by HBM.  537 million elements: bf16
+// 486 us (4.4 TB/s), fp16 471, fp32 (half as many) 415; a plain copy 329.  The
+// 36 products of eight elements, four cycles a warp, are 260 us of that, and the
+// logical operations beside them fill the other pipe: ALU 58 % of the cycles,
+// FMA 43 %, issue slots 62 %, DRAM 41 % (67 million elements); the warps wait
+// for a math pipe first.  Of 475 us before the scaling went to 32 bits: 340
+// without the generator's last seven rounds, 437 without the memory.  Loading an
+// iteration ahead does not help: the warps that are resident hide the loads.
 #include <algorithm>
 
 #include "host_util.h"

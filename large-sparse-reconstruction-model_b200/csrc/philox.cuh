@@ -8,7 +8,7 @@
 // `seed`, and is kept when the word is >= threshold = floor(p * 2^32).
 //
 // The rounds bound a dropout that streams through HBM (18 products, 36 logical
-// operations per four elements), so what does not change from block to block is
+// operations per four elements, which keep two pipes busier than DRAM), so what does not change from block to block is
 // taken out of them: the round keys come from the host as constants, and of a
 // counter (low, high, 0, 0) the first round needs one product and the second
 // one has one operand that depends on the upper word alone.

@@ -8,11 +8,19 @@
 //   dresidual = dh_total, dx = drop(dh_total), dw_c = sum_rows dy * h * r
 // where drop regenerates the forward's mask from its counter (philox.cuh).
 //
-// All passes are bound by HBM (with dropout, by the generator's products beside
-// it): 131072 x 1024 bf16, forward 174 us without dropout and 229 with it (6.2 and
-// 4.7 TB/s), backward with dropout 302 us (4.4 TB/s); 16384 x 4096 to int8 103 us
-// and back 44 us (4.6 TB/s).  Every tensor is read or written once, a row stays in
-// registers between its statistics and its output.  A team of 32 to
+// The stored h is what the backward reads: its rounding to the stream's type
+// enters the gradients once (a 16-bit stream: error against 64 bits 0.0023 where
+// the results' own rounding is 0.0017); an fp32 h of its own, or x and the residual
+// once more, would be a tensor more to move.
+//
+// What bounds the passes.  131072 x 1024 bf16: forward 174 us without dropout
+// (6.2 TB/s, HBM: the warps wait for loads), 229 with it; backward 211 and 311
+// with dw's sum (5.1 and 4.3 TB/s); 16384 x 4096 to int8 104 us (4.5 TB/s) and
+// back 44.  In all but the first, instruction issue is busier than DRAM: issue
+// slots 65 % in the forward with dropout, 74 and 66 % in the backward, 76 % to
+// 8 bits, with DRAM at 51, 60, 51 and 51 % (65536 x 1024; 16384 x 4096).  Every
+// tensor is read or written once, a row stays in registers between its
+// statistics and its output.  A team of 32 to
 // 512 threads owns a row; a thread holds NV chunks of eight consecutive
 // elements.  Chunks are cut from the flat tensor (chunk = flat index / 8), so
 // that rows of any width use 16-byte accesses: a row that does not start or

@@ -327,9 +327,11 @@ template <int D, bool BF16>
 int launch_decode(const DecodeParams& p, cudaStream_t s) {
   const int blocks = (p.g + kDcRows - 1) / kDcRows;
   const long long ctas = (long long)p.batch * p.hkv * blocks;
-  // Cut a row's positions while the GPU has room for more CTAs (two a multiprocessor) and each keeps a stage; past that
-  // only long rows, whose ragged lengths then even out over a few rounds (64 sequences, window 8192, 8 kv heads: 332
-  // us at four cuts, 413 at one, 380 at eight; 16 sequences, window 1024, 16 kv heads of 64: 19 us at two, 35 at eight).
+  // Cut a row's positions while fewer than two CTAs a multiprocessor run and each keeps a stage; past that only long
+  // rows, whose ragged lengths then even out over a few rounds.  At one, two, four and eight cuts, * the rule's: 64
+  // sequences, window 8192, 8 kv heads of 128: 331, 322, 318*, 344 us; 16 sequences, window 1024, 16 kv heads of 64:
+  // 21.6, 15.1*, 16.6, 20.6; 32 of window 512: 14.6*, 16.1, 19.9, 31.8; one sequence, window 8192, 8 kv heads of 128: 188,
+  // 98, 52, 29.1* (34 MB, 5.2 us at a copy's rate: 64 CTAs with a stage each in flight do not fill HBM).
   const int stages = (int)((std::min<long long>((long long)p.window + p.sinks, p.capacity) + kDcKeys - 1) / kDcKeys);
   int splits = 1;
   while (splits < kDcMaxSplit && splits < stages &&

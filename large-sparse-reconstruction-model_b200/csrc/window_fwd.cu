@@ -17,8 +17,9 @@
 // heads of 64 channels, window 512, 766 us against 730).  S has two buffers of 64
 // columns a row tile and P lies over its S, so that the products of the tiles
 // before and after run under a tile's softmax.  Rounding: S, m, l and O are fp32;
-// P is rounded to the operand type (the sum l takes it unrounded), O once at the
-// end.
+// P is rounded to the operand type (the product's one choice; the sum l takes it
+// unrounded), O once at the end: error against 64 bits 0.0022 in bf16 at most, 0.0017
+// from O's rounding alone.
 //
 // What bounds it: 16384 tokens in two sequences, 32 / 8 heads of 128 channels,
 // causal window 2048: 530 us, 900 TFLOP/s (0.54 of the library's GEMM rate; 560 us

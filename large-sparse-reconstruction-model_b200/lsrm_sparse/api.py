@@ -132,10 +132,11 @@ def window_sink_attention(q, k, v, cu_seqlens_q, cu_seqlens_k=None, *, window: i
 
     A query that sees nothing gives 0, and so do tokens outside the sequences.
     ``sinks`` is at most 128, Hq at most 64 times Hkv; ``softmax_scale`` None or 0
-    selects 1 / sqrt(D), a negative one is refused.  Differentiable in q, k and v.  With
-    ``return_lse`` also the natural-log LSE [Hq, Nq] fp32.  A value that is no
-    finite number stays within its sequence, where it may reach queries that do
-    not see it (0 times it, in a shared tile of keys)."""
+    selects 1 / sqrt(D), a negative one is refused.  Differentiable in q, k and v
+    (the scores' gradients pass through the operand type: fp16 wants the usual
+    loss scale).  With ``return_lse`` also the natural-log LSE [Hq, Nq] fp32.  A
+    value that is no finite number stays within its sequence, where it may reach
+    queries that do not see it (0 times it, in a shared tile of keys)."""
     cu_k = cu_seqlens_q if cu_seqlens_k is None else cu_seqlens_k
     out, lse = F.window_sink_attention(q, k, v, cu_seqlens_q, cu_k, window, sinks, causal, softmax_scale)
     _raise_on_device_errors()
@@ -160,7 +161,9 @@ def dropout(x, p: float, seed: int, offset: int = 0):
     """Dropout whose mask is a function of (seed, offset, element index) and is
     never stored: the backward, or a second call, regenerates it.  Element e
     draws word e % 4 of the Philox4x32-10 block ``offset + e // 4``, so calls that
-    must differ take other seeds, or offsets that are numel / 4 apart.  p in [0, 1)."""
+    must differ take other seeds, or offsets at least ceil(numel / 4) apart.  p in
+    [0, 1).  Seed and offset are host integers: a captured CUDA graph replays the
+    masks of its capture, so a step that draws new ones is launched or captured anew."""
     if not 0.0 <= p < 1.0:
         raise ValueError(f"dropout: p ({p}) must be in [0, 1)")
     return F.dropout(x, float(p), seed, offset)
@@ -171,7 +174,8 @@ def residual_rms_norm(x, residual=None, weight=None, *, eps: float = 1e-6, p: fl
     """The step between a block's branches: h = residual + dropout(x) and
     y = h / sqrt(mean(h**2) + eps) * weight over the last dimension.  Returns
     (y, h): y in x's dtype, h in the residual's (x's or fp32).  Differentiable in
-    x, residual and weight; the dropout is ``dropout``'s, with its mask."""
+    x, residual and weight; the dropout is ``dropout``'s, with its mask (and its
+    host-side seed).  The backward reads h as it was stored."""
     if not 0.0 <= p < 1.0:
         raise ValueError(f"residual_rms_norm: p ({p}) must be in [0, 1)")
     return F.residual_rms_norm(x, residual, weight, float(eps), float(p), seed, offset)

@@ -75,7 +75,8 @@ class WindowCache:
     def fill(self, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor):
         """Keep what later tokens can see of packed prompts k / v [N, heads, head_dim].
         Tokens before the first and after the last sequence are padding, as in
-        ``window_sink_attention``."""
+        ``window_sink_attention``.  Selecting the tokens waits for the GPU, so a
+        prefill cannot be captured in a CUDA graph."""
         n = cu_seqlens.numel() - 1
         if n == 0:
             return
