@@ -40,8 +40,9 @@ namespace {
 constexpr int kNormMaxCols = 16384;  // 512 threads x 4 chunks x 8 elements
 constexpr int kRowWarps = 8;         // rows per block when a warp owns a row
 // Chunks a thread holds at most.  131072 x 1024 bf16, forward with dropout:
-// 264 us at one, 230 at two, 272 at four; backward 343, 388, 422 (three more
-// tensors in registers: rows in flight count for more than barriers saved).
+// 264 us at one, 230 at two, 272 at four; backward, before its loads went a row
+// ahead, 343, 388, 422 (three more tensors in registers: rows in flight count for
+// more than barriers saved).
 constexpr int kFwdChunks = 2, kBwdChunks = 1;
 
 struct NormParams {
