@@ -11,12 +11,11 @@
 //
 // Rounding: P and dS are rounded once to the operand type, everything else is
 // fp32.  The products take operands of one 16-bit type; the remainders would be two
-// more products, with operands in TMEM, which is full.  The gradients' error against 64 bits
-// grows by sqrt(2) over that of rounding the results (bf16 0.0024 for 0.0017, fp16
-// 0.0003 for 0.0002; up to 1.56 times in rows of a few keys, where P's rounding in
-// the output still shows in delta).  dS is not scaled: fp16 gradients of the output
-// far below 0.01 fall into the type's subnormal range there, so fp16 training wants
-// its usual loss scale.
+// more products, with operands in TMEM, which is full.  The gradients' error
+// against 64 bits grows by sqrt(2) over that of rounding the results (bf16 0.0024
+// for 0.0017, fp16 0.0003 for 0.0002).  dS is not scaled: fp16 gradients of the
+// output far below 0.01 fall into the type's subnormal range there, so fp16 training
+// wants its usual loss scale.
 //
 // Sinks are seen by every later query.  The key tile that holds them sums the
 // queries that its window reaches; the queries past it are cut into chunks

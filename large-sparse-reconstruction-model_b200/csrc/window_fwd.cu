@@ -17,9 +17,9 @@
 // heads of 64 channels, window 512, 766 us against 730).  S has two buffers of 64
 // columns a row tile and P lies over its S, so that the products of the tiles
 // before and after run under a tile's softmax.  Rounding: S, m, l and O are fp32;
-// P is rounded to the operand type (the product's one choice; the sum l takes it
-// unrounded), O once at the end: error against 64 bits 0.0022 in bf16 at most, 0.0017
-// from O's rounding alone.
+// P is rounded to the operand type (the sum l takes it unrounded, and rows of few
+// keys keep the remainder: few_keys), O once at the end.  Error against 64 bits 0.0023
+// in bf16 at most, 0.0017 from O's rounding alone.
 //
 // What bounds it: 16384 tokens in two sequences, 32 / 8 heads of 128 channels,
 // causal window 2048: 530 us, 900 TFLOP/s (0.54 of the library's GEMM rate; 560 us
@@ -42,6 +42,21 @@ namespace {
 constexpr int kFwThreads = 352;
 constexpr int kFwKeys = 64;
 
+// Rows that see at most this many keys (one tile) enter the product with P and
+// with what P's rounding left over: over a few keys the roundings do not average,
+// and through the output they move delta, which showed in dq and dk (error against
+// 64 bits up to 1.56 times a 32-bit form's; with the remainder, as in longer rows,
+// sqrt(2) from dS alone, and a little).  It costs such a forward 18 % (131072 tokens,
+// 16 heads of 64 channels, 68 keys a row: 393 to 462 us).  A kernel of its own (FEW),
+// since its registers cost long rows 3 to 5 % (131072 tokens 774 us against 751, 16384
+// of 128 channels 577 against 551): taken where the window is that short, or the
+// sequences are on average.
+constexpr int kFewKeys = kFwKeys;
+__host__ __device__ __forceinline__ bool few_keys(const WindowParams& p, long long lk) {
+  const long long reach = (long long)p.left + p.right + 1 + p.sinks;
+  return (lk < reach ? lk : reach) <= kFewKeys;
+}
+
 template <int D>
 struct FwSmem {
   static constexpr int QT = TileShape<D>::bytes(128), KT = TileShape<D>::bytes(kFwKeys);
@@ -60,7 +75,7 @@ struct FwSmem {
   static_assert(OFF_BAR % 8 == 0 && ALLOC <= 227 * 1024, "shared memory budget");
 };
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool FEW>
 __global__ void __launch_bounds__(kFwThreads, 1)
     window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                       const __grid_constant__ CUtensorMap tm_v, const WindowParams p, const int n_items) {
@@ -112,7 +127,8 @@ __global__ void __launch_bounds__(kFwThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // TMEM columns: S of row tile u, buffer i [128 u + 64 i, +64) with P over its first half; O [256 + u D, +D)
+  // TMEM columns: S of row tile u, buffer i [128 u + 64 i, +64) with P over its first half (and its remainder over the
+  // second, few_keys); O [256 + u D, +D)
 
   if (warp == 10) {
     // ------------------------------ producer ------------------------------
@@ -193,6 +209,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
       const int st_q = u * L::NQ + nq % L::NQ;
       const uint32_t q_base = smem_u32(sQ + st_q * L::QT);
       const int a = it.a[u], b = it.b[u];
+      const bool few = FEW && few_keys(p, it.lk);
       // sinks of their own tile: only as many columns as they need
       auto cols_of = [&](int t) { return t < it.sep ? min(kFwKeys, (p.sinks - t * kFwKeys + 31) / 32 * 32) : kFwKeys; };
       auto wait_slot = [&](int j) { return wait_phase(&kv_full[j % L::NS], (j / L::NS) & 1, abort_flag, p.err); };
@@ -239,6 +256,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
         if (elect_one()) {
           const uint32_t v_base = smem_u32(sKV + st * L::KT);
           mma_sum<D, kFwKeys>(tm_o, tm_s + 64 * (np & 1), v_base, idesc_o, t > a, cols / 16);
+          if (few) mma_sum<D, kFwKeys>(tm_o, tm_s + 64 * (np & 1) + 32, v_base, idesc_o, true, cols / 16);
           umma_commit(&pv_done[2 * u + (np & 1)]);
           umma_commit(&kv_empty[st]);
         }
@@ -322,6 +340,7 @@ __global__ void __launch_bounds__(kFwThreads, 1)
         break;
       }
       const int a = it.a[u], b = it.b[u];
+      const bool few = FEW && few_keys(p, it.lk);
       const bool live = t_row < it.n[u] && t_row < TT;
       const long long orow = live ? (long long)(it.tok + u * TT + t_row) * p.hq + it.hk * G + g : -1;
       const RowView<kFwKeys> view(p, it, it.pos + u * TT + t_row, live, 0, kFwKeys);
@@ -396,12 +415,23 @@ __global__ void __launch_bounds__(kFwThreads, 1)
               e.y = ex2(e.y);
               l2[(i >> 1) & 1] = add2(l2[(i >> 1) & 1], e);
               w[i / 2] = pack2<BF16>(e.x, e.y);
+              if (FEW) s[c][i] = e.x, s[c][i + 1] = e.y;
             }
           } else {
 #pragma unroll
             for (int i = 0; i < 16; ++i) w[i] = 0u;
           }
           tmem_st16(tm_s + 16 * c, w);
+          if (few) {
+            if (some[c]) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                const float2 h = unpack2<BF16>(w[i / 2]);
+                w[i / 2] = pack2<BF16>(s[c][i] - h.x, s[c][i + 1] - h.y);
+              }
+            }
+            tmem_st16(tm_s + 32 + 16 * c, w);
+          }
         }
         tmem_wait_st();
         tc_fence_before();
@@ -440,10 +470,14 @@ int launch_fwd(const WindowParams& p, cudaStream_t s) {
   if ((rc = make_tmap_3d(&mv, v, D, p.hkv, p.total_k, p.total_k ? p.v_stride : p.q_stride, 1, kFwKeys, S::kCols))) return rc;
   const int n_items = tile_slots(p.total_q, p.num_seqs, 2 * tt) * p.hkv;
   const int grid = std::min(n_items, num_sms());
-  LSRM_CUDA_TRY(cudaFuncSetAttribute(window_fwd_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC));
-  window_fwd_kernel<D, BF16><<<grid, kFwThreads, L::ALLOC, s>>>(mq, mk, mv, p, n_items);
-  LSRM_LAUNCH_CHECK();
-  return LSRM_OK;
+  auto launch = [&](auto kernel) {
+    LSRM_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::ALLOC));
+    kernel<<<grid, kFwThreads, L::ALLOC, s>>>(mq, mk, mv, p, n_items);
+    LSRM_LAUNCH_CHECK();
+    return LSRM_OK;
+  };
+  const bool few = few_keys(p, p.total_k / std::max(p.num_seqs, 1));
+  return few ? launch(window_fwd_kernel<D, BF16, true>) : launch(window_fwd_kernel<D, BF16, false>);
 }
 
 }  // namespace

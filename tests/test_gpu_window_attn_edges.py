@@ -165,3 +165,51 @@ def test_delta_does_not_inherit_the_outputs_rounding(dtype):
     predicted = moved[rows].norm().item()
     assert 0.7 * predicted <= err["without"] <= 1.4 * predicted
     assert err["with"] <= 0.35 * predicted
+
+
+FEW = [
+    # lens, Hq, Hkv, D, window, sinks, causal
+    ([81, 40], 1, 1, 32, 1, 7, False),
+    ([1005], 2, 2, 64, 8, 7, True),
+    ([1, 2, 3, 9, 40, 64, 33, 50], 16, 8, 64, 3000, 1, True),
+    ([5, 17, 64, 3], 64, 4, 64, 3000, 16, False),
+    ([700, 130], 6, 2, 128, 20, 40, True),   # the sinks in a tile of their own
+    ([900], 4, 1, 32, 40, 23, False),        # 20 + 20 + 1 + 23 keys: the most that counts as few
+    ([466, 30], 8, 1, 128, 50, 14, True),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens,hq,hkv,d,window,sinks,causal", FEW)
+def test_rows_of_few_keys_keep_what_rounding_p_leaves_over(lens, hq, hkv, d, window, sinks, causal, dtype):
+    """Up to 64 keys a row, P enters the output's product unrounded to 2^-16: out is off by its own rounding, and dq and
+    dk by dS's and theirs.  Scores of some units from sums of up to 128 products in 32 bits, and the exponentials, are
+    within 2^-17."""
+    u = oracle.UNIT[dtype]
+    tiny = 2.0**-25 if dtype == torch.float16 else 0.0
+    rel, left = 2.0**-17, 2.0**-16
+    cu = _cu(lens)
+    n = int(cu[-1])
+    q, k, v, do = _inputs(n, n, hq, hkv, d, dtype, seed=18)
+    got = _run(q, k, v, do, cu, cu, window=window, sinks=sinks, causal=causal)
+    ref = oracle.attention(q, k, v, cu, cu, window, sinks, causal, dout=do)
+    bound = {x: u * ref[x].abs() + tiny for x in ("out", "dq", "dk")}
+    scale = d**-0.5
+    at = 0
+    for length in lens:
+        s = slice(at, at + length)
+        at += length
+        vis = oracle.visible(length, length, window, sinks, causal, "cuda")
+        for h in range(hq):
+            qq, kk, vv, dd = q[s, h].double(), k[s, h // (hq // hkv)].double(), v[s, h // (hq // hkv)].double(), do[s, h].double()
+            p = torch.softmax((qq @ kk.T * scale).masked_fill(~vis, -math.inf), 1)
+            spread = p @ vv.abs()
+            bound["out"][s, h] += (left + rel) * spread + tiny * (vis.double() @ vv.abs())
+            dp, delta = dd @ vv.T, (dd * ref["out"][s, h]).sum(1, keepdim=True)
+            big = (dd.abs() * spread).sum(1, keepdim=True)
+            ds = u * (p * (dp - delta)).abs() + p * ((left + rel) * big + 2 * rel * (dd.abs() @ vv.abs().T + big)) + tiny * vis
+            bound["dq"][s, h] += ds @ kk.abs() * scale
+            bound["dk"][s, h // (hq // hkv)] += ds.T @ qq.abs() * scale
+    for x in ("out", "dq", "dk"):
+        over = ((got[x].double() - ref[x]).abs() - bound[x]).max().item()
+        assert over <= 1e-12, f"{x}: {over:.3g} beyond the bound"
